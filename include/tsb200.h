@@ -532,6 +532,60 @@ int tsb_to_dense_fwd(const void* feats, const int32_t* coords, int64_t n, int32_
 int tsb_to_dense_bwd(const void* grad_dense, const int32_t* coords, int64_t n, int32_t c,
                      const int32_t* range, int32_t dtype, void* grad_feats, tsb_stream_t stream);
 
+/* ---------------------------------------------------------------- rows grouped by an index
+ * No counterpart in the reference's pybind module.  Sums over the rows of a group run in a fixed order: the same call
+ * gives the same bits. */
+
+/* Stable grouping of n keys (int32, or int64 when keys_are_i64, `stride` elements apart) into n_groups groups:
+ * order int32 [n] = the row at each grouped position, inverse int32 [n] (may be NULL) = the position of each row,
+ * offsets int32 [n_groups + 1] = first position of each group.  Keys outside [0, n_groups) come last, in their order,
+ * from position offsets[n_groups] on.  n, n_groups < 2^31. */
+size_t tsb_group_rows_workspace_bytes(int64_t n, int64_t n_groups);
+int tsb_group_rows(const void* keys, int32_t keys_are_i64, int64_t stride, int64_t n, int64_t n_groups, int32_t* order,
+                   int32_t* inverse, int32_t* offsets, void* workspace, size_t workspace_bytes, tsb_stream_t stream);
+
+/* Group norm with an activation over the rows of each sample, channels last: x, y [n, c] of `dtype`, g groups of
+ * c / g channels, sample s = the grouped positions offsets[s] .. offsets[s + 1] (int32 [b + 1], ascending), order int32
+ * [n] = the row at each position (NULL: the rows are grouped already).  weight, bias [c] of `param_dtype` or NULL.
+ * act: 0 none, 1 ReLU, 2 leaky ReLU with `slope`, 3 SiLU.  Rows of no sample become zero.  mean, rstd: fp32 [b, g],
+ * what the backward call needs.  A group of one value becomes act(bias).  c <= 65536.
+ * Replaces the loop of torchsparse/nn/modules/norm.py:25-57. */
+size_t tsb_group_norm_fwd_workspace_bytes(int64_t n, int64_t c, int64_t g, int64_t b);
+int tsb_group_norm_fwd(const void* x, const int32_t* order, const int32_t* offsets, const void* weight, const void* bias,
+                       int64_t n, int64_t c, int64_t g, int64_t b, float eps, int32_t act, float slope, int32_t dtype,
+                       int32_t param_dtype, void* y, float* mean, float* rstd, void* workspace, size_t workspace_bytes,
+                       tsb_stream_t stream);
+/* Its gradient: dx [n, c] of `dtype`, dweight and dbias [c] of `param_dtype` (either may be NULL). */
+size_t tsb_group_norm_bwd_workspace_bytes(int64_t n, int64_t c, int64_t g, int64_t b);
+int tsb_group_norm_bwd(const void* x, const void* dy, const int32_t* order, const int32_t* offsets, const void* weight,
+                       const void* bias, const float* mean, const float* rstd, int64_t n, int64_t c, int64_t g, int64_t b,
+                       int32_t act, float slope, int32_t dtype, int32_t param_dtype, void* dx, void* dweight, void* dbias,
+                       void* workspace, size_t workspace_bytes, tsb_stream_t stream);
+
+/* out[i] = scale * table[tokens[i]] (table [n_rows, c], out [n, c], of `dtype`); a token that is no row gives zeros. */
+int tsb_embedding_fwd(const void* table, const void* tokens, int32_t tokens_are_i64, int64_t n, int64_t n_rows, int64_t c,
+                      float scale, int32_t dtype, void* out, tsb_stream_t stream);
+/* dtable [n_rows, c] (fully written) = scale * the sum of grad[i] over the rows of each token, accumulated in fp32 in
+ * the order of i and rounded once; the row `padding_row` (-1: none) gets zeros. */
+size_t tsb_embedding_bwd_workspace_bytes(int64_t n, int64_t n_rows, int64_t c, int32_t dtype);
+int tsb_embedding_bwd(const void* grad, const void* tokens, int32_t tokens_are_i64, int64_t n, int64_t n_rows, int64_t c,
+                      float scale, int64_t padding_row, int32_t dtype, void* dtable, void* workspace, size_t workspace_bytes,
+                      tsb_stream_t stream);
+
+/* Rows sorted by expert and back.  `inverse` int32 [n, k] and `kept` (device int32: the number of choices that have an
+ * expert, offsets[n_groups]) come from tsb_group_rows over the n * k choices.
+ * dispatch: xs[inverse[i][j]] = x[i], zeros at and behind *kept.  combine: out[i] = the sum over j of
+ * weights[i][j] * rows[inverse[i][j]] (weights NULL: 1; choices without an expert add nothing).  combine_bwd:
+ * drows[inverse[i][j]] = weights[i][j] * dout[i], dweights[i][j] = <dout[i], rows[inverse[i][j]]>, zeros for choices
+ * without an expert.  Products and sums in fp32.  n * k < 2^31. */
+int tsb_expert_dispatch(const void* x, const int32_t* inverse, const int32_t* kept, int64_t n, int32_t k, int64_t c,
+                        int32_t dtype, void* xs, tsb_stream_t stream);
+int tsb_expert_combine(const void* rows, const void* weights, int32_t weights_dtype, const int32_t* inverse,
+                       const int32_t* kept, int64_t n, int32_t k, int64_t c, int32_t dtype, void* out, tsb_stream_t stream);
+int tsb_expert_combine_bwd(const void* dout, const void* rows, const void* weights, int32_t weights_dtype,
+                           const int32_t* inverse, const int32_t* kept, int64_t n, int32_t k, int64_t c, int32_t dtype,
+                           void* drows, void* dweights, tsb_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

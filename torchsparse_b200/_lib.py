@@ -15,6 +15,7 @@ P = C.c_void_p
 I32 = C.c_int32
 I64 = C.c_int64
 SZ = C.c_size_t
+F32 = C.c_float
 
 # name -> (restype, argtypes); mirrors include/tsb200.h declaration by declaration
 SIGNATURES = {
@@ -80,6 +81,18 @@ SIGNATURES = {
     "tsb_devoxelize_bwd": (C.c_int, [P, P, P, I64, I64, I32, P, P]),
     "tsb_to_dense_fwd": (C.c_int, [P, P, I64, I32, P, I32, P, P]),
     "tsb_to_dense_bwd": (C.c_int, [P, P, I64, I32, P, I32, P, P]),
+    "tsb_group_rows_workspace_bytes": (SZ, [I64, I64]),
+    "tsb_group_rows": (C.c_int, [P, I32, I64, I64, I64, P, P, P, P, SZ, P]),
+    "tsb_group_norm_fwd_workspace_bytes": (SZ, [I64, I64, I64, I64]),
+    "tsb_group_norm_fwd": (C.c_int, [P, P, P, P, P, I64, I64, I64, I64, F32, I32, F32, I32, I32, P, P, P, P, SZ, P]),
+    "tsb_group_norm_bwd_workspace_bytes": (SZ, [I64, I64, I64, I64]),
+    "tsb_group_norm_bwd": (C.c_int, [P, P, P, P, P, P, P, P, I64, I64, I64, I64, I32, F32, I32, I32, P, P, P, P, SZ, P]),
+    "tsb_embedding_fwd": (C.c_int, [P, P, I32, I64, I64, I64, F32, I32, P, P]),
+    "tsb_embedding_bwd_workspace_bytes": (SZ, [I64, I64, I64, I32]),
+    "tsb_embedding_bwd": (C.c_int, [P, P, I32, I64, I64, I64, F32, I64, I32, P, P, SZ, P]),
+    "tsb_expert_dispatch": (C.c_int, [P, P, P, I64, I32, I64, I32, P, P]),
+    "tsb_expert_combine": (C.c_int, [P, P, I32, P, P, I64, I32, I64, I32, P, P]),
+    "tsb_expert_combine_bwd": (C.c_int, [P, P, P, I32, P, P, I64, I32, I64, I32, P, P, P]),
 }
 
 class IgemmDesc(C.Structure):

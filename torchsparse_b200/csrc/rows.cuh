@@ -1,0 +1,95 @@
+// Shared by the operators over grouped rows (rows.cu, norm.cu): vector loads and stores of feature rows, the
+// activations and the parameter loads whose type is only known at run time.
+#pragma once
+
+#include "common.cuh"
+
+namespace tsb {
+
+template <int BYTES>
+struct RawOf;
+template <>
+struct RawOf<16> { using type = uint4; };
+template <>
+struct RawOf<8> { using type = uint2; };
+template <>
+struct RawOf<4> { using type = unsigned; };
+template <>
+struct RawOf<2> { using type = unsigned short; };
+
+// VEC neighbouring values of a row, moved as one load or store of VEC * sizeof(T) bytes
+template <typename T, int VEC>
+struct Pack {
+  using Raw = typename RawOf<(int)sizeof(T) * VEC>::type;
+  Raw raw;
+  __device__ __forceinline__ void load(const T* p) { raw = __ldg(reinterpret_cast<const Raw*>(p)); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Raw*>(p) = raw; }
+  __device__ __forceinline__ void clear() { raw = Raw{}; }
+  __device__ __forceinline__ void get(float (&v)[VEC]) const {
+    const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = to_f32(e[i]);
+  }
+  __device__ __forceinline__ void set(const float (&v)[VEC]) {
+    T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) e[i] = from_f32<T>(v[i]);
+  }
+};
+
+// Largest vector (in elements, up to 16 bytes) that divides a row of c elements and to which every base pointer is
+// aligned; `bits` is the OR of the pointers.
+inline int vector_width(int dtype, int64_t c, uintptr_t bits) {
+  const int size = (int)dtype_size(dtype);
+  for (int bytes = 16; bytes > size; bytes >>= 1)
+    if (((c * size) % bytes == 0) && (bits % bytes == 0)) return bytes / size;
+  return 1;
+}
+
+template <typename T_, int VEC_>
+struct PackTag {
+  using T = T_;
+  static constexpr int VEC = VEC_;
+};
+
+// f(PackTag<T, VEC>()) for the type and vector width found at run time
+template <typename F>
+inline int dispatch_pack(int dtype, int vec, F&& f) {
+  switch (dtype) {
+    case TSB_F32:
+      switch (vec) {
+        case 4: return f(PackTag<float, 4>());
+        case 2: return f(PackTag<float, 2>());
+        default: return f(PackTag<float, 1>());
+      }
+    case TSB_F16:
+      switch (vec) {
+        case 8: return f(PackTag<__half, 8>());
+        case 4: return f(PackTag<__half, 4>());
+        case 2: return f(PackTag<__half, 2>());
+        default: return f(PackTag<__half, 1>());
+      }
+    case TSB_BF16:
+      switch (vec) {
+        case 8: return f(PackTag<__nv_bfloat16, 8>());
+        case 4: return f(PackTag<__nv_bfloat16, 4>());
+        case 2: return f(PackTag<__nv_bfloat16, 2>());
+        default: return f(PackTag<__nv_bfloat16, 1>());
+      }
+  }
+  return TSB_ERR_UNSUPPORTED;
+}
+
+// One value of an array whose type is a run-time argument (parameters, router weights: few values, read once).
+__device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
+  if (dtype == TSB_F32) return __ldg(reinterpret_cast<const float*>(p) + i);
+  if (dtype == TSB_F16) return to_f32(reinterpret_cast<const __half*>(p)[i]);
+  return to_f32(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+}
+__device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float v) {
+  if (dtype == TSB_F32) reinterpret_cast<float*>(p)[i] = v;
+  else if (dtype == TSB_F16) reinterpret_cast<__half*>(p)[i] = from_f32<__half>(v);
+  else reinterpret_cast<__nv_bfloat16*>(p)[i] = from_f32<__nv_bfloat16>(v);
+}
+
+}  // namespace tsb

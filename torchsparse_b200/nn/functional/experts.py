@@ -1,0 +1,77 @@
+from typing import NamedTuple
+
+import torch
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from ... import backend
+
+__all__ = ["ExpertRows", "expert_sort", "expert_dispatch", "expert_combine"]
+
+
+class ExpertRows(NamedTuple):
+    """The N * k choices of N rows sorted by expert (all int32): ``order`` [N * k] the choice at each sorted position,
+    ``inverse`` [N, k] the position of each choice, ``offsets`` [experts + 1] the first position of each expert.
+    Choices without an expert stand behind ``offsets[-1]``."""
+
+    order: torch.Tensor
+    inverse: torch.Tensor
+    offsets: torch.Tensor
+
+
+class _Dispatch(Function):
+    @staticmethod
+    def forward(ctx, feats: torch.Tensor, inverse: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+        ctx.save_for_backward(inverse, offsets)
+        return backend.expert_dispatch_cuda(feats, inverse, offsets)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_output: torch.Tensor):
+        inverse, offsets = ctx.saved_tensors
+        return backend.expert_combine_cuda(grad_output, None, inverse, offsets), None, None
+
+
+class _Combine(Function):
+    @staticmethod
+    def forward(ctx, rows: torch.Tensor, weights: torch.Tensor, inverse: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+        ctx.save_for_backward(rows, weights, inverse, offsets)
+        return backend.expert_combine_cuda(rows, weights, inverse, offsets)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_output: torch.Tensor):
+        rows, weights, inverse, offsets = ctx.saved_tensors
+        drows, dweights = backend.expert_combine_backward_cuda(grad_output, rows, weights, inverse, offsets)
+        return drows, dweights, None, None
+
+
+def expert_sort(experts: torch.Tensor, num_experts: int) -> ExpertRows:
+    """Sort the choices of a router: ``experts`` int32 or int64 [N, k] (or [N]) names the weight matrices that row i is
+    sent to.  Choices of one expert keep their order; a choice outside [0, num_experts) (-1, say, for one dropped for
+    want of room) goes to no expert."""
+    if experts.dim() not in (1, 2):
+        raise ValueError(f"experts must be [N, k] or [N], not {tuple(experts.shape)}")
+    if experts.dim() == 1:
+        experts = experts[:, None]
+    if experts.shape[1] < 1:
+        raise ValueError("every row needs at least one choice")
+    order, inverse, offsets = backend.group_rows_cuda(experts.reshape(-1), num_experts, want_inverse=True)
+    return ExpertRows(order, inverse.view(experts.shape), offsets)
+
+
+def expert_dispatch(feats: torch.Tensor, rows: ExpertRows) -> torch.Tensor:
+    """[N * k, C]: the rows of ``feats`` sorted by expert, those of expert e at positions ``offsets[e]`` to
+    ``offsets[e + 1]``; zeros behind the last expert.  The gradient adds up a row's k copies in their order."""
+    if torch.is_grad_enabled() and feats.requires_grad:
+        return _Dispatch.apply(feats, rows.inverse, rows.offsets)
+    return backend.expert_dispatch_cuda(feats, rows.inverse, rows.offsets)
+
+
+def expert_combine(feats: torch.Tensor, weights: torch.Tensor, rows: ExpertRows) -> torch.Tensor:
+    """[N, C]: row i is the sum over its choices of ``weights[i, j]`` times the sorted row of that choice (``feats``
+    [N * k, C], what the experts made of the dispatched rows); a choice without an expert adds nothing.  Products and
+    sums are fp32.  ``weights`` fp32, fp16 or bf16 [N, k]."""
+    if torch.is_grad_enabled() and (feats.requires_grad or weights.requires_grad):
+        return _Combine.apply(feats, weights, rows.inverse, rows.offsets)
+    return backend.expert_combine_cuda(feats, weights, rows.inverse, rows.offsets)

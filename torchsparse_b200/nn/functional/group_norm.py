@@ -1,0 +1,72 @@
+from typing import NamedTuple, Optional
+
+import torch
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from ... import backend
+from ...tensor import SparseTensor
+
+__all__ = ["RowGroups", "group_rows", "sample_rows", "group_norm"]
+
+
+class RowGroups(NamedTuple):
+    """Rows grouped by an index (both int32): ``order`` [N] the row at each grouped position, ``offsets`` [groups + 1]
+    the first position of each group.  Rows of no group stand behind ``offsets[-1]``."""
+
+    order: torch.Tensor
+    offsets: torch.Tensor
+
+
+def group_rows(keys: torch.Tensor, num_groups: int) -> RowGroups:
+    """Group rows by ``keys`` (int32 or int64 [N]); rows of one group keep their order, a key outside
+    [0, num_groups) belongs to no group."""
+    order, _, offsets = backend.group_rows_cuda(keys, num_groups)
+    return RowGroups(order, offsets)
+
+
+def sample_rows(input: SparseTensor, batch_size: Optional[int] = None) -> RowGroups:
+    """The rows of a tensor grouped by batch sample.  Without ``batch_size`` the largest batch index is read from the
+    device.  The result serves every layer on the same coordinates."""
+    batch = input.coords[:, 0]
+    if batch_size is None:
+        batch_size = int(batch.max().item()) + 1 if batch.numel() else 0
+    return group_rows(batch, max(int(batch_size), 1))
+
+
+class _GroupNorm(Function):
+    """Group norm with an activation (torchsparse/nn/modules/norm.py:25-57) and its gradient."""
+
+    @staticmethod
+    def forward(ctx, feats, weight, bias, offsets, order, num_groups, eps, activation, negative_slope):
+        y, mean, rstd = backend.group_norm_forward_cuda(feats, order, offsets, num_groups, weight, bias, eps, activation,
+                                                        negative_slope)
+        ctx.save_for_backward(feats, weight, bias, offsets, order, mean, rstd)
+        ctx.args = num_groups, activation, negative_slope
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_output: torch.Tensor):
+        feats, weight, bias, offsets, order, mean, rstd = ctx.saved_tensors
+        num_groups, activation, negative_slope = ctx.args
+        dx, dweight, dbias = backend.group_norm_backward_cuda(feats, grad_output, order, offsets, num_groups, weight, bias,
+                                                              mean, rstd, activation, negative_slope)
+        return dx, dweight, dbias, None, None, None, None, None, None
+
+
+def group_norm(feats: torch.Tensor, offsets: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] = None,
+               bias: Optional[torch.Tensor] = None, eps: float = 1e-5, activation: Optional[str] = None,
+               negative_slope: float = 0.01, order: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``act(group_norm(feats))`` over the rows of each sample, features [N, C] (fp32, fp16 or bf16).
+
+    ``offsets`` int32 [samples + 1], ascending: sample s is rows ``offsets[s]`` to ``offsets[s + 1]``, or, with
+    ``order`` int32 [N], the rows ``order[offsets[s] : offsets[s + 1]]`` (see ``group_rows``).  A sample may be empty;
+    rows of no sample become zero.  A group with one value becomes ``act(bias)``.  ``weight`` and ``bias`` [C] may have a
+    dtype of their own (fp32 beside 16-bit features).  ``activation``: None, "relu", "leaky_relu" or "silu".
+    Statistics and sums are fp32 and run in a fixed order."""
+    if torch.is_grad_enabled() and (feats.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
+        return _GroupNorm.apply(feats, weight, bias, offsets, order, num_groups, eps, activation, negative_slope)
+    return backend.group_norm_forward_cuda(feats, order, offsets, num_groups, weight, bias, eps, activation,
+                                           negative_slope)[0]
