@@ -12,12 +12,16 @@
 //
 // Variances are joined from means and sums of squares about them, piece by piece, never as a difference of two large
 // sums, in 32 bits.
+#include <type_traits>
+
 #include "rows.cuh"
 
 namespace tsb {
 namespace {
 
-constexpr int kNormThreads = 512;
+constexpr int kNormThreads = 256;
+constexpr int kNormWarps = kNormThreads / 32;
+constexpr int kNormBlocks = 3 * kSmCount;      // three blocks of 256 threads and up to 80 registers are resident on an SM
 enum { kActNone = 0, kActRelu = 1, kActLeaky = 2, kActSilu = 3 };
 
 struct Norm {
@@ -26,7 +30,6 @@ struct Norm {
   int b;                 // samples
   int cols;              // vectors of a row
   int tile;              // vectors of a row that one block takes (grid.y tiles)
-  int lanes;             // rows that a block takes at once
   int64_t chunk;         // rows of a block
   int nblk;
   const int* order;      // row at a grouped position, or null: the rows are grouped already
@@ -42,21 +45,52 @@ __device__ __forceinline__ int64_t offset_of(const Norm& a, int s) {
   return v < 0 ? 0 : v > a.n ? a.n : v;
 }
 
-// first sample that ends behind position p (a.b: none)
+// First sample that ends behind position p (a.b: none).  The whole warp searches: 32 samples per load, so that a batch of
+// usual size costs one round trip.
 __device__ __forceinline__ int first_sample(const Norm& a, int64_t p) {
-  int lo = 0, hi = a.b;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (offset_of(a, mid + 1) <= p) lo = mid + 1; else hi = mid;
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = a.b;      // samples before lo end at or before p; sample hi (if any) ends behind it
+  while (hi - lo > 32) {
+    const int step = (hi - lo + 31) / 32, at = lo + (lane + 1) * step - 1;
+    const bool before = at < hi && offset_of(a, at + 1) <= p;
+    const int k = __popc(__ballot_sync(0xffffffffu, before));
+    hi = min(hi, lo + (k + 1) * step - 1);
+    lo += k * step;
   }
-  return lo;
+  const bool before = lo + lane < hi && offset_of(a, lo + lane + 1) <= p;
+  return lo + __popc(__ballot_sync(0xffffffffu, before));
 }
 
-// row at a grouped position, -1 for an entry of a caller's order that is no row
+// Row at a grouped position; -1 for an entry of a caller's order that is no row.
+template <bool ORDERED>
 __device__ __forceinline__ int64_t row_at(const Norm& a, int64_t p) {
-  if (!a.order) return p;
+  if constexpr (!ORDERED) return p;
   const int64_t r = __ldg(a.order + p);
   return r >= 0 && r < a.n ? r : -1;
+}
+
+// Byte offsets of U rows, `step` positions apart from p on; -1 for those at or beyond `end` (below it when step is
+// negative: `end` is then the first position that still counts).
+template <bool ORDERED, int U>
+__device__ __forceinline__ void rows_at(const Norm& a, int64_t p, int step, int64_t end, int64_t (&at)[U]) {
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t q = p + u * step;
+    const bool in = step > 0 ? q < end : q >= end;
+    int64_t r = -1;
+    if (in) r = row_at<ORDERED>(a, q);
+    at[u] = r < 0 ? -1 : r * a.c;
+  }
+}
+
+// 1 / (1 + 2^(-z log2 e)) with the hardware's exponential and reciprocal, each good to 2^-22: half the instructions of the
+// library's forms, which also serve subnormal arguments (here 2^x below 2^-126 vanishes beside the 1, and beyond 2^126
+// the quotient is below 2^-126 and becomes zero).
+__device__ __forceinline__ float sigmoid(float z) {
+  float e, p;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(1.f + e));
+  return p;
 }
 
 template <int N>
@@ -69,7 +103,7 @@ __device__ __forceinline__ void activate(float (&z)[N], int act, float slope) {
     for (int i = 0; i < N; ++i) z[i] = z[i] > 0.f ? z[i] : z[i] * slope;
   } else if (act == kActSilu) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) z[i] = z[i] / (1.f + __expf(-z[i]));
+    for (int i = 0; i < N; ++i) z[i] *= sigmoid(z[i]);
   }
 }
 
@@ -85,8 +119,8 @@ __device__ __forceinline__ void activate_grad(const float (&z)[N], float (&g)[N]
   } else if (act == kActSilu) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float p = 1.f / (1.f + __expf(-z[i]));
-      g[i] *= p * (1.f + z[i] * (1.f - p));
+      const float p = sigmoid(z[i]);
+      g[i] *= fmaf(z[i] * p, 1.f - p, p);
     }
   }
 }
@@ -107,75 +141,90 @@ __device__ __forceinline__ int tile_channels(const Norm& a, int vec, int y, int 
 }
 
 // ------------------------------------------------------------------------------------------------ statistics
-// A thread holds the mean and the sum of squares about it of the values that it has seen: one pair where a vector lies in
-// one group (A == 1), one pair per channel otherwise (A == VEC).  U rows are read together; their own mean and squares
-// are exact to rounding and are joined to the running pair.
-template <typename T, int VEC, int A>
-__global__ void __launch_bounds__(kNormThreads) norm_stats_kernel(Norm a, const T* __restrict__ x, float2* __restrict__ slots) {
+// The mean and the sum of squares about it of the values that a thread has seen: one pair where a vector lies in one
+// group (A == 1), one pair per channel otherwise (A == VEC).
+template <int VEC, int A>
+struct Running {
+  static constexpr int W = VEC / A;
+  float n, mean[A], m2[A];
+  __device__ __forceinline__ void clear() {
+    n = 0.f;
+#pragma unroll
+    for (int i = 0; i < A; ++i) mean[i] = m2[i] = 0.f;
+  }
+  // U vectors at once: their own mean and squares are exact to rounding and are joined to the running pair
+  template <typename T, int U>
+  __device__ __forceinline__ void add(const Pack<T, VEC> (&v)[U]) {
+    constexpr float kCount = (float)(U * W), kInv = 1.f / kCount;      // W values of a vector share a pair
+    float sum[A], sq[A];
+#pragma unroll
+    for (int i = 0; i < A; ++i) sum[i] = sq[i] = 0.f;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float f[VEC];
+      v[u].get(f);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) sum[e / W] += f[e];
+    }
+#pragma unroll
+    for (int i = 0; i < A; ++i) sum[i] *= kInv;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float f[VEC];
+      v[u].get(f);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float t = f[e] - sum[e / W];
+        sq[e / W] = fmaf(t, t, sq[e / W]);
+      }
+    }
+    const float all = n + kCount, share = __fdividef(kCount, all), cross = n * share;
+#pragma unroll
+    for (int i = 0; i < A; ++i) {
+      const float t = sum[i] - mean[i];
+      mean[i] = fmaf(t, share, mean[i]);
+      m2[i] += fmaf(t * t, cross, sq[i]);
+    }
+    n = all;
+  }
+};
+
+template <typename T, int VEC, int A, bool ORDERED>
+__global__ void __launch_bounds__(kNormThreads, 3) norm_stats_kernel(Norm a, const T* __restrict__ x, float2* __restrict__ slots) {
   __shared__ float2 part[A * kNormThreads];
   const int first = blockIdx.y * a.tile, width = min(a.tile, a.cols - first);
   const int lane = threadIdx.x / width, col = threadIdx.x - lane * width;
   const int lanes = kNormThreads / width;
   const int64_t p0 = blockIdx.x * a.chunk, p1 = min(p0 + a.chunk, a.n);
+  const T* xc = x + (int64_t)(first + col) * VEC;
   for (int s = first_sample(a, p0); s < a.b; ++s) {
     const int64_t begin = offset_of(a, s);
     if (begin >= p1) break;
     const int64_t lo = max(p0, begin), hi = min(p1, offset_of(a, s + 1));
     if (lo >= hi) continue;
-    float n = 0.f, mean[A], m2[A];
-#pragma unroll
-    for (int i = 0; i < A; ++i) mean[i] = m2[i] = 0.f;
     if (lane < lanes) {
       constexpr int U = 4;
-      const int64_t at = (int64_t)(first + col) * VEC;
-      for (int64_t p = lo + lane; p < hi; p += (int64_t)lanes * U) {
+      Running<VEC, A> run;
+      run.clear();
+      int64_t p = lo + lane;
+      for (; p + (U - 1) * lanes < hi; p += U * lanes) {
         Pack<T, VEC> v[U];
-        int got = 0;
+        int64_t at[U];
+        rows_at<ORDERED>(a, p, lanes, hi, at);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int64_t q = p + (int64_t)u * lanes;
-          v[u].clear();
-          if (q < hi) {
-            const int64_t r = row_at(a, q);
-            if (r >= 0) v[u].load(x + r * a.c + at);
-            ++got;
-          }
+          if (!ORDERED || at[u] >= 0) v[u].load(xc + at[u]); else v[u].clear();
         }
-        constexpr int W = VEC / A;
-        const float cnt = (float)(got * W), inv = 1.f / cnt, all = n + cnt, share = cnt / all;
-        float sum[A], sq[A];
-#pragma unroll
-        for (int i = 0; i < A; ++i) sum[i] = sq[i] = 0.f;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          float f[VEC];
-          v[u].get(f);      // zeros beyond the end
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) sum[e / W] += f[e];
-        }
-#pragma unroll
-        for (int i = 0; i < A; ++i) sum[i] *= inv;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (u >= got) continue;
-          float f[VEC];
-          v[u].get(f);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const float t = f[e] - sum[e / W];
-            sq[e / W] = fmaf(t, t, sq[e / W]);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < A; ++i) {
-          const float t = sum[i] - mean[i];
-          mean[i] = fmaf(t, share, mean[i]);
-          m2[i] += sq[i] + t * t * n * share;
-        }
-        n = all;
+        run.add(v);
+      }
+      for (; p < hi; p += lanes) {
+        Pack<T, VEC> v[1];
+        const int64_t r = row_at<ORDERED>(a, p);
+        if (r >= 0) v[0].load(xc + r * a.c); else v[0].clear();
+        run.add(v);
       }
 #pragma unroll
-      for (int i = 0; i < A; ++i) part[i * kNormThreads + threadIdx.x] = make_float2(mean[i], m2[i]);
+      for (int i = 0; i < A; ++i) part[i * kNormThreads + threadIdx.x] = make_float2(run.mean[i], run.m2[i]);
     }
     __syncthreads();
     // one warp per group of this column tile
@@ -183,7 +232,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_stats_kernel(Norm a, const 
     const int g_lo = c_lo / a.d, g_hi = (c_hi - 1) / a.d;
     const int64_t rows = hi - lo;
     float2* slot = slots + ((int64_t)blockIdx.y * (a.nblk + a.b) + blockIdx.x + s) * a.g;
-    for (int gr = g_lo + (threadIdx.x >> 5); gr <= g_hi; gr += kNormThreads / 32) {
+    for (int gr = g_lo + (threadIdx.x >> 5); gr <= g_hi; gr += kNormWarps) {
       const int k_lo = max(gr * a.d, c_lo), k_hi = min((gr + 1) * a.d, c_hi);
       const int per_lane = (k_hi - k_lo) / (VEC / A), entries = per_lane * lanes;
       float w = 0.f, m = 0.f, q = 0.f;
@@ -193,7 +242,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_stats_kernel(Norm a, const 
           const int l = t / per_lane, k = k_lo + (t - l * per_lane) * (VEC / A) - c_lo;
           const float cnt = (float)lane_rows(rows, lanes, l) * (VEC / A);
           if (cnt == 0.f) continue;
-          const float2 e = part[(A == 1 ? 0 : k % VEC) * kNormThreads + l * width + k / VEC];
+          const float2 e = part[k % VEC / (VEC / A) * kNormThreads + l * width + k / VEC];
           if (pass == 0) {
             w += cnt;
             acc = fmaf(cnt, e.x, acc);
@@ -230,9 +279,11 @@ __global__ void __launch_bounds__(128) norm_join_kernel(Norm a, int vec, int til
         for (int y = 0; y < tiles; ++y) {
           const int width = tile_channels(a, vec, y, gr);
           if (width == 0) continue;
+          const float2* at = slots + ((int64_t)y * (a.nblk + a.b) + s) * a.g + gr;
+#pragma unroll 4
           for (int j = j0 + lane; j <= j1; j += 32) {
             const float cnt = (float)(min(end, (j + 1) * a.chunk) - max(begin, j * a.chunk)) * width;
-            const float2 e = slots[((int64_t)y * (a.nblk + a.b) + j + s) * a.g + gr];
+            const float2 e = at[(int64_t)j * a.g];
             if (pass == 0) {
               w += cnt;
               acc = fmaf(cnt, e.x, acc);
@@ -257,109 +308,130 @@ __global__ void __launch_bounds__(128) norm_join_kernel(Norm a, int vec, int til
   }
 }
 
-// What a thread needs of its VEC channels within one sample.
-template <int VEC>
+// What a thread needs of its VEC channels within one sample: z = (x - mean) * a + b with a = rstd * w.
+template <int VEC, int A>
 struct Channels {
-  float mean[VEC], rstd[VEC], w[VEC], b[VEC];
-  __device__ __forceinline__ void load(const Norm& a, int s, int k0, const float* __restrict__ mean_, const float* __restrict__ rstd_) {
+  static constexpr int W = VEC / A;
+  float mean[A], a[VEC], b[VEC];
+  __device__ __forceinline__ void load(const Norm& n, int s, int k0, const float* __restrict__ mean_, const float* __restrict__ rstd_) {
+#pragma unroll
+    for (int i = 0; i < A; ++i) mean[i] = __ldg(mean_ + (int64_t)s * n.g + (k0 + i * W) / n.d);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      const int64_t at = (int64_t)s * a.g + (k0 + e) / a.d;
-      mean[e] = __ldg(mean_ + at);
-      rstd[e] = __ldg(rstd_ + at);
-      w[e] = a.w ? load_any(a.w, a.p_dtype, k0 + e) : 1.f;
-      b[e] = a.bias ? load_any(a.bias, a.p_dtype, k0 + e) : 0.f;
+      a[e] = __ldg(rstd_ + (int64_t)s * n.g + (k0 + e / W * W) / n.d) * (n.w ? load_any(n.w, n.p_dtype, k0 + e) : 1.f);
+      b[e] = n.bias ? load_any(n.bias, n.p_dtype, k0 + e) : 0.f;
     }
   }
 };
 
-// f(row, sample, sample changed) for every row of the block's chunk that belongs to this thread's lane; the rows come last
-// chunk first, so that those read last by the pass before are still in the L2 cache.  Rows of no sample have sample -1.
-template <typename T, int VEC, typename Begin, typename Row>
-__device__ __forceinline__ void walk(const Norm& a, int lane, int lanes, Begin&& begin_sample, Row&& row) {
-  const int64_t p0 = blockIdx.x * a.chunk, p1 = min(p0 + a.chunk, a.n);
-  int64_t covered = p0;
-  for (int s = first_sample(a, p0); s < a.b; ++s) {
-    const int64_t begin = offset_of(a, s);
-    if (begin >= p1) break;
-    const int64_t lo = max(p0, begin), hi = min(p1, offset_of(a, s + 1));
-    for (int64_t p = covered + lane; p < lo; p += lanes) row(p, false);
-    if (lo >= hi) continue;
-    begin_sample(s);
-    for (int64_t p = lo + lane; p < hi; p += lanes) row(p, true);
-    covered = max(covered, hi);
+// Zeros in the rows of the block's chunk that belong to no sample.
+template <typename T, int VEC, bool ORDERED>
+__device__ __forceinline__ void clear_outside(const Norm& a, int64_t p0, int64_t p1, int lane, int lanes, T* __restrict__ out) {
+  const int64_t begin = a.b ? offset_of(a, 0) : a.n, end = a.b ? offset_of(a, a.b) : a.n;
+  if (begin <= p0 && end >= p1) return;
+  Pack<T, VEC> zero;
+  zero.clear();
+  for (int64_t p = p0 + lane; p < p1; p += lanes) {
+    if (p >= begin && p < end) continue;
+    const int64_t r = row_at<ORDERED>(a, p);
+    if (r >= 0) zero.store(out + r * a.c);
   }
-  for (int64_t p = covered + lane; p < p1; p += lanes) row(p, false);
 }
 
-template <typename T, int VEC>
-__global__ void __launch_bounds__(kNormThreads) norm_apply_kernel(Norm a, const T* __restrict__ x, const float* __restrict__ mean,
-                                                                  const float* __restrict__ rstd, T* __restrict__ y) {
+// The rows are walked from the end of the chunk to its beginning: what the statistics read last is still in the L2 cache.
+template <typename T, int VEC, int A, bool ORDERED>
+__global__ void __launch_bounds__(kNormThreads, 3) norm_apply_kernel(Norm a, const T* __restrict__ x, const float* __restrict__ mean,
+                                                                     const float* __restrict__ rstd, T* __restrict__ y) {
+  constexpr int U = 4, W = VEC / A;
   const int first = blockIdx.y * a.tile, width = min(a.tile, a.cols - first);
   const int lane = threadIdx.x / width, lanes = kNormThreads / width;
-  if (lane >= lanes) return;
   const int k0 = (first + threadIdx.x - lane * width) * VEC;
-  Channels<VEC> ch;
-  walk<T, VEC>(a, lane, lanes, [&](int s) { ch.load(a, s, k0, mean, rstd); }, [&](int64_t p, bool in) {
-    const int64_t r = row_at(a, p);
-    if (r < 0) return;
-    Pack<T, VEC> v;
-    if (in) {
-      v.load(x + r * a.c + k0);
-      float z[VEC];
-      v.get(z);
+  const int64_t p0 = blockIdx.x * a.chunk, p1 = min(p0 + a.chunk, a.n);
+  const T* xc = x + k0;
+  T* yc = y + k0;
+  const int last = min(first_sample(a, p1 - 1), a.b - 1);
+  if (lane >= lanes) return;
+  clear_outside<T, VEC, ORDERED>(a, p0, p1, lane, lanes, yc);
+  for (int s = last; s >= 0; --s) {
+    const int64_t end = offset_of(a, s + 1);
+    if (end <= p0) break;
+    const int64_t lo = max(p0, offset_of(a, s)), hi = min(p1, end);
+    if (lo >= hi) continue;
+    Channels<VEC, A> ch;
+    ch.load(a, s, k0, mean, rstd);
+    for (int64_t p = hi - 1 - lane; p >= lo; p -= U * lanes) {
+      Pack<T, VEC> v[U];
+      int64_t at[U];
+      rows_at<ORDERED>(a, p, -lanes, lo, at);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) z[e] = fmaf((z[e] - ch.mean[e]) * ch.rstd[e], ch.w[e], ch.b[e]);
-      activate(z, a.act, a.slope);
-      v.set(z);
-    } else {
-      v.clear();
+      for (int u = 0; u < U; ++u)
+        if (at[u] >= 0) v[u].load(xc + at[u]);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (at[u] < 0) continue;
+        float z[VEC];
+        v[u].get(z);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) z[e] = fmaf(z[e] - ch.mean[e / W], ch.a[e], ch.b[e]);
+        activate(z, a.act, a.slope);
+        v[u].set(z);
+        v[u].store(yc + at[u]);
+      }
     }
-    v.store(y + r * a.c + k0);
-  });
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ gradient
 // Per slot and channel: the sums of dz and of dz * xhat.
-template <typename T, int VEC>
-__global__ void __launch_bounds__(kNormThreads) norm_grad_sums_kernel(Norm a, const T* __restrict__ x, const T* __restrict__ dy,
-                                                                      const float* __restrict__ mean, const float* __restrict__ rstd,
-                                                                      float2* __restrict__ slots) {
+template <typename T, int VEC, int A, bool ORDERED>
+__global__ void __launch_bounds__(kNormThreads, 3) norm_grad_sums_kernel(Norm a, const T* __restrict__ x, const T* __restrict__ dy,
+                                                                         const float* __restrict__ mean,
+                                                                         const float* __restrict__ rstd, float2* __restrict__ slots) {
+  constexpr int U = 2, W = VEC / A;
   __shared__ float2 part[VEC * kNormThreads];
   const int first = blockIdx.y * a.tile, width = min(a.tile, a.cols - first);
   const int lane = threadIdx.x / width, lanes = kNormThreads / width, col = threadIdx.x - lane * width;
   const int k0 = (first + col) * VEC;
   const int64_t p0 = blockIdx.x * a.chunk, p1 = min(p0 + a.chunk, a.n);
+  const T *xc = x + k0, *gc = dy + k0;
   for (int s = first_sample(a, p0); s < a.b; ++s) {
     const int64_t begin = offset_of(a, s);
     if (begin >= p1) break;
     const int64_t lo = max(p0, begin), hi = min(p1, offset_of(a, s + 1));
     if (lo >= hi) continue;
-    float s1[VEC], s2[VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) s1[e] = s2[e] = 0.f;
     if (lane < lanes) {
-      Channels<VEC> ch;
+      float s1[VEC], s2[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s1[e] = s2[e] = 0.f;
+      Channels<VEC, A> ch;
       ch.load(a, s, k0, mean, rstd);
-      for (int64_t p = lo + lane; p < hi; p += lanes) {
-        const int64_t r = row_at(a, p);
-        if (r < 0) continue;
-        Pack<T, VEC> vx, vg;
-        vx.load(x + r * a.c + k0);
-        vg.load(dy + r * a.c + k0);
-        float h[VEC], z[VEC], g[VEC];
-        vx.get(h);
-        vg.get(g);
+      for (int64_t p = lo + lane; p < hi; p += U * lanes) {
+        Pack<T, VEC> vx[U], vg[U];
+        int64_t at[U];
+        rows_at<ORDERED>(a, p, lanes, hi, at);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          h[e] = (h[e] - ch.mean[e]) * ch.rstd[e];
-          z[e] = fmaf(h[e], ch.w[e], ch.b[e]);
+        for (int u = 0; u < U; ++u) {
+          if (at[u] < 0) continue;
+          vx[u].load(xc + at[u]);
+          vg[u].load(gc + at[u]);
         }
-        activate_grad(z, g, a.act, a.slope);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          s1[e] += g[e];
-          s2[e] = fmaf(g[e], h[e], s2[e]);
+        for (int u = 0; u < U; ++u) {
+          if (at[u] < 0) continue;
+          float h[VEC], z[VEC], g[VEC];
+          vx[u].get(h);
+          vg[u].get(g);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            h[e] -= ch.mean[e / W];
+            z[e] = fmaf(h[e], ch.a[e], ch.b[e]);
+          }
+          activate_grad(z, g, a.act, a.slope);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            s1[e] += g[e];
+            s2[e] = fmaf(g[e], h[e], s2[e]);
+          }
         }
       }
 #pragma unroll
@@ -368,14 +440,14 @@ __global__ void __launch_bounds__(kNormThreads) norm_grad_sums_kernel(Norm a, co
     __syncthreads();
     float2* slot = slots + ((int64_t)blockIdx.x + s) * a.c;
     for (int t = threadIdx.x; t < width * VEC; t += kNormThreads) {
-      const int e = t / width, q = t - e * width;
+      const int e = t / width, q = t - e * width, k = (first + q) * VEC + e;
       float u = 0.f, v = 0.f;
       for (int l = 0; l < lanes; ++l) {
         const float2 f = part[e * kNormThreads + l * width + q];
         u += f.x;
         v += f.y;
       }
-      slot[(first + q) * VEC + e] = make_float2(u, v);
+      slot[k] = make_float2(u, v * __ldg(rstd + (int64_t)s * a.g + k / a.d));
     }
     __syncthreads();
   }
@@ -434,50 +506,67 @@ __global__ void __launch_bounds__(kJoinThreads) norm_grad_join_kernel(Norm a, co
   }
 }
 
-template <typename T, int VEC>
-__global__ void __launch_bounds__(kNormThreads) norm_grad_apply_kernel(Norm a, const T* __restrict__ x, const T* __restrict__ dy,
-                                                                       const float* __restrict__ mean, const float* __restrict__ rstd,
-                                                                       const float2* __restrict__ by_group, T* __restrict__ dx) {
+// dx = rstd * (dz * w - m1 - xhat * m2) = dz * a - (x - mean) * k2 - k1 with k1 = rstd * m1, k2 = rstd^2 * m2
+template <typename T, int VEC, int A, bool ORDERED>
+__global__ void __launch_bounds__(kNormThreads, 3) norm_grad_apply_kernel(Norm a, const T* __restrict__ x, const T* __restrict__ dy,
+                                                                          const float* __restrict__ mean,
+                                                                          const float* __restrict__ rstd,
+                                                                          const float2* __restrict__ by_group, T* __restrict__ dx) {
+  constexpr int U = 2, W = VEC / A;
   const int first = blockIdx.y * a.tile, width = min(a.tile, a.cols - first);
   const int lane = threadIdx.x / width, lanes = kNormThreads / width;
-  if (lane >= lanes) return;
   const int k0 = (first + threadIdx.x - lane * width) * VEC;
-  Channels<VEC> ch;
-  float m1[VEC], m2[VEC];
-  walk<T, VEC>(a, lane, lanes,
-               [&](int s) {
-                 ch.load(a, s, k0, mean, rstd);
+  const int64_t p0 = blockIdx.x * a.chunk, p1 = min(p0 + a.chunk, a.n);
+  const T *xc = x + k0, *gc = dy + k0;
+  T* dc = dx + k0;
+  const int last = min(first_sample(a, p1 - 1), a.b - 1);
+  if (lane >= lanes) return;
+  clear_outside<T, VEC, ORDERED>(a, p0, p1, lane, lanes, dc);
+  for (int s = last; s >= 0; --s) {
+    const int64_t end = offset_of(a, s + 1);
+    if (end <= p0) break;
+    const int64_t lo = max(p0, offset_of(a, s)), hi = min(p1, end);
+    if (lo >= hi) continue;
+    Channels<VEC, A> ch;
+    ch.load(a, s, k0, mean, rstd);
+    float k1[A], k2[A];
 #pragma unroll
-                 for (int e = 0; e < VEC; ++e) {
-                   const float2 f = __ldg(by_group + (int64_t)s * a.g + (k0 + e) / a.d);
-                   m1[e] = f.x;
-                   m2[e] = f.y;
-                 }
-               },
-               [&](int64_t p, bool in) {
-                 const int64_t r = row_at(a, p);
-                 if (r < 0) return;
-                 Pack<T, VEC> vx, vg;
-                 if (in) {
-                   vx.load(x + r * a.c + k0);
-                   vg.load(dy + r * a.c + k0);
-                   float h[VEC], z[VEC], g[VEC];
-                   vx.get(h);
-                   vg.get(g);
+    for (int i = 0; i < A; ++i) {
+      const int64_t at = (int64_t)s * a.g + (k0 + i * W) / a.d;
+      const float2 f = __ldg(by_group + at);
+      const float r = __ldg(rstd + at);
+      k1[i] = r * f.x;
+      k2[i] = r * r * f.y;
+    }
+    for (int64_t p = hi - 1 - lane; p >= lo; p -= U * lanes) {
+      Pack<T, VEC> vx[U], vg[U];
+      int64_t at[U];
+      rows_at<ORDERED>(a, p, -lanes, lo, at);
 #pragma unroll
-                   for (int e = 0; e < VEC; ++e) {
-                     h[e] = (h[e] - ch.mean[e]) * ch.rstd[e];
-                     z[e] = fmaf(h[e], ch.w[e], ch.b[e]);
-                   }
-                   activate_grad(z, g, a.act, a.slope);
+      for (int u = 0; u < U; ++u) {
+        if (at[u] < 0) continue;
+        vx[u].load(xc + at[u]);
+        vg[u].load(gc + at[u]);
+      }
 #pragma unroll
-                   for (int e = 0; e < VEC; ++e) g[e] = ch.rstd[e] * (fmaf(g[e], ch.w[e], -m1[e]) - h[e] * m2[e]);
-                   vg.set(g);
-                 } else {
-                   vg.clear();
-                 }
-                 vg.store(dx + r * a.c + k0);
-               });
+      for (int u = 0; u < U; ++u) {
+        if (at[u] < 0) continue;
+        float h[VEC], z[VEC], g[VEC];
+        vx[u].get(h);
+        vg[u].get(g);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          h[e] -= ch.mean[e / W];
+          z[e] = fmaf(h[e], ch.a[e], ch.b[e]);
+        }
+        activate_grad(z, g, a.act, a.slope);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) g[e] = fmaf(g[e], ch.a[e], -fmaf(h[e], k2[e / W], k1[e / W]));
+        vg[u].set(g);
+        vg[u].store(dc + at[u]);
+      }
+    }
+  }
 }
 
 // dw and db: the channels' sums over the samples, in their order
@@ -514,6 +603,24 @@ int check_norm(int64_t n, int64_t c, int64_t g, int64_t b, const void* offsets, 
   return TSB_OK;
 }
 
+// f(PackTag<T, VEC>, A, ORDERED): A = 1 where a vector lies in one group, 2 where its halves do, else VEC
+template <typename F>
+int dispatch_norm(int dtype, int vec, int d, bool ordered, F&& f) {
+  return dispatch_pack(dtype, vec, [&](auto tag) -> int {
+    using T = typename decltype(tag)::T;
+    constexpr int VEC = decltype(tag)::VEC;
+    auto with = [&](auto each) -> int {
+      return ordered ? f(tag, each, std::true_type()) : f(tag, each, std::false_type());
+    };
+    if constexpr (VEC == 8) {
+      if (d % 8 != 0) return with(std::integral_constant<int, 2>());
+    } else if constexpr (VEC * sizeof(T) < 16 && VEC > 1) {
+      if (d % VEC != 0) return with(std::integral_constant<int, VEC>());
+    }
+    return with(std::integral_constant<int, 1>());
+  });
+}
+
 Norm norm_shape(int64_t n, int64_t c, int64_t g, int64_t b, int vec) {
   Norm a{};
   a.n = n;
@@ -522,10 +629,10 @@ Norm norm_shape(int64_t n, int64_t c, int64_t g, int64_t b, int vec) {
   a.d = (int)(c / g);
   a.b = (int)b;
   a.cols = (int)(c / vec);
-  a.tile = a.cols < kNormThreads ? a.cols : kNormThreads;
-  a.lanes = kNormThreads / a.tile;
-  int64_t blocks = cdiv(n, (int64_t)a.lanes * 4);      // four rows per lane at least
-  if (blocks > 2 * kSmCount) blocks = 2 * kSmCount;
+  a.tile = (int)cdiv(a.cols, cdiv(a.cols, kNormThreads));
+  const int64_t tiles = cdiv(a.cols, a.tile);
+  int64_t blocks = cdiv(n, (int64_t)(kNormThreads / a.tile) * 4);      // four rows per lane at least
+  if (blocks > cdiv(kNormBlocks, tiles)) blocks = cdiv(kNormBlocks, tiles);
   if (blocks < 1) blocks = 1;
   a.chunk = cdiv(n, blocks);
   if (a.chunk < 1) a.chunk = 1;
@@ -533,10 +640,18 @@ Norm norm_shape(int64_t n, int64_t c, int64_t g, int64_t b, int vec) {
   return a;
 }
 
+// The widest vector, or half of it (8 bytes) where 16 bytes lie in more than two groups: with a mean and a deviation for
+// each channel of the wide one the gradient kernels would spill.
+int norm_vector(int dtype, int64_t c, int64_t g, uintptr_t bits) {
+  const int vec = vector_width(dtype, c, bits);
+  const int64_t d = c / g, part = vec == 8 ? 4 : vec;
+  return vec * (int)dtype_size(dtype) == 16 && d % part != 0 ? vec / 2 : vec;
+}
+
 // slots of the forward statistics for the vector width that needs the most column tiles
 size_t fwd_slot_bytes(int64_t n, int64_t c, int64_t g, int64_t b) {
   const int64_t tiles = cdiv(c, kNormThreads);
-  return align_up((size_t)tiles * (2 * kSmCount + b) * g * sizeof(float2), 256);
+  return align_up((size_t)tiles * (kNormBlocks + b) * g * sizeof(float2), 256);
 }
 
 }  // namespace
@@ -560,7 +675,7 @@ int tsb_group_norm_fwd(const void* x, const int32_t* order, const int32_t* offse
   if ((n && (!x || !y)) || (b && (!mean || !rstd))) return TSB_ERR_BAD_ARG;
   cudaStream_t st = as_stream(stream);
   if (workspace_bytes < fwd_slot_bytes(n, c, g, b) || !workspace) return TSB_ERR_WORKSPACE;
-  const int vec = vector_width(dtype, c, (uintptr_t)x | (uintptr_t)y);
+  const int vec = norm_vector(dtype, c, g, (uintptr_t)x | (uintptr_t)y);
   Norm a = norm_shape(n, c, g, b, vec);
   a.order = order;
   a.offsets = offsets;
@@ -573,12 +688,12 @@ int tsb_group_norm_fwd(const void* x, const int32_t* order, const int32_t* offse
   float2* slots = static_cast<float2*>(workspace);
   const int tiles = (int)cdiv(a.cols, a.tile);
   const dim3 grid((unsigned)a.nblk, (unsigned)tiles);
-  return dispatch_pack(dtype, vec, [&](auto tag) -> int {
+  return dispatch_norm(dtype, vec, a.d, order != nullptr, [&](auto tag, auto each, auto ordered) -> int {
     using T = typename decltype(tag)::T;
-    constexpr int VEC = decltype(tag)::VEC;
+    constexpr int VEC = decltype(tag)::VEC, A = decltype(each)::value;
+    constexpr bool ORDERED = decltype(ordered)::value;
     if (n && b) {
-      if (a.d % VEC == 0) norm_stats_kernel<T, VEC, 1><<<grid, kNormThreads, 0, st>>>(a, (const T*)x, slots);
-      else norm_stats_kernel<T, VEC, VEC><<<grid, kNormThreads, 0, st>>>(a, (const T*)x, slots);
+      norm_stats_kernel<T, VEC, A, ORDERED><<<grid, kNormThreads, 0, st>>>(a, (const T*)x, slots);
       TSB_LAUNCH_CHECK();
     }
     if (b) {
@@ -586,7 +701,7 @@ int tsb_group_norm_fwd(const void* x, const int32_t* order, const int32_t* offse
       TSB_LAUNCH_CHECK();
     }
     if (n) {
-      norm_apply_kernel<T, VEC><<<grid, kNormThreads, 0, st>>>(a, (const T*)x, mean, rstd, (T*)y);
+      norm_apply_kernel<T, VEC, A, ORDERED><<<grid, kNormThreads, 0, st>>>(a, (const T*)x, mean, rstd, (T*)y);
       TSB_LAUNCH_CHECK();
     }
     return TSB_OK;
@@ -595,7 +710,7 @@ int tsb_group_norm_fwd(const void* x, const int32_t* order, const int32_t* offse
 
 size_t tsb_group_norm_bwd_workspace_bytes(int64_t n, int64_t c, int64_t g, int64_t b) {
   if (check_norm(n, c, g, 0, nullptr, 0, 0, 0) != TSB_OK || b < 0) return 0;
-  return align_up((size_t)(2 * kSmCount + b) * c * sizeof(float2), 256) + align_up((size_t)b * c * sizeof(float2), 256) +
+  return align_up((size_t)(kNormBlocks + b) * c * sizeof(float2), 256) + align_up((size_t)b * c * sizeof(float2), 256) +
          align_up((size_t)b * g * sizeof(float2), 256) + 256;
 }
 
@@ -608,7 +723,7 @@ int tsb_group_norm_bwd(const void* x, const void* dy, const int32_t* order, cons
   if ((n && (!x || !dy || !dx)) || (b && (!mean || !rstd))) return TSB_ERR_BAD_ARG;
   cudaStream_t st = as_stream(stream);
   if (workspace_bytes < tsb_group_norm_bwd_workspace_bytes(n, c, g, b) || !workspace) return TSB_ERR_WORKSPACE;
-  const int vec = vector_width(dtype, c, (uintptr_t)x | (uintptr_t)dy | (uintptr_t)dx);
+  const int vec = norm_vector(dtype, c, g, (uintptr_t)x | (uintptr_t)dy | (uintptr_t)dx);
   Norm a = norm_shape(n, c, g, b, vec);
   a.order = order;
   a.offsets = offsets;
@@ -619,15 +734,16 @@ int tsb_group_norm_bwd(const void* x, const void* dy, const int32_t* order, cons
   a.slope = slope;
   char* ws = static_cast<char*>(workspace);
   float2* slots = reinterpret_cast<float2*>(ws);
-  ws += align_up((size_t)(2 * kSmCount + b) * c * sizeof(float2), 256);
+  ws += align_up((size_t)(kNormBlocks + b) * c * sizeof(float2), 256);
   float2* by_channel = reinterpret_cast<float2*>(ws);
   float2* by_group = reinterpret_cast<float2*>(ws + align_up((size_t)b * c * sizeof(float2), 256));
   const dim3 grid((unsigned)a.nblk, (unsigned)cdiv(a.cols, a.tile));
-  return dispatch_pack(dtype, vec, [&](auto tag) -> int {
+  return dispatch_norm(dtype, vec, a.d, order != nullptr, [&](auto tag, auto each, auto ordered) -> int {
     using T = typename decltype(tag)::T;
-    constexpr int VEC = decltype(tag)::VEC;
+    constexpr int VEC = decltype(tag)::VEC, A = decltype(each)::value;
+    constexpr bool ORDERED = decltype(ordered)::value;
     if (n && b) {
-      norm_grad_sums_kernel<T, VEC><<<grid, kNormThreads, 0, st>>>(a, (const T*)x, (const T*)dy, mean, rstd, slots);
+      norm_grad_sums_kernel<T, VEC, A, ORDERED><<<grid, kNormThreads, 0, st>>>(a, (const T*)x, (const T*)dy, mean, rstd, slots);
       TSB_LAUNCH_CHECK();
     }
     if (b) {
@@ -635,7 +751,7 @@ int tsb_group_norm_bwd(const void* x, const void* dy, const int32_t* order, cons
       TSB_LAUNCH_CHECK();
     }
     if (n && dx) {
-      norm_grad_apply_kernel<T, VEC><<<grid, kNormThreads, 0, st>>>(a, (const T*)x, (const T*)dy, mean, rstd, by_group, (T*)dx);
+      norm_grad_apply_kernel<T, VEC, A, ORDERED><<<grid, kNormThreads, 0, st>>>(a, (const T*)x, (const T*)dy, mean, rstd, by_group, (T*)dx);
       TSB_LAUNCH_CHECK();
     }
     if (dweight || dbias) {
