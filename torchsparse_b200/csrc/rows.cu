@@ -3,20 +3,28 @@
 //
 // Every sum over the rows of a group runs over the grouped order in fixed pieces, so results do not depend on the
 // order in which thread blocks run: there is no floating-point atomic in this file.
+#include <cooperative_groups.h>
+
+#include <mutex>
+
 #include "rows.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace tsb {
 namespace {
 
 // ------------------------------------------------------------------------------------------------ grouping
-// A least-significant-digit radix sort of (key, row) with digits of up to 8 bits.  A tile of 4096 keys is ranked by one
-// block: warp w owns 256 consecutive keys and counts them 32 at a time with __match_any_sync, so equal keys keep
-// their order; a scan over the warps of a tile and one over the tiles of a digit make the ranks global.
-constexpr int kSortThreads = 512;
-constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kSortItems = 8;
-constexpr int kSortTile = kSortThreads * kSortItems;
-constexpr int kMaxDigits = 256;
+// A least-significant-digit radix sort of (key, row) with digits of up to 9 bits: 511 groups need one pass, 262143 two.
+// Keys are ranked in tiles: warp w owns 256 consecutive keys and counts them 32 at a time with __match_any_sync, so equal
+// keys keep their order; sums over the warps of a tile and over the tiles make the ranks global.
+constexpr int kItems = 8;                        // keys of a thread
+constexpr int kMaxDigits = 512;
+constexpr int kSortThreads = 256;                // of a tile of the sort of many keys
+constexpr int kSortTile = kSortThreads * kItems;
+constexpr int kClusterThreads = 1024;            // of a block of the sort of few keys, at most
+constexpr int kClusterBlocks = 8;                // the largest cluster that every device guarantees
+constexpr int kClusterKeys = kClusterBlocks * kClusterThreads * kItems;
 
 struct KeySource {
   const void* keys;      // int32 or int64, `stride` elements apart
@@ -34,14 +42,13 @@ __device__ __forceinline__ unsigned read_key(const KeySource& s, int64_t i) {
 
 // Ranks of the keys of a tile among equal digits of the same warp; whist[w][d] ends as the exclusive sum over the
 // warps before w and total[d] as the tile's count.  Item `it` of lane l is key w * 256 + it * 32 + l of the tile.
-__device__ __forceinline__ void rank_tile(const unsigned (&digit)[kSortItems], const bool (&on)[kSortItems],
-                                          unsigned (&rank)[kSortItems], unsigned short (*whist)[kMaxDigits],
-                                          unsigned* total, int n_digits) {
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+__device__ __forceinline__ void rank_tile(const unsigned (&digit)[kItems], const bool (&on)[kItems], unsigned (&rank)[kItems],
+                                          unsigned short (*whist)[kMaxDigits], unsigned* total, int n_digits) {
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   for (int d = lane; d < n_digits; d += 32) whist[w][d] = 0;
   __syncwarp();
 #pragma unroll
-  for (int it = 0; it < kSortItems; ++it) {
+  for (int it = 0; it < kItems; ++it) {
     const unsigned d = on[it] ? digit[it] : (unsigned)kMaxDigits;      // keys beyond the end match only one another
     const unsigned same = __match_any_sync(0xffffffffu, d);
     const unsigned before = on[it] ? whist[w][d] : 0u;
@@ -51,9 +58,9 @@ __device__ __forceinline__ void rank_tile(const unsigned (&digit)[kSortItems], c
     __syncwarp();
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < n_digits; d += kSortThreads) {
+  for (int d = threadIdx.x; d < n_digits; d += blockDim.x) {
     unsigned sum = 0;
-    for (int i = 0; i < kSortWarps; ++i) {
+    for (int i = 0; i < warps; ++i) {
       const unsigned v = whist[i][d];
       whist[i][d] = (unsigned short)sum;
       sum += v;
@@ -63,86 +70,106 @@ __device__ __forceinline__ void rank_tile(const unsigned (&digit)[kSortItems], c
   __syncthreads();
 }
 
-// in place: total[0..n_digits) -> exclusive sums, by the first warp
-__device__ __forceinline__ void scan_digits(unsigned* total, int n_digits) {
-  if (threadIdx.x < 32) {
-    unsigned carry = 0;
-    for (int d0 = 0; d0 < n_digits; d0 += 32) {
-      const int d = d0 + threadIdx.x;
-      const unsigned v = d < n_digits ? total[d] : 0u;
-      unsigned inc = v;
+// in place: v[0..n) -> exclusive sums, by the whole block; wsum: one word per warp
+__device__ __forceinline__ void scan_digits(unsigned* v, int n, unsigned* wsum) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  unsigned carry = 0;
+  for (int d0 = 0; d0 < n; d0 += blockDim.x) {
+    const int d = d0 + threadIdx.x;
+    const unsigned own = d < n ? v[d] : 0u;
+    unsigned inc = own;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const unsigned up = __shfl_up_sync(0xffffffffu, inc, o);
-        if ((int)threadIdx.x >= o) inc += up;
-      }
-      if (d < n_digits) total[d] = carry + inc - v;
-      carry += __shfl_sync(0xffffffffu, inc, 31);
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned up = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += up;
     }
+    if (lane == 31) wsum[w] = inc;
+    __syncthreads();
+    unsigned before = carry;
+    for (int i = 0; i < warps; ++i) {
+      if (i < w) before += wsum[i];
+      carry += wsum[i];
+    }
+    if (d < n) v[d] = before + inc - own;
+    __syncthreads();
   }
-  __syncthreads();
 }
 
 struct SortOut {
   int* order;        // [n] row at a sorted position
   int* inverse;      // [n] sorted position of a row, or null
   unsigned* keys;    // [n] key at a sorted position, or null
+  int* offsets;      // [n_groups + 1], or null; written where one digit holds the whole key
 };
 
-// n <= kSortTile: every pass in one block, through shared memory
-__global__ void __launch_bounds__(kSortThreads) sort_one_tile_kernel(KeySource src, int n, int passes, int bits, SortOut out,
-                                                                     int* __restrict__ offsets) {
-  __shared__ unsigned short whist[kSortWarps][kMaxDigits];
-  __shared__ unsigned total[kMaxDigits];
-  __shared__ unsigned skey[kSortTile];
-  __shared__ unsigned short srow[kSortTile];
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int base = w * 32 * kSortItems + lane;
-  unsigned key[kSortItems], row[kSortItems], digit[kSortItems], rank[kSortItems];
-  bool on[kSortItems];
+// n <= kClusterKeys: one cluster does every pass in one launch.  Block r holds the positions from r * tile on; its keys
+// stay in registers, the counts and the sorted pairs cross through the blocks' shared memory, the last pass writes the
+// result.
+size_t cluster_smem(int threads) {
+  return (size_t)threads * kItems * 8 + (2 * kMaxDigits + 32) * sizeof(unsigned) + (size_t)(threads / 32) * kMaxDigits * 2;
+}
+
+__global__ void __launch_bounds__(kClusterThreads) sort_cluster_kernel(KeySource src, int n, int passes, int bits, SortOut out) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int tile = blockDim.x * kItems;
+  uint2* pairs = reinterpret_cast<uint2*>(smem);
+  unsigned* total = reinterpret_cast<unsigned*>(pairs + tile);
+  unsigned* start = total + kMaxDigits;
+  unsigned* wsum = start + kMaxDigits;
+  auto whist = reinterpret_cast<unsigned short(*)[kMaxDigits]>(wsum + 32);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int w = threadIdx.x >> 5, blocks = (int)gridDim.x;
+  const int local = w * 32 * kItems + (threadIdx.x & 31), base = (int)blockIdx.x * tile + local;
+  const unsigned per = 0xffffffffu / (unsigned)tile + 1;      // pos / tile = pos * per >> 32 for pos, tile <= 65536
+  unsigned key[kItems], row[kItems], digit[kItems], rank[kItems];
+  bool on[kItems];
 #pragma unroll
-  for (int it = 0; it < kSortItems; ++it) {
+  for (int it = 0; it < kItems; ++it) {
     row[it] = (unsigned)(base + it * 32);
     on[it] = (int)row[it] < n;
     key[it] = on[it] ? read_key(src, row[it]) : 0u;
   }
+  const int n_digits = 1 << bits;
   for (int p = 0; p < passes; ++p) {
 #pragma unroll
-    for (int it = 0; it < kSortItems; ++it) digit[it] = (key[it] >> (p * bits)) & ((1u << bits) - 1);
-    rank_tile(digit, on, rank, whist, total, 1 << bits);
-    scan_digits(total, 1 << bits);
-#pragma unroll
-    for (int it = 0; it < kSortItems; ++it) {
-      if (!on[it]) continue;
-      const unsigned pos = total[digit[it]] + whist[w][digit[it]] + rank[it];
-      skey[pos] = key[it];
-      srow[pos] = (unsigned short)row[it];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int it = 0; it < kSortItems; ++it) {
-      if (!on[it]) continue;
-      key[it] = skey[base + it * 32];
-      row[it] = srow[base + it * 32];
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int it = 0; it < kSortItems; ++it) {
-    if (!on[it]) continue;
-    const int pos = base + it * 32;
-    out.order[pos] = (int)row[it];
-    if (out.inverse) out.inverse[row[it]] = pos;
-    if (out.keys) out.keys[pos] = key[it];
-  }
-  if (offsets) {       // first position whose key is not below the group
-    for (unsigned g = threadIdx.x; g <= src.n_groups; g += kSortThreads) {
-      int lo = 0, hi = n;
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (skey[mid] < g) lo = mid + 1; else hi = mid;
+    for (int it = 0; it < kItems; ++it) digit[it] = (key[it] >> (p * bits)) & (n_digits - 1);
+    rank_tile(digit, on, rank, whist, total, n_digits);
+    if (blocks > 1) cluster.sync();      // every block's counts are there
+    for (int d = threadIdx.x; d < n_digits; d += blockDim.x) {
+      unsigned sum = 0, mine = 0;
+      for (int q = 0; q < blocks; ++q) {
+        if (q == (int)blockIdx.x) mine = sum;      // what earlier blocks have of this digit
+        sum += *cluster.map_shared_rank(total + d, q);
       }
-      offsets[g] = lo;
+      start[d] = sum;
+      for (int i = 0; i < (int)(blockDim.x >> 5); ++i) whist[i][d] += (unsigned short)mine;      // below 65536: fewer than n
+    }
+    __syncthreads();
+    scan_digits(start, n_digits, wsum);
+    if (out.offsets && blockIdx.x == 0)
+      for (int d = threadIdx.x; d <= (int)src.n_groups; d += blockDim.x) out.offsets[d] = (int)start[d];
+    const bool end = p + 1 == passes;
+#pragma unroll
+    for (int it = 0; it < kItems; ++it) {
+      if (!on[it]) continue;
+      const unsigned pos = start[digit[it]] + whist[w][digit[it]] + rank[it];
+      if (end) {
+        out.order[pos] = (int)row[it];
+        if (out.inverse) out.inverse[row[it]] = (int)pos;
+        if (out.keys) out.keys[pos] = key[it];
+      } else {
+        const unsigned to = __umulhi(pos, per);
+        cluster.map_shared_rank(pairs, (int)to)[pos - to * tile] = make_uint2(key[it], row[it]);
+      }
+    }
+    if (blocks > 1) cluster.sync(); else __syncthreads();      // the pairs are there, and no block reads counts any more
+    if (end) break;
+#pragma unroll
+    for (int it = 0; it < kItems; ++it) {
+      if (!on[it]) continue;
+      const uint2 v = pairs[local + it * 32];
+      key[it] = v.x;
+      row[it] = v.y;
     }
   }
 }
@@ -154,10 +181,9 @@ struct PassIn {
   const int* rows;
 };
 
-__device__ __forceinline__ void load_tile(const PassIn& in, int64_t n, unsigned (&key)[kSortItems], bool (&on)[kSortItems],
-                                          int64_t first) {
+__device__ __forceinline__ void load_tile(const PassIn& in, int64_t n, unsigned (&key)[kItems], bool (&on)[kItems], int64_t first) {
 #pragma unroll
-  for (int it = 0; it < kSortItems; ++it) {
+  for (int it = 0; it < kItems; ++it) {
     const int64_t i = first + it * 32;
     on[it] = i < n;
     key[it] = on[it] ? (in.keys ? __ldg(in.keys + i) : read_key(in.src, i)) : 0u;
@@ -166,14 +192,14 @@ __device__ __forceinline__ void load_tile(const PassIn& in, int64_t n, unsigned 
 
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(PassIn in, int64_t n, int shift, int bits, int64_t tiles,
                                                                   unsigned* __restrict__ counts) {
-  __shared__ unsigned short whist[kSortWarps][kMaxDigits];
+  __shared__ unsigned short whist[kSortThreads / 32][kMaxDigits];
   __shared__ unsigned total[kMaxDigits];
-  const int64_t first = (int64_t)blockIdx.x * kSortTile + (threadIdx.x >> 5) * 32 * kSortItems + (threadIdx.x & 31);
-  unsigned key[kSortItems], digit[kSortItems], rank[kSortItems];
-  bool on[kSortItems];
+  const int64_t first = (int64_t)blockIdx.x * kSortTile + (threadIdx.x >> 5) * 32 * kItems + (threadIdx.x & 31);
+  unsigned key[kItems], digit[kItems], rank[kItems];
+  bool on[kItems];
   load_tile(in, n, key, on, first);
 #pragma unroll
-  for (int it = 0; it < kSortItems; ++it) digit[it] = (key[it] >> shift) & ((1u << bits) - 1);
+  for (int it = 0; it < kItems; ++it) digit[it] = (key[it] >> shift) & ((1u << bits) - 1);
   rank_tile(digit, on, rank, whist, total, 1 << bits);
   for (int d = threadIdx.x; d < (1 << bits); d += kSortThreads) counts[d * tiles + blockIdx.x] = total[d];
 }
@@ -209,21 +235,24 @@ __global__ void __launch_bounds__(256) sort_scan_kernel(unsigned* __restrict__ c
 
 __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(PassIn in, int64_t n, int shift, int bits, int64_t tiles,
                                                                     const unsigned* __restrict__ counts, SortOut out) {
-  __shared__ unsigned short whist[kSortWarps][kMaxDigits];
+  __shared__ unsigned short whist[kSortThreads / 32][kMaxDigits];
   __shared__ unsigned total[kMaxDigits];
   __shared__ unsigned start[kMaxDigits];
+  __shared__ unsigned wsum[kSortThreads / 32];
   const int w = threadIdx.x >> 5;
-  const int64_t first = (int64_t)blockIdx.x * kSortTile + w * 32 * kSortItems + (threadIdx.x & 31);
-  unsigned key[kSortItems], digit[kSortItems], rank[kSortItems];
-  bool on[kSortItems];
+  const int64_t first = (int64_t)blockIdx.x * kSortTile + w * 32 * kItems + (threadIdx.x & 31);
+  unsigned key[kItems], digit[kItems], rank[kItems];
+  bool on[kItems];
   load_tile(in, n, key, on, first);
   for (int d = threadIdx.x; d < (1 << bits); d += kSortThreads) start[d] = counts[(int64_t)(1 << bits) * tiles + d];
 #pragma unroll
-  for (int it = 0; it < kSortItems; ++it) digit[it] = (key[it] >> shift) & ((1u << bits) - 1);
+  for (int it = 0; it < kItems; ++it) digit[it] = (key[it] >> shift) & ((1u << bits) - 1);
   rank_tile(digit, on, rank, whist, total, 1 << bits);      // its barriers also publish start[]
-  scan_digits(start, 1 << bits);
+  scan_digits(start, 1 << bits, wsum);
+  if (out.offsets && blockIdx.x == 0)
+    for (int d = threadIdx.x; d <= (int)in.src.n_groups; d += kSortThreads) out.offsets[d] = (int)start[d];
 #pragma unroll
-  for (int it = 0; it < kSortItems; ++it) {
+  for (int it = 0; it < kItems; ++it) {
     if (!on[it]) continue;
     const unsigned d = digit[it];
     const int64_t pos = (int64_t)start[d] + counts[d * tiles + blockIdx.x] + whist[w][d] + rank[it];
@@ -258,101 +287,157 @@ struct SortPlan {
 SortPlan sort_plan(int64_t n, int64_t n_groups) {
   SortPlan p;
   int total = 1;
-  while ((n_groups >> total) != 0) ++total;
-  p.passes = (total + 7) / 8;
+  while ((n_groups >> total) != 0) ++total;      // keys are 0 .. n_groups
+  p.passes = (total + 8) / 9;
   p.bits = (total + p.passes - 1) / p.passes;
   p.tiles = cdiv(n, kSortTile);
-  p.counts = align_up(((size_t)(p.tiles + 1) << p.bits) * sizeof(unsigned), 256);
   p.pairs = align_up((size_t)n * 4, 256);
-  p.bytes = n <= kSortTile ? 256 : p.counts + 5 * p.pairs;      // two sets of (key, row), the sorted keys
+  p.counts = n <= kClusterKeys ? 0 : align_up(((size_t)(p.tiles + 1) << p.bits) * sizeof(unsigned), 256);
+  // the sorted keys, and two sets of (key, row) beside the tiles' counts
+  p.bytes = p.pairs + (n <= kClusterKeys ? 0 : p.counts + 4 * p.pairs);
   return p;
 }
 
-// order / inverse / keys / offsets of n keys; `sorted` (never null) receives the sorted keys when n > one tile
-int run_sort(const KeySource& src, int64_t n, SortOut out, int* offsets, void* workspace, cudaStream_t st) {
+int allow_cluster_smem() {
+  static std::mutex mu;
+  static bool done[64] = {};
+  int dev = 0;
+  TSB_CUDA_TRY(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return TSB_ERR_LIMIT;
+  std::lock_guard<std::mutex> lock(mu);
+  if (!done[dev]) {
+    TSB_CUDA_TRY(cudaFuncSetAttribute(sort_cluster_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)cluster_smem(kClusterThreads)));
+    done[dev] = true;
+  }
+  return TSB_OK;
+}
+
+// order / inverse / keys / offsets of n >= 1 keys
+int run_sort(const KeySource& src, int64_t n, SortOut out, void* workspace, cudaStream_t st) {
   const SortPlan p = sort_plan(n, src.n_groups);
-  if (n <= kSortTile) {
-    sort_one_tile_kernel<<<1, kSortThreads, 0, st>>>(src, (int)n, p.passes, p.bits, out, offsets);
-    TSB_LAUNCH_CHECK();
-    return TSB_OK;
-  }
   char* ws = static_cast<char*>(workspace);
-  unsigned* counts = reinterpret_cast<unsigned*>(ws);
-  unsigned* keys[2];
-  int* rows[2];
-  for (int i = 0; i < 2; ++i) {
-    keys[i] = reinterpret_cast<unsigned*>(ws + p.counts + 2 * i * p.pairs);
-    rows[i] = reinterpret_cast<int*>(ws + p.counts + (2 * i + 1) * p.pairs);
+  int* const offsets = out.offsets;
+  const bool search = offsets && p.passes > 1;      // more than one digit: the offsets are searched in the sorted keys
+  if (search && !out.keys) out.keys = reinterpret_cast<unsigned*>(ws);
+  if (p.passes > 1) out.offsets = nullptr;
+  if (n <= kClusterKeys) {
+    const int rc = allow_cluster_smem();
+    if (rc != TSB_OK) return rc;
+    // 2048 keys fit a block of 8 warps; more of them are spread over the whole cluster
+    const int64_t warps = cdiv(n, (n <= kSortTile ? 1 : kClusterBlocks) * 32 * kItems);
+    const int threads = 32 * (int)(warps < 2 ? 2 : warps);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)cdiv(n, (int64_t)threads * kItems));
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = cluster_smem(threads);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cfg.gridDim.x;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    count_launch();
+    TSB_CUDA_TRY(cudaLaunchKernelEx(&cfg, sort_cluster_kernel, src, (int)n, p.passes, p.bits, out));
+  } else {
+    unsigned* counts = reinterpret_cast<unsigned*>(ws + p.pairs);
+    ws += p.pairs + p.counts;
+    PassIn in{src, nullptr, nullptr};
+    for (int i = 0; i < p.passes; ++i) {
+      SortOut to = out;
+      if (i + 1 < p.passes)
+        to = SortOut{reinterpret_cast<int*>(ws + (2 * (i & 1) + 1) * p.pairs), nullptr,
+                     reinterpret_cast<unsigned*>(ws + 2 * (i & 1) * p.pairs), nullptr};
+      sort_count_kernel<<<(unsigned)p.tiles, kSortThreads, 0, st>>>(in, n, i * p.bits, p.bits, p.tiles, counts);
+      TSB_LAUNCH_CHECK();
+      sort_scan_kernel<<<1 << p.bits, 256, 0, st>>>(counts, p.tiles, 1 << p.bits);
+      TSB_LAUNCH_CHECK();
+      sort_scatter_kernel<<<(unsigned)p.tiles, kSortThreads, 0, st>>>(in, n, i * p.bits, p.bits, p.tiles, counts, to);
+      TSB_LAUNCH_CHECK();
+      in.keys = to.keys;
+      in.rows = to.order;
+    }
   }
-  unsigned* last = out.keys ? out.keys : reinterpret_cast<unsigned*>(ws + p.counts + 4 * p.pairs);
-  PassIn in{src, nullptr, nullptr};
-  for (int i = 0; i < p.passes; ++i) {
-    const bool end = i + 1 == p.passes;
-    const SortOut to = end ? SortOut{out.order, out.inverse, last} : SortOut{rows[i & 1], nullptr, keys[i & 1]};
-    sort_count_kernel<<<(unsigned)p.tiles, kSortThreads, 0, st>>>(in, n, i * p.bits, p.bits, p.tiles, counts);
-    TSB_LAUNCH_CHECK();
-    sort_scan_kernel<<<1 << p.bits, 256, 0, st>>>(counts, p.tiles, 1 << p.bits);
-    TSB_LAUNCH_CHECK();
-    sort_scatter_kernel<<<(unsigned)p.tiles, kSortThreads, 0, st>>>(in, n, i * p.bits, p.bits, p.tiles, counts, to);
-    TSB_LAUNCH_CHECK();
-    in.keys = to.keys;
-    in.rows = to.order;
-  }
-  if (offsets) {
-    group_offsets_kernel<<<grid_for((int64_t)src.n_groups + 1, 256), 256, 0, st>>>(last, n, src.n_groups, offsets);
+  if (search) {
+    group_offsets_kernel<<<grid_for((int64_t)src.n_groups + 1, 256), 256, 0, st>>>(out.keys, n, src.n_groups, offsets);
     TSB_LAUNCH_CHECK();
   }
   return TSB_OK;
 }
 
 // ------------------------------------------------------------------------------------------------ embedding
-// y[i] = scale * table[token[i]], zeros where the token is no row of the table: one vector of a row per thread.
+constexpr int kThreads = 256;
+constexpr int kUnroll = 4;      // vectors of a thread in the row copies: 64 bytes in flight for each
+
+// y[i] = scale * table[token[i]], zeros where the token is no row of the table.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256) embed_kernel(const T* __restrict__ table, KeySource src, int64_t n, int64_t c, float scale,
-                                                    T* __restrict__ out) {
-  const int64_t cols = c / VEC, total = n * cols;
-  for (int64_t t = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; t < total; t += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t i = t / cols, j = (t - i * cols) * VEC;
-    const unsigned row = read_key(src, i);
-    Pack<T, VEC> p;
-    if (row < src.n_groups) {
-      p.load(table + (int64_t)row * c + j);
-      float v[VEC];
-      p.get(v);
+__global__ void __launch_bounds__(kThreads) embed_kernel(const T* __restrict__ table, KeySource src, int64_t total, RowSplit split,
+                                                         float scale, T* __restrict__ out) {
+  const int64_t t0 = blockIdx.x * (int64_t)(kThreads * kUnroll) + threadIdx.x;
+  const int64_t c = (int64_t)split.cols * VEC;
+  Pack<T, VEC> v[kUnroll];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) v[e] *= scale;
-      p.set(v);
-    } else {
-      p.clear();
+  for (int u = 0; u < kUnroll; ++u) {
+    const int64_t t = t0 + u * kThreads;
+    v[u].clear();
+    if (t < total) {
+      const int64_t i = split.row(t);
+      const unsigned row = read_key(src, i);
+      if (row < src.n_groups) v[u].load(table + (int64_t)row * c + (t - i * split.cols) * VEC);
     }
-    p.store(out + i * c + j);
+  }
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const int64_t t = t0 + u * kThreads;
+    if (t >= total) break;
+    float f[VEC];
+    v[u].get(f);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[e] *= scale;
+    v[u].set(f);
+    v[u].store(out + t * VEC);
   }
 }
 
 // The gradient of the table: dtable[v] = scale * sum of grad[i] over the rows i whose token is v.
 //
 // The rows are walked in sorted order by workers of `cols` threads (one thread per vector of a row), each over `len`
-// positions.  A token whose positions lie inside one worker is summed and written there; one that crosses workers
-// leaves a 32-bit partial sum per worker, `tail` where it begins and `head` where it goes on, which embed_join_kernel
-// adds up in order.  The blocks behind the workers write the zeros of the tokens that do not occur.
+// positions; a block holds `per_block` workers of consecutive positions.  A token whose positions lie inside one
+// worker is summed and written there.  One that crosses workers leaves 32-bit partial sums in shared memory, `tail`
+// where it begins and `head` where it goes on, which the worker in which it begins adds up in order; one that crosses
+// blocks leaves them in memory for embed_join_kernel.  The blocks behind the workers write the zeros of the tokens that
+// do not occur, so every row of the table is written exactly once.
 struct EmbedGrad {
   const unsigned* keys;      // sorted; n_rows marks rows without a token
   const int* order;
   int64_t n, n_rows, c;
   int len;                   // positions of a worker
-  int64_t workers;
-  int cols, per_block;       // threads of a worker, workers of a block
+  int tile;                  // vectors of a row that a block takes (grid.y tiles)
+  int per_block;             // workers of a block
+  int64_t span, blocks;      // positions of a block, blocks
   float scale;
-  float* head;               // [workers, c]
+  float* head;               // [blocks, c]
   float* tail;
 };
 
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256) embed_grad_kernel(EmbedGrad a, const T* __restrict__ grad, T* __restrict__ dtable,
-                                                         int64_t worker_blocks, int zero_rows) {
-  if (blockIdx.x >= worker_blocks) {
-    __shared__ unsigned char absent[256];
-    const int64_t v0 = (blockIdx.x - worker_blocks) * (int64_t)zero_rows;
+__device__ __forceinline__ void write_row(const EmbedGrad& a, float (&acc)[VEC], T* __restrict__ to) {
+  Pack<T, VEC> o;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) acc[e] *= a.scale;
+  o.set(acc);
+  o.store(to);
+}
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kThreads, 4) embed_grad_kernel(EmbedGrad a, const T* __restrict__ grad, T* __restrict__ dtable,
+                                                              int zero_rows) {
+  __shared__ float s_head[VEC][kThreads], s_tail[VEC][kThreads];
+  __shared__ unsigned char s_flags[kThreads];      // of a worker: 1 = it has a tail, 2 = its head goes on behind it
+  const int first = blockIdx.y * a.tile, width = min(a.tile, (int)(a.c / VEC) - first);
+  if (blockIdx.x >= a.blocks) {
+    const int64_t v0 = (blockIdx.x - a.blocks) * (int64_t)zero_rows;
     if ((int)threadIdx.x < zero_rows) {
       const int64_t v = v0 + threadIdx.x;
       bool none = false;
@@ -360,31 +445,33 @@ __global__ void __launch_bounds__(256) embed_grad_kernel(EmbedGrad a, const T* _
         const int64_t at = lower_bound(a.keys, a.n, (unsigned)v);
         none = at >= a.n || __ldg(a.keys + at) != (unsigned)v;
       }
-      absent[threadIdx.x] = none;
+      s_flags[threadIdx.x] = none;
     }
     __syncthreads();
-    const int cols = (int)(a.c / VEC);
     Pack<T, VEC> zero;
     zero.clear();
-    for (int t = threadIdx.x; t < zero_rows * cols; t += blockDim.x) {
-      const int r = t / cols;
-      if (absent[r]) zero.store(dtable + (v0 + r) * a.c + (int64_t)(t - r * cols) * VEC);
+    for (int t = threadIdx.x; t < zero_rows * width; t += kThreads) {
+      const int r = t / width;
+      if (s_flags[r]) zero.store(dtable + (v0 + r) * a.c + (int64_t)(first + t - r * width) * VEC);
     }
     return;
   }
-  const int slot = threadIdx.x / a.cols;
-  const int64_t w = blockIdx.x * (int64_t)a.per_block + slot;
-  if (slot >= a.per_block || w >= a.workers) return;
-  const int64_t p0 = w * a.len, p1 = min(p0 + a.len, a.n);
   const unsigned none = (unsigned)a.n_rows;
-  for (int64_t j = (int64_t)(threadIdx.x - slot * a.cols) * VEC; j < a.c; j += (int64_t)a.cols * VEC) {
-    float acc[VEC];
+  const int slot = threadIdx.x / width, col = threadIdx.x - slot * width;
+  const int64_t j = (int64_t)(first + col) * VEC;
+  const int64_t p0 = blockIdx.x * a.span + (int64_t)slot * a.len, p1 = min(p0 + a.len, a.n);
+  const bool live = slot < a.per_block && p0 < a.n;
+  bool has_head = false, through = false, has_tail = false;
+  unsigned cur = none;
+  float acc[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
-    unsigned cur = __ldg(a.keys + p0);
-    bool goes_on = p0 > 0 && __ldg(a.keys + p0 - 1) == cur;      // the run began in an earlier worker
-    for (int64_t p = p0; p < p1 && cur != none;) {
-      constexpr int U = 4;
+  for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+  if (live) {
+    cur = __ldg(a.keys + p0);
+    bool goes_on = cur != none && p0 > 0 && __ldg(a.keys + p0 - 1) == cur;      // the run began in an earlier worker
+    has_head = goes_on;
+    constexpr int U = 4;
+    for (int64_t p = p0; p < p1 && cur != none; p += U) {
       Pack<T, VEC> v[U];
       unsigned key[U];
 #pragma unroll
@@ -398,13 +485,9 @@ __global__ void __launch_bounds__(256) embed_grad_kernel(EmbedGrad a, const T* _
         if (key[u] != cur) {      // the run of `cur` ended inside this worker
           if (goes_on) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) a.head[w * a.c + j + e] = acc[e];
+            for (int e = 0; e < VEC; ++e) s_head[e][threadIdx.x] = acc[e];
           } else {
-            Pack<T, VEC> o;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[e] *= a.scale;
-            o.set(acc);
-            o.store(dtable + (int64_t)cur * a.c + j);
+            write_row(a, acc, dtable + (int64_t)cur * a.c + j);
           }
 #pragma unroll
           for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
@@ -417,69 +500,119 @@ __global__ void __launch_bounds__(256) embed_grad_kernel(EmbedGrad a, const T* _
 #pragma unroll
         for (int e = 0; e < VEC; ++e) acc[e] += g[e];
       }
-      p += U;
     }
-    if (cur == none) continue;
-    const bool on = p1 < a.n && __ldg(a.keys + p1) == cur;      // the run goes on in the next worker
-    if (goes_on || on) {
-      float* to = goes_on ? a.head : a.tail;
+    if (cur != none) {
+      const bool on = p1 < a.n && __ldg(a.keys + p1) == cur;      // the run goes on in the next worker
+      if (goes_on) {
+        through = on;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) to[w * a.c + j + e] = acc[e];
+        for (int e = 0; e < VEC; ++e) s_head[e][threadIdx.x] = acc[e];
+      } else if (on) {
+        has_tail = true;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s_tail[e][threadIdx.x] = acc[e];
+      } else {
+        write_row(a, acc, dtable + (int64_t)cur * a.c + j);
+      }
+    }
+    if (col == 0) s_flags[slot] = (has_tail ? 1 : 0) | (through ? 2 : 0);
+  }
+  __syncthreads();
+  if (!live) return;
+  // A run that began before this block: the first worker collects its heads.  One that began in a worker: that worker.
+  const bool begins = slot == 0 && has_head;
+  if (!begins && !has_tail) return;
+  for (int which = begins ? 0 : 1; which < (has_tail ? 2 : 1); ++which) {
+    int x = slot;
+    bool more = which == 0 ? through : true;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) acc[e] = which == 0 ? s_head[e][threadIdx.x] : s_tail[e][threadIdx.x];
+    while (more && x + 1 < a.per_block) {
+      ++x;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) acc[e] += s_head[e][x * width + col];
+      more = s_flags[x] & 2;
+    }
+    if (which == 0 || more) {
+      float* to = (which == 0 ? a.head : a.tail) + blockIdx.x * a.c + j;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) to[e] = acc[e];
     } else {
-      Pack<T, VEC> o;
+      write_row(a, acc, dtable + (int64_t)cur * a.c + j);
+    }
+  }
+}
+
+// A block per block of embed_grad_kernel in which a run begins that goes on behind it, and per 256 channels: its tail and
+// the heads of the blocks that follow (those whose first key is the same), threads = channels (JV a thread) x slices of
+// those blocks.
+constexpr int kJoinThreads = 512;
+template <typename T, int JV>
+__global__ void __launch_bounds__(kJoinThreads) embed_join_kernel(EmbedGrad a, T* __restrict__ dtable) {
+  __shared__ float part[JV][kJoinThreads];
+  const int64_t p0 = blockIdx.x * a.span, p1 = p0 + a.span;
+  if (p1 >= a.n) return;
+  const unsigned key = __ldg(a.keys + p1 - 1);
+  if (key == (unsigned)a.n_rows || __ldg(a.keys + p1) != key) return;
+  if (p0 > 0 && __ldg(a.keys + p0 - 1) == key) return;      // it began before (the keys are sorted)
+  const int64_t j0 = blockIdx.y * 256;
+  const int cols = (int)((min(a.c - j0, (int64_t)256) + JV - 1) / JV), slices = kJoinThreads / cols;
+  const int slice = threadIdx.x / cols, q = threadIdx.x - slice * cols;
+  const int64_t j = j0 + q * JV;
+  float s[JV];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) acc[e] *= a.scale;
-      o.set(acc);
-      o.store(dtable + (int64_t)cur * a.c + j);
+  for (int e = 0; e < JV; ++e) s[e] = 0.f;
+  if (slice < slices) {
+    constexpr int U = 4;
+    bool more = true;
+    for (int64_t k = blockIdx.x + 1 + slice; more; k += U * slices) {
+      Pack<float, JV> v[U];
+      bool on[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t b = k + u * slices;
+        on[u] = b < a.blocks && __ldg(a.keys + b * a.span) == key;
+        v[u].clear();
+        if (on[u]) v[u].load(a.head + b * a.c + j);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float f[JV];
+        v[u].get(f);
+        if (on[u]) {
+#pragma unroll
+          for (int e = 0; e < JV; ++e) s[e] += f[e];
+        }
+      }
+      more = on[U - 1];
     }
+  }
+#pragma unroll
+  for (int e = 0; e < JV; ++e) part[e][threadIdx.x] = s[e];
+  __syncthreads();
+  if (slice != 0) return;
+#pragma unroll
+  for (int e = 0; e < JV; ++e) {
+    float all = a.tail[blockIdx.x * a.c + j + e];
+    for (int i = 0; i < slices; ++i) all += part[e][i * cols + q];
+    dtable[(int64_t)key * a.c + j + e] = from_f32<T>(all * a.scale);
   }
 }
 
-// One block per worker in which a run begins that goes on: tail + the heads of the workers that follow.
-template <typename T>
-__global__ void __launch_bounds__(256) embed_join_kernel(EmbedGrad a, T* __restrict__ dtable) {
-  __shared__ float part[256];
-  for (int64_t w = blockIdx.x; w < a.workers; w += gridDim.x) {
-    const int64_t p0 = w * a.len, p1 = p0 + a.len;
-    if (p1 >= a.n) continue;
-    const unsigned key = __ldg(a.keys + p1 - 1);
-    if (key == (unsigned)a.n_rows || __ldg(a.keys + p1) != key) continue;
-    if (__ldg(a.keys + p0) == key && p0 > 0 && __ldg(a.keys + p0 - 1) == key) continue;      // it began before
-    const int64_t last = (lower_bound(a.keys, a.n, key + 1) - 1) / a.len;      // the worker in which it ends
-    // 256 threads = columns x slices of the workers w + 1 .. last
-    const int cols = a.c < 256 ? (int)a.c : 256, slices = 256 / cols;
-    const int slice = threadIdx.x / cols;
-    for (int64_t j0 = 0; j0 < a.c; j0 += cols) {
-      const int64_t j = j0 + (threadIdx.x - slice * cols);
-      float s = 0.f;
-      if (slice < slices && j < a.c) {
-#pragma unroll 4
-        for (int64_t k = w + 1 + slice; k <= last; k += slices) s += a.head[k * a.c + j];
-      }
-      part[threadIdx.x] = s;
-      __syncthreads();
-      if (slice == 0 && j < a.c) {
-        float all = a.tail[w * a.c + j];
-        for (int i = 0; i < slices; ++i) all += part[i * cols + threadIdx.x];
-        dtable[(int64_t)key * a.c + j] = from_f32<T>(all * a.scale);
-      }
-      __syncthreads();
-    }
-  }
-}
-
-EmbedGrad embed_plan(int64_t n, int64_t n_rows, int64_t c, int dtype, int vec) {
+EmbedGrad embed_plan(int64_t n, int64_t n_rows, int64_t c, int vec) {
   EmbedGrad a{};
   a.n = n;
   a.n_rows = n_rows;
   a.c = c;
   const int64_t vecs = c / vec;
-  a.cols = (int)(vecs < 256 ? vecs : 256);
-  a.per_block = 256 / a.cols;
-  int64_t len = cdiv(n * a.cols, (int64_t)kSmCount * 2048);
+  a.tile = (int)cdiv(vecs, cdiv(vecs, kThreads));
+  a.per_block = kThreads / a.tile;
+  // one wave of four blocks an SM where that leaves workers of 8 to 64 positions
+  int64_t len = cdiv(n, cdiv(4 * kSmCount, cdiv(vecs, a.tile)) * a.per_block);
   len = len < 8 ? 8 : len > 64 ? 64 : len;
   a.len = (int)len;
-  a.workers = cdiv(n, len);
+  a.span = len * a.per_block;
+  a.blocks = cdiv(n, a.span);
   return a;
 }
 
@@ -487,90 +620,151 @@ EmbedGrad embed_plan(int64_t n, int64_t n_rows, int64_t c, int dtype, int vec) {
 // Position p of the sorted rows belongs to choice order[p] of the n * k choices; positions at and behind offsets[E]
 // belong to choices of no expert.
 
-// xs[inverse[i][j]] = x[i], zeros behind the kept rows: one vector of a (row, choice) per thread, so the k reads of a
-// row meet in the L1 cache.
+// xs[inverse[i][j]] = x[i], zeros behind the kept rows: a vector of x is read once and written k times.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256) dispatch_kernel(const T* __restrict__ x, const int* __restrict__ inverse,
-                                                       const int* __restrict__ kept, int64_t pairs, int k, int64_t c,
-                                                       T* __restrict__ xs) {
-  const int64_t cols = c / VEC, total = pairs * cols, n_kept = __ldg(kept);
-  for (int64_t t = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; t < total; t += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t q = t / cols, j = (t - q * cols) * VEC;
-    const int64_t pos = __ldg(inverse + q);
-    if (pos < 0 || pos >= pairs) continue;
-    Pack<T, VEC> p;
-    if (pos < n_kept) p.load(x + q / k * c + j); else p.clear();
-    p.store(xs + pos * c + j);
-  }
-}
-
-// out[i] = sum over j of w[i][j] * rows[inverse[i][j]] (w null: 1), in the order of j
-template <typename T, int VEC>
-__global__ void __launch_bounds__(256) combine_kernel(const T* __restrict__ rows, const void* __restrict__ w, int w_dtype,
-                                                      const int* __restrict__ inverse, const int* __restrict__ kept, int64_t n,
-                                                      int k, int64_t c, T* __restrict__ out) {
-  const int64_t cols = c / VEC, total = n * cols, pairs = n * k;
-  const int64_t n_kept = min((int64_t)__ldg(kept), pairs);
-  for (int64_t t = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; t < total; t += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t i = t / cols, j = (t - i * cols) * VEC;
-    float acc[VEC];
+__global__ void __launch_bounds__(kThreads) dispatch_kernel(const T* __restrict__ x, const int* __restrict__ inverse,
+                                                            const int* __restrict__ kept, int64_t total, int64_t pairs, int k,
+                                                            RowSplit split, T* __restrict__ xs) {
+  constexpr int U = 2;
+  const int64_t t0 = blockIdx.x * (int64_t)(kThreads * U) + threadIdx.x;
+  const int64_t c = (int64_t)split.cols * VEC, n_kept = __ldg(kept);
+  Pack<T, VEC> v[U], zero;
+  zero.clear();
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
-#pragma unroll 4
+  for (int u = 0; u < U; ++u)
+    if (t0 + u * kThreads < total) v[u].load(x + (t0 + u * kThreads) * VEC);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t t = t0 + u * kThreads;
+    if (t >= total) break;
+    const int64_t i = split.row(t), j = (t - i * split.cols) * VEC;
     for (int q = 0; q < k; ++q) {
       const int64_t pos = __ldg(inverse + i * k + q);
-      if (pos < 0 || pos >= n_kept) continue;
-      Pack<T, VEC> p;
-      p.load(rows + pos * c + j);
-      const float f = w ? load_any(w, w_dtype, i * k + q) : 1.f;
-      float v[VEC];
-      p.get(v);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) acc[e] = fmaf(f, v[e], acc[e]);
+      if (pos >= 0 && pos < pairs) (pos < n_kept ? v[u] : zero).store(xs + pos * c + j);
     }
-    Pack<T, VEC> o;
-    o.set(acc);
-    o.store(out + i * c + j);
   }
 }
 
-// One warp per choice: drows[pos] = w * dout[i] and dw = <dout[i], rows[pos]>, both zero for a choice of no expert.
-template <typename T, int VEC>
-__global__ void __launch_bounds__(256) combine_grad_kernel(const T* __restrict__ dout, const T* __restrict__ rows,
-                                                           const void* __restrict__ w, int w_dtype,
+// out[i] = sum over j of w[i][j] * rows[inverse[i][j]] (w null: 1), in the order of j.  A thread has ROWS vectors of the
+// result and reads KU choices of each at once: eight vectors in flight.
+template <typename T, int VEC, int KU>
+__global__ void __launch_bounds__(kThreads) combine_kernel(const T* __restrict__ rows, const void* __restrict__ w, int w_dtype,
                                                            const int* __restrict__ inverse, const int* __restrict__ kept,
-                                                           int64_t n, int k, int64_t c, T* __restrict__ drows,
-                                                           void* __restrict__ dw) {
-  const int64_t pairs = n * k, cols = c / VEC;
+                                                           int64_t total, int64_t pairs, int k, RowSplit split,
+                                                           T* __restrict__ out) {
+  constexpr int ROWS = 8 / KU;
+  const int64_t t0 = blockIdx.x * (int64_t)(kThreads * ROWS) + threadIdx.x, c = (int64_t)split.cols * VEC;
+  const int n_kept = (int)min((int64_t)__ldg(kept), pairs);
+  float acc[ROWS][VEC];
+  int64_t i[ROWS];
+  const T* base[ROWS];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const int64_t t = min(t0 + r * kThreads, total - 1);
+    i[r] = split.row(t);
+    base[r] = rows + (t - i[r] * split.cols) * VEC;
+    i[r] *= k;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) acc[r][e] = 0.f;
+  }
+  for (int q0 = 0; q0 < k; q0 += KU) {
+    Pack<T, VEC> p[ROWS][KU];
+    int pos[ROWS][KU];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+      for (int u = 0; u < KU; ++u) {
+        pos[r][u] = q0 + u < k ? __ldg(inverse + i[r] + q0 + u) : -1;
+        if (pos[r][u] >= n_kept) pos[r][u] = -1;
+      }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+      for (int u = 0; u < KU; ++u)
+        if (pos[r][u] >= 0) p[r][u].load(base[r] + pos[r][u] * c);
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+      for (int u = 0; u < KU; ++u) {
+        if (pos[r][u] < 0) continue;
+        const float f = w ? load_any(w, w_dtype, i[r] + q0 + u) : 1.f;
+        float v[VEC];
+        p[r][u].get(v);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[r][e] = fmaf(f, v[e], acc[r][e]);
+      }
+  }
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    if (t0 + r * kThreads >= total) break;
+    Pack<T, VEC> o;
+    o.set(acc[r]);
+    o.store(out + (t0 + r * kThreads) * VEC);
+  }
+}
+
+// One group of `lanes` threads (a power of two up to a warp) for PAIRS choices at a time: drows[pos] = w * dout[i] and
+// dw = <dout[i], rows[pos]>, both zero for a choice of no expert.  Choices of one row share its dout through the L1 cache.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kThreads) combine_grad_kernel(const T* __restrict__ dout, const T* __restrict__ rows,
+                                                                const void* __restrict__ w, int w_dtype,
+                                                                const int* __restrict__ inverse, const int* __restrict__ kept,
+                                                                int64_t pairs, RowSplit by_k, int64_t c, int lanes,
+                                                                T* __restrict__ drows, void* __restrict__ dw) {
+  constexpr int PAIRS = 2, U = 2;
+  const int cols = (int)(c / VEC), lane = threadIdx.x & (lanes - 1);
   const int64_t n_kept = __ldg(kept);
-  const int lane = threadIdx.x & 31;
-  for (int64_t q = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5; q < pairs; q += ((int64_t)gridDim.x * blockDim.x) >> 5) {
-    const int64_t pos = __ldg(inverse + q), i = q / k;
-    const bool there = pos >= 0 && pos < pairs, used = there && pos < n_kept;
-    const float f = used ? load_any(w, w_dtype, q) : 0.f;
-    float dot = 0.f;
-    for (int64_t v = lane; v < cols; v += 32) {
-      Pack<T, VEC> g, r;
-      if (used) {
-        g.load(dout + i * c + v * VEC);
-        r.load(rows + pos * c + v * VEC);
+  const int64_t q0 = (blockIdx.x * (int64_t)(kThreads / lanes) + threadIdx.x / lanes) * PAIRS;
+  float f[PAIRS], dot[PAIRS];
+  const T *g0[PAIRS], *r0[PAIRS];
+  T* d0[PAIRS];
+  bool there[PAIRS], used[PAIRS];
+#pragma unroll
+  for (int q = 0; q < PAIRS; ++q) {
+    const int64_t pos = q0 + q < pairs ? (int64_t)__ldg(inverse + q0 + q) : -1;
+    there[q] = pos >= 0 && pos < pairs;
+    used[q] = there[q] && pos < n_kept;
+    dot[q] = 0.f;
+    f[q] = used[q] ? load_any(w, w_dtype, q0 + q) : 0.f;
+    g0[q] = dout + by_k.row(min(q0 + q, pairs - 1)) * c;
+    r0[q] = rows + (there[q] ? pos : 0) * c;
+    d0[q] = drows + (there[q] ? pos : 0) * c;
+  }
+  for (int v0 = lane; v0 < cols; v0 += lanes * U) {
+    Pack<T, VEC> g[PAIRS][U], r[PAIRS][U];
+#pragma unroll
+    for (int q = 0; q < PAIRS; ++q)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (!used[q] || v0 + u * lanes >= cols) {
+          g[q][u].clear();
+          r[q][u].clear();
+          continue;
+        }
+        r[q][u].load(r0[q] + (v0 + u * lanes) * VEC);
+        g[q][u].load(g0[q] + (v0 + u * lanes) * VEC);
+      }
+#pragma unroll
+    for (int q = 0; q < PAIRS; ++q)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (!there[q] || v0 + u * lanes >= cols) continue;
         float a[VEC], b[VEC];
-        g.get(a);
-        r.get(b);
+        g[q][u].get(a);
+        r[q][u].get(b);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          dot = fmaf(a[e], b[e], dot);
-          a[e] *= f;
+          dot[q] = fmaf(a[e], b[e], dot[q]);
+          a[e] *= f[q];
         }
-        g.set(a);
-      } else {
-        g.clear();
+        g[q][u].set(a);
+        g[q][u].store(d0[q] + (v0 + u * lanes) * VEC);
       }
-      if (there) g.store(drows + pos * c + v * VEC);
-    }
+  }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) dot += __shfl_down_sync(0xffffffffu, dot, o);
-    if (lane == 0) store_any(dw, w_dtype, q, dot);
+  for (int q = 0; q < PAIRS; ++q) {
+    for (int o = lanes >> 1; o > 0; o >>= 1) dot[q] += __shfl_down_sync(0xffffffffu, dot[q], o, lanes);
+    if (lane == 0 && q0 + q < pairs) store_any(dw, w_dtype, q0 + q, dot[q]);
   }
 }
 
@@ -600,36 +794,38 @@ int tsb_group_rows(const void* keys, int32_t keys_are_i64, int64_t stride, int64
   }
   if (!workspace || workspace_bytes < sort_plan(n, n_groups).bytes) return TSB_ERR_WORKSPACE;
   const KeySource src{keys, stride, keys_are_i64, (unsigned)n_groups, -1};
-  return run_sort(src, n, SortOut{order, inverse, nullptr}, offsets, workspace, st);
+  return run_sort(src, n, SortOut{order, inverse, nullptr, offsets}, workspace, st);
 }
 
 int tsb_embedding_fwd(const void* table, const void* tokens, int32_t tokens_are_i64, int64_t n, int64_t n_rows, int64_t c,
                       float scale, int32_t dtype, void* out, tsb_stream_t stream) {
   if (n < 0 || n_rows < 0 || c < 1 || (n && (!tokens || !out)) || (n && n_rows && !table)) return TSB_ERR_BAD_ARG;
   if (!good_dtype(dtype)) return TSB_ERR_UNSUPPORTED;
-  if (n_rows > kMaxRows) return TSB_ERR_LIMIT;
+  if (n > kMaxRows || n_rows > kMaxRows || c > kMaxChannels) return TSB_ERR_LIMIT;
   if (n == 0) return TSB_OK;
   const KeySource src{tokens, 1, tokens_are_i64, (unsigned)n_rows, -1};
   const int vec = vector_width(dtype, c, (uintptr_t)table | (uintptr_t)out);
+  const int64_t total = n * (c / vec), blocks = cdiv(total, kThreads * kUnroll);
+  if (blocks > 0x7fffffff) return TSB_ERR_LIMIT;
   return dispatch_pack(dtype, vec, [&](auto tag) -> int {
     using T = typename decltype(tag)::T;
     constexpr int VEC = decltype(tag)::VEC;
-    embed_kernel<T, VEC><<<grid_for(n * (c / VEC), 256, 32), 256, 0, as_stream(stream)>>>((const T*)table, src, n, c, scale, (T*)out);
+    embed_kernel<T, VEC><<<(unsigned)blocks, kThreads, 0, as_stream(stream)>>>((const T*)table, src, total, row_split(c / VEC), scale,
+                                                                               (T*)out);
     TSB_LAUNCH_CHECK();
     return TSB_OK;
   });
 }
 
 size_t tsb_embedding_bwd_workspace_bytes(int64_t n, int64_t n_rows, int64_t c, int32_t dtype) {
-  if (n < 1 || n_rows < 1 || c < 1 || n > kMaxRows || n_rows > kMaxRows || !good_dtype(dtype)) return 256;
-  // the widest vector has the fewest threads per worker and with them the shortest, most numerous workers
-  size_t partials = 0;
+  if (n < 1 || n_rows < 1 || c < 1 || n > kMaxRows || n_rows > kMaxRows || c > kMaxChannels || !good_dtype(dtype)) return 256;
+  size_t partials = 0;      // of the vector width that leaves the most
   for (int vec = 1; vec <= 16 / (int)dtype_size(dtype); vec *= 2) {
     if (c % vec) continue;
-    const size_t b = align_up((size_t)embed_plan(n, n_rows, c, dtype, vec).workers * c * sizeof(float), 256);
+    const size_t b = align_up((size_t)embed_plan(n, n_rows, c, vec).blocks * c * sizeof(float), 256);
     if (b > partials) partials = b;
   }
-  return align_up(sort_plan(n, n_rows).bytes, 256) + 2 * align_up((size_t)n * 4, 256) + 2 * partials;
+  return sort_plan(n, n_rows).bytes + 2 * align_up((size_t)n * 4, 256) + 2 * partials;
 }
 
 int tsb_embedding_bwd(const void* grad, const void* tokens, int32_t tokens_are_i64, int64_t n, int64_t n_rows, int64_t c,
@@ -637,7 +833,7 @@ int tsb_embedding_bwd(const void* grad, const void* tokens, int32_t tokens_are_i
                       tsb_stream_t stream) {
   if (n < 0 || n_rows < 0 || c < 1 || (n && (!tokens || !grad)) || (n_rows && !dtable)) return TSB_ERR_BAD_ARG;
   if (!good_dtype(dtype)) return TSB_ERR_UNSUPPORTED;
-  if (n > kMaxRows || n_rows > kMaxRows) return TSB_ERR_LIMIT;
+  if (n > kMaxRows || n_rows > kMaxRows || c > kMaxChannels) return TSB_ERR_LIMIT;
   cudaStream_t st = as_stream(stream);
   if (n_rows == 0) return TSB_OK;
   if (n == 0) {
@@ -646,32 +842,33 @@ int tsb_embedding_bwd(const void* grad, const void* tokens, int32_t tokens_are_i
   }
   if (!workspace || workspace_bytes < tsb_embedding_bwd_workspace_bytes(n, n_rows, c, dtype)) return TSB_ERR_WORKSPACE;
   const int vec = vector_width(dtype, c, (uintptr_t)grad | (uintptr_t)dtable);
-  EmbedGrad a = embed_plan(n, n_rows, c, dtype, vec);
+  EmbedGrad a = embed_plan(n, n_rows, c, vec);
+  const int zero_rows = c >= 256 ? 64 : 256;      // rows that a block looks up and clears
+  const int64_t blocks = a.blocks + cdiv(n_rows, zero_rows);
+  if (blocks > 0x7fffffff) return TSB_ERR_LIMIT;
   a.scale = scale;
-  char* ws = static_cast<char*>(workspace) + align_up(sort_plan(n, n_rows).bytes, 256);
+  char* ws = static_cast<char*>(workspace) + sort_plan(n, n_rows).bytes;
   unsigned* keys = reinterpret_cast<unsigned*>(ws);
   ws += align_up((size_t)n * 4, 256);
   int* order = reinterpret_cast<int*>(ws);
   ws += align_up((size_t)n * 4, 256);
-  const size_t partials = align_up((size_t)a.workers * c * sizeof(float), 256);
   a.keys = keys;
   a.order = order;
   a.head = reinterpret_cast<float*>(ws);
-  a.tail = reinterpret_cast<float*>(ws + partials);
+  a.tail = reinterpret_cast<float*>(ws + align_up((size_t)a.blocks * c * sizeof(float), 256));
   const KeySource src{tokens, 1, tokens_are_i64, (unsigned)n_rows, padding_row};
-  const int rc = run_sort(src, n, SortOut{order, nullptr, keys}, nullptr, workspace, st);
+  const int rc = run_sort(src, n, SortOut{order, nullptr, keys, nullptr}, workspace, st);
   if (rc != TSB_OK) return rc;
   return dispatch_pack(dtype, vec, [&](auto tag) -> int {
     using T = typename decltype(tag)::T;
     constexpr int VEC = decltype(tag)::VEC;
-    const int64_t worker_blocks = cdiv(a.workers, a.per_block);
-    const int zero_rows = c >= 256 ? 16 : 256;      // rows that a block looks up and clears
-    const int64_t blocks = worker_blocks + cdiv(n_rows, zero_rows);
-    if (blocks > 0x7fffffff) return TSB_ERR_LIMIT;
-    embed_grad_kernel<T, VEC><<<(unsigned)blocks, 256, 0, st>>>(a, (const T*)grad, (T*)dtable, worker_blocks, zero_rows);
+    const dim3 grid((unsigned)blocks, (unsigned)cdiv(c / VEC, a.tile));
+    embed_grad_kernel<T, VEC><<<grid, kThreads, 0, st>>>(a, (const T*)grad, (T*)dtable, zero_rows);
     TSB_LAUNCH_CHECK();
-    if (a.workers > 1) {
-      embed_join_kernel<T><<<grid_for(a.workers, 1, 8), 256, 0, st>>>(a, (T*)dtable);
+    if (a.blocks > 1) {
+      const dim3 join((unsigned)(a.blocks - 1), (unsigned)cdiv(c, 256));
+      if (c % 4 == 0) embed_join_kernel<T, 4><<<join, kJoinThreads, 0, st>>>(a, (T*)dtable);
+      else embed_join_kernel<T, 1><<<join, kJoinThreads, 0, st>>>(a, (T*)dtable);
       TSB_LAUNCH_CHECK();
     }
     return TSB_OK;
@@ -682,14 +879,16 @@ int tsb_expert_dispatch(const void* x, const int32_t* inverse, const int32_t* ke
                         int32_t dtype, void* xs, tsb_stream_t stream) {
   if (n < 0 || k < 1 || c < 1 || (n && (!x || !inverse || !kept || !xs))) return TSB_ERR_BAD_ARG;
   if (!good_dtype(dtype)) return TSB_ERR_UNSUPPORTED;
-  if (n > kMaxRows / k) return TSB_ERR_LIMIT;
+  if (n > kMaxRows / k || c > kMaxChannels) return TSB_ERR_LIMIT;
   if (n == 0) return TSB_OK;
   const int vec = vector_width(dtype, c, (uintptr_t)x | (uintptr_t)xs);
+  const int64_t total = n * (c / vec), blocks = cdiv(total, kThreads * 2);
+  if (blocks > 0x7fffffff) return TSB_ERR_LIMIT;
   return dispatch_pack(dtype, vec, [&](auto tag) -> int {
     using T = typename decltype(tag)::T;
     constexpr int VEC = decltype(tag)::VEC;
-    dispatch_kernel<T, VEC><<<grid_for(n * k * (c / VEC), 256, 32), 256, 0, as_stream(stream)>>>((const T*)x, inverse, kept, n * k, k,
-                                                                                                c, (T*)xs);
+    dispatch_kernel<T, VEC><<<(unsigned)blocks, kThreads, 0, as_stream(stream)>>>((const T*)x, inverse, kept, total, n * k, k,
+                                                                                  row_split(c / VEC), (T*)xs);
     TSB_LAUNCH_CHECK();
     return TSB_OK;
   });
@@ -699,14 +898,19 @@ int tsb_expert_combine(const void* rows, const void* weights, int32_t weights_dt
                        int64_t n, int32_t k, int64_t c, int32_t dtype, void* out, tsb_stream_t stream) {
   if (n < 0 || k < 1 || c < 1 || (n && (!rows || !inverse || !kept || !out))) return TSB_ERR_BAD_ARG;
   if (!good_dtype(dtype) || (weights && !good_dtype(weights_dtype))) return TSB_ERR_UNSUPPORTED;
-  if (n > kMaxRows / k) return TSB_ERR_LIMIT;
+  if (n > kMaxRows / k || c > kMaxChannels) return TSB_ERR_LIMIT;
   if (n == 0) return TSB_OK;
   const int vec = vector_width(dtype, c, (uintptr_t)rows | (uintptr_t)out);
+  const int64_t total = n * (c / vec), blocks = cdiv(total, kThreads * (k <= 2 ? 4 : 2));
+  if (blocks > 0x7fffffff) return TSB_ERR_LIMIT;
   return dispatch_pack(dtype, vec, [&](auto tag) -> int {
     using T = typename decltype(tag)::T;
     constexpr int VEC = decltype(tag)::VEC;
-    combine_kernel<T, VEC><<<grid_for(n * (c / VEC), 256, 32), 256, 0, as_stream(stream)>>>((const T*)rows, weights, weights_dtype,
-                                                                                          inverse, kept, n, k, c, (T*)out);
+    const auto run = [&](auto kernel) {
+      kernel<<<(unsigned)blocks, kThreads, 0, as_stream(stream)>>>((const T*)rows, weights, weights_dtype, inverse, kept, total, n * k,
+                                                                   k, row_split(c / VEC), (T*)out);
+    };
+    if (k <= 2) run(combine_kernel<T, VEC, 2>); else run(combine_kernel<T, VEC, 4>);
     TSB_LAUNCH_CHECK();
     return TSB_OK;
   });
@@ -718,14 +922,17 @@ int tsb_expert_combine_bwd(const void* dout, const void* rows, const void* weigh
   if (n < 0 || k < 1 || c < 1 || (n && (!dout || !rows || !weights || !inverse || !kept || !drows || !dweights)))
     return TSB_ERR_BAD_ARG;
   if (!good_dtype(dtype) || !good_dtype(weights_dtype)) return TSB_ERR_UNSUPPORTED;
-  if (n > kMaxRows / k) return TSB_ERR_LIMIT;
+  if (n > kMaxRows / k || c > kMaxChannels) return TSB_ERR_LIMIT;
   if (n == 0) return TSB_OK;
   const int vec = vector_width(dtype, c, (uintptr_t)dout | (uintptr_t)rows | (uintptr_t)drows);
+  int lanes = 1;
+  while (lanes < 32 && lanes < c / vec) lanes *= 2;
+  const int64_t blocks = cdiv(n * k, 2 * (kThreads / lanes));
   return dispatch_pack(dtype, vec, [&](auto tag) -> int {
     using T = typename decltype(tag)::T;
     constexpr int VEC = decltype(tag)::VEC;
-    combine_grad_kernel<T, VEC><<<grid_for(n * k * 32, 256, 32), 256, 0, as_stream(stream)>>>(
-        (const T*)dout, (const T*)rows, weights, weights_dtype, inverse, kept, n, k, c, (T*)drows, dweights);
+    combine_grad_kernel<T, VEC><<<(unsigned)blocks, kThreads, 0, as_stream(stream)>>>(
+        (const T*)dout, (const T*)rows, weights, weights_dtype, inverse, kept, n * k, row_split(k), c, lanes, (T*)drows, dweights);
     TSB_LAUNCH_CHECK();
     return TSB_OK;
   });

@@ -80,6 +80,16 @@ inline int dispatch_pack(int dtype, int vec, F&& f) {
   return TSB_ERR_UNSUPPORTED;
 }
 
+// Row and vector of a flat index over rows of `cols` vectors, without a 64-bit division: m = floor(2^64 / cols) + 1 gives the
+// exact quotient while index * cols < 2^64.
+struct RowSplit {
+  uint64_t m;
+  unsigned cols;
+  __device__ __forceinline__ int64_t row(int64_t t) const { return m ? (int64_t)__umul64hi((uint64_t)t, m) : t; }
+};
+inline RowSplit row_split(int64_t cols) { return RowSplit{cols == 1 ? 0 : ~0ull / (uint64_t)cols + 1, (unsigned)cols}; }
+constexpr int64_t kMaxChannels = 1 << 20;      // keeps index * cols of a row split below 2^64
+
 // One value of an array whose type is a run-time argument (parameters, router weights: few values, read once).
 __device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
   if (dtype == TSB_F32) return __ldg(reinterpret_cast<const float*>(p) + i);
