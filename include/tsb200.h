@@ -539,7 +539,7 @@ int tsb_to_dense_bwd(const void* grad_dense, const int32_t* coords, int64_t n, i
 /* Stable grouping of n keys (int32, or int64 when keys_are_i64, `stride` elements apart) into n_groups groups:
  * order int32 [n] = the row at each grouped position, inverse int32 [n] (may be NULL) = the position of each row,
  * offsets int32 [n_groups + 1] = first position of each group.  Keys outside [0, n_groups) come last, in their order,
- * from position offsets[n_groups] on.  n, n_groups < 2^31. */
+ * from position offsets[n_groups] on.  n, n_groups < 2^31.  The workspace may be NULL where its size is 0. */
 size_t tsb_group_rows_workspace_bytes(int64_t n, int64_t n_groups);
 int tsb_group_rows(const void* keys, int32_t keys_are_i64, int64_t stride, int64_t n, int64_t n_groups, int32_t* order,
                    int32_t* inverse, int32_t* offsets, void* workspace, size_t workspace_bytes, tsb_stream_t stream);
@@ -548,15 +548,16 @@ int tsb_group_rows(const void* keys, int32_t keys_are_i64, int64_t stride, int64
  * c / g channels, sample s = the grouped positions offsets[s] .. offsets[s + 1] (int32 [b + 1], ascending), order int32
  * [n] = the row at each position (NULL: the rows are grouped already).  weight, bias [c] of `param_dtype` or NULL.
  * act: 0 none, 1 ReLU, 2 leaky ReLU with `slope`, 3 SiLU.  Rows of no sample become zero.  mean, rstd: fp32 [b, g],
- * what the backward call needs.  A group of one value becomes act(bias).  c <= 65536.
+ * what the backward call needs (both may be NULL here).  A group of one value becomes act(bias).  c <= 65536.  The
+ * workspace may be NULL where its size is 0.
  * Replaces the loop of torchsparse/nn/modules/norm.py:25-57. */
-size_t tsb_group_norm_fwd_workspace_bytes(int64_t n, int64_t c, int64_t g, int64_t b);
+size_t tsb_group_norm_fwd_workspace_bytes(int64_t n, int64_t c, int64_t g, int64_t b, int32_t dtype);
 int tsb_group_norm_fwd(const void* x, const int32_t* order, const int32_t* offsets, const void* weight, const void* bias,
                        int64_t n, int64_t c, int64_t g, int64_t b, float eps, int32_t act, float slope, int32_t dtype,
                        int32_t param_dtype, void* y, float* mean, float* rstd, void* workspace, size_t workspace_bytes,
                        tsb_stream_t stream);
 /* Its gradient: dx [n, c] of `dtype`, dweight and dbias [c] of `param_dtype` (either may be NULL). */
-size_t tsb_group_norm_bwd_workspace_bytes(int64_t n, int64_t c, int64_t g, int64_t b);
+size_t tsb_group_norm_bwd_workspace_bytes(int64_t n, int64_t c, int64_t g, int64_t b, int32_t dtype);
 int tsb_group_norm_bwd(const void* x, const void* dy, const int32_t* order, const int32_t* offsets, const void* weight,
                        const void* bias, const float* mean, const float* rstd, int64_t n, int64_t c, int64_t g, int64_t b,
                        int32_t act, float slope, int32_t dtype, int32_t param_dtype, void* dx, void* dweight, void* dbias,

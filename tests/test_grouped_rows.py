@@ -13,13 +13,13 @@ def test_c_entries_refuse_bad_arguments_before_any_cuda_call():
     assert lib.tsb_group_rows(x, 0, 1, 5, 0, x, None, x, x, 1 << 20, None) == 1
     assert lib.tsb_group_rows(x, 0, -1, 5, 2, x, None, x, x, 1 << 20, None) == 1
     assert lib.tsb_group_rows(x, 0, 1, 1 << 31, 2, x, None, x, x, 1 << 20, None) == 5
-    assert lib.tsb_group_rows(x, 0, 1, 5, 2, x, None, x, x, 0, None) == 3
-    norm = lambda n=4, c=8, g=2, b=1, act=0, dtype=0, p=0, ws=1 << 20: lib.tsb_group_norm_fwd(      # noqa: E731
+    assert lib.tsb_group_rows(x, 0, 1, 5, 600, x, None, x, x, 0, None) == 3
+    norm = lambda n=100_000, c=8, g=2, b=1, act=0, dtype=0, p=0, ws=1 << 26: lib.tsb_group_norm_fwd(      # noqa: E731
         x, None, x, None, None, n, c, g, b, 1e-5, act, 0.1, dtype, p, x, x, x, x, ws, None)
     assert [norm(n=-1), norm(c=0), norm(g=3), norm(g=0), norm(b=-1), norm(act=4)] == [1] * 6
     assert [norm(dtype=3), norm(p=9)] == [2, 2] and norm(ws=0) == 3
     assert [norm(n=1 << 31), norm(c=1 << 17)] == [5, 5]
-    grad = lambda n=4, c=8, g=2, ws=1 << 20, dx=x: lib.tsb_group_norm_bwd(      # noqa: E731
+    grad = lambda n=100_000, c=8, g=2, ws=1 << 26, dx=x: lib.tsb_group_norm_bwd(      # noqa: E731
         x, x, None, x, None, None, x, x, n, c, g, 1, 0, 0.1, 0, 0, dx, None, None, x, ws, None)
     assert [grad(g=3), grad(n=-1), grad(dx=None), grad(ws=0)] == [1, 1, 1, 3]
     assert lib.tsb_embedding_fwd(None, x, 0, 5, 3, 8, 1.0, 0, x, None) == 1
@@ -42,8 +42,9 @@ def test_workspaces_grow_with_the_sizes():
     from torchsparse_b200._lib import lib
 
     assert lib.tsb_group_rows_workspace_bytes(1_000_000, 300) >= 5 * 4_000_000
-    assert lib.tsb_group_norm_fwd_workspace_bytes(1000, 64, 8, 10_000) >= 10_000 * 8 * 8
-    assert lib.tsb_group_norm_bwd_workspace_bytes(1000, 64, 8, 10_000) >= 2 * 10_000 * 64 * 8
+    assert lib.tsb_group_norm_fwd_workspace_bytes(1_000_000, 64, 8, 10_000, 0) >= 10_000 * 8 * 8
+    assert lib.tsb_group_norm_bwd_workspace_bytes(1_000_000, 64, 8, 10_000, 0) >= 2 * 10_000 * 64 * 8
+    assert lib.tsb_group_norm_fwd_workspace_bytes(1000, 64, 8, 1, 0) == 0      # one block per sample and group
     assert lib.tsb_embedding_bwd_workspace_bytes(100_000, 50, 64, 1) > lib.tsb_embedding_bwd_workspace_bytes(1000, 50, 64, 1)
 
 

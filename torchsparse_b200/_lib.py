@@ -83,9 +83,9 @@ SIGNATURES = {
     "tsb_to_dense_bwd": (C.c_int, [P, P, I64, I32, P, I32, P, P]),
     "tsb_group_rows_workspace_bytes": (SZ, [I64, I64]),
     "tsb_group_rows": (C.c_int, [P, I32, I64, I64, I64, P, P, P, P, SZ, P]),
-    "tsb_group_norm_fwd_workspace_bytes": (SZ, [I64, I64, I64, I64]),
+    "tsb_group_norm_fwd_workspace_bytes": (SZ, [I64, I64, I64, I64, I32]),
     "tsb_group_norm_fwd": (C.c_int, [P, P, P, P, P, I64, I64, I64, I64, F32, I32, F32, I32, I32, P, P, P, P, SZ, P]),
-    "tsb_group_norm_bwd_workspace_bytes": (SZ, [I64, I64, I64, I64]),
+    "tsb_group_norm_bwd_workspace_bytes": (SZ, [I64, I64, I64, I64, I32]),
     "tsb_group_norm_bwd": (C.c_int, [P, P, P, P, P, P, P, P, I64, I64, I64, I64, I32, F32, I32, I32, P, P, P, P, SZ, P]),
     "tsb_embedding_fwd": (C.c_int, [P, P, I32, I64, I64, I64, F32, I32, P, P]),
     "tsb_embedding_bwd_workspace_bytes": (SZ, [I64, I64, I64, I32]),

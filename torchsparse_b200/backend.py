@@ -16,6 +16,7 @@ Differences from the reference that callers can see:
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import List, Optional, Sequence, Tuple
 
 import torch
@@ -1264,6 +1265,11 @@ def quantize_unique_cuda(xyz: torch.Tensor, voxel_size: Sequence[float], return_
 # device, which need not be the current device.
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "leaky_relu": 2, "silu": 3}
 _MAX_ROWS = 2 ** 31 - 1
+# workspace sizes depend on sizes alone; at small ones the call costs as much as a lookup saves
+_group_rows_bytes = lru_cache(1024)(lib.tsb_group_rows_workspace_bytes)
+_norm_fwd_bytes = lru_cache(1024)(lib.tsb_group_norm_fwd_workspace_bytes)
+_norm_bwd_bytes = lru_cache(1024)(lib.tsb_group_norm_bwd_workspace_bytes)
+_embed_bwd_bytes = lru_cache(1024)(lib.tsb_embedding_bwd_workspace_bytes)
 
 
 class _Here:
@@ -1283,11 +1289,22 @@ def _on_device_of(t: torch.Tensor):
     return _HERE if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
+def _scratch(nbytes: int, device):
+    """(tensor or None, address or None) of a workspace that may be empty."""
+    if nbytes == 0:
+        return None, None
+    t = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return t, t.data_ptr()
+
+
 def _same_device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
-    _need_cuda(first, *others)
+    if not first.is_cuda:
+        _need_cuda(first)
+    device = first.device
     for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"tensors live on {first.device} and {t.device}")
+        if t is not None and t.device != device:
+            _need_cuda(t)
+            raise ValueError(f"tensors live on {device} and {t.device}")
 
 
 def _index_tensor(t: torch.Tensor, what: str) -> torch.Tensor:
@@ -1296,10 +1313,9 @@ def _index_tensor(t: torch.Tensor, what: str) -> torch.Tensor:
     return t
 
 
-def _int32_vector(t: torch.Tensor, length: int, what: str) -> torch.Tensor:
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != length or not t.is_contiguous():
-        raise ValueError(f"{what} must be a contiguous int32 vector of length {length}")
-    return t
+def _int32_vector(t: torch.Tensor, length: Optional[int], what: str) -> None:
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or (length is not None and t.shape[0] != length):
+        raise ValueError(f"{what} must be a contiguous int32 vector" + ("" if length is None else f" of length {length}"))
 
 
 def group_rows_cuda(keys: torch.Tensor, num_groups: int, want_inverse: bool = False):
@@ -1316,25 +1332,25 @@ def group_rows_cuda(keys: torch.Tensor, num_groups: int, want_inverse: bool = Fa
     order = torch.empty(n, dtype=torch.int32, device=dev)
     inverse = torch.empty(n, dtype=torch.int32, device=dev) if want_inverse else None
     offsets = torch.empty(num_groups + 1, dtype=torch.int32, device=dev)
-    ws = _workspace(lib.tsb_group_rows_workspace_bytes(n, num_groups), dev)
+    nbytes = _group_rows_bytes(n, num_groups)
+    ws, at = _scratch(nbytes, dev)
     with _on_device_of(keys):
-        check(lib.tsb_group_rows(_p(keys), int(keys.dtype == torch.int64), keys.stride(0), n, num_groups, _p(order),
-                                 _p(inverse), _p(offsets), _p(ws), ws.numel(), _stream()), "group_rows")
+        check(lib.tsb_group_rows(keys.data_ptr(), keys.dtype == torch.int64, keys.stride(0), n, num_groups, order.data_ptr(),
+                                 _p(inverse), offsets.data_ptr(), at, nbytes, _stream()), "group_rows")
     return order, inverse, offsets
 
 
 def _norm_args(feats, order, offsets, num_groups, weight, bias, activation):
-    """Checked arguments of the two group norm calls: (num_groups, activation code, parameter dtype code)."""
+    """Checked arguments of the two group norm calls: (activation code, feature dtype code, parameter dtype code)."""
     _same_device(feats, order, offsets, weight, bias)
     if feats.dim() != 2 or feats.shape[1] < 1:
         raise ValueError(f"group_norm expects features [N, C], not {tuple(feats.shape)}")
     n, c = feats.shape
-    num_groups = int(num_groups)
     if num_groups < 1 or c % num_groups != 0:
         raise ValueError(f"{c} channels do not divide into {num_groups} groups")
-    if offsets.dim() != 1 or offsets.shape[0] < 1:
+    _int32_vector(offsets, None, "offsets")
+    if offsets.shape[0] < 1:
         raise ValueError("offsets must hold the first row of every sample and the end of the last")
-    _int32_vector(offsets, offsets.shape[0], "offsets")
     if order is not None:
         _int32_vector(order, n, "order")
     code = None
@@ -1347,54 +1363,58 @@ def _norm_args(feats, order, offsets, num_groups, weight, bias, activation):
             code = _dtype_code(p)
     if activation not in ACTIVATIONS:
         raise ValueError(f"unknown activation {activation!r}: one of {sorted(k for k in ACTIVATIONS if k)}")
-    return num_groups, ACTIVATIONS[activation], _lib.TSB_F32 if code is None else code
+    return ACTIVATIONS[activation], _dtype_code(feats), _lib.TSB_F32 if code is None else code
 
 
 def group_norm_forward_cuda(feats: torch.Tensor, order: Optional[torch.Tensor], offsets: torch.Tensor, num_groups: int,
                             weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5,
-                            activation: Optional[str] = None, negative_slope: float = 0.01):
-    """``(y, mean, rstd)`` of ``act(group_norm(feats))`` over the samples ``offsets`` delimits; mean and rstd are fp32
-    [samples, num_groups]."""
-    num_groups, act, code = _norm_args(feats, order, offsets, num_groups, weight, bias, activation)
-    dtype = _dtype_code(feats)
+                            activation: Optional[str] = None, negative_slope: float = 0.01, want_stats: bool = True):
+    """``(y, stats)`` of ``act(group_norm(feats))`` over the samples ``offsets`` delimits; stats is fp32
+    [2, samples, num_groups], the means and the reciprocal deviations (None unless wanted)."""
+    act, dtype, code = _norm_args(feats, order, offsets, num_groups, weight, bias, activation)
     feats = feats.contiguous()
-    weight, bias = (None if p is None else p.contiguous() for p in (weight, bias))
+    weight, bias = weight if weight is None else weight.contiguous(), bias if bias is None else bias.contiguous()
     n, c = feats.shape
-    samples = offsets.shape[0] - 1
+    samples, device = offsets.shape[0] - 1, feats.device
     y = torch.empty_like(feats)
-    stats = torch.empty((2, samples, num_groups), dtype=torch.float32, device=feats.device)
-    mean, rstd = stats[0], stats[1]
-    ws = _workspace(lib.tsb_group_norm_fwd_workspace_bytes(n, c, num_groups, samples), feats.device)
+    stats = mean = rstd = None
+    if want_stats:
+        stats = torch.empty((2, samples, num_groups), dtype=torch.float32, device=device)
+        mean = stats.data_ptr()
+        rstd = mean + 4 * samples * num_groups
+    nbytes = _norm_fwd_bytes(n, c, num_groups, samples, dtype)
+    ws, at = _scratch(nbytes, device)
     with _on_device_of(feats):
-        check(lib.tsb_group_norm_fwd(_p(feats), _p(order), _p(offsets), _p(weight), _p(bias), n, c, num_groups, samples,
-                                     float(eps), act, float(negative_slope), dtype, code, _p(y), _p(mean), _p(rstd), _p(ws),
-                                     ws.numel(), _stream()), "group_norm")
-    return y, mean, rstd
+        check(lib.tsb_group_norm_fwd(feats.data_ptr(), _p(order), offsets.data_ptr(), _p(weight), _p(bias), n, c, num_groups,
+                                     samples, eps, act, negative_slope, dtype, code, y.data_ptr(), mean, rstd, at, nbytes,
+                                     _stream()), "group_norm")
+    return y, stats
 
 
 def group_norm_backward_cuda(feats: torch.Tensor, grad: torch.Tensor, order: Optional[torch.Tensor], offsets: torch.Tensor,
                              num_groups: int, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor],
-                             mean: torch.Tensor, rstd: torch.Tensor, activation: Optional[str] = None,
-                             negative_slope: float = 0.01):
+                             stats: torch.Tensor, activation: Optional[str] = None, negative_slope: float = 0.01):
     """``(dfeats, dweight or None, dbias or None)`` of ``group_norm_forward_cuda``."""
-    num_groups, act, code = _norm_args(feats, order, offsets, num_groups, weight, bias, activation)
-    _same_device(feats, grad, mean, rstd)
+    act, dtype, code = _norm_args(feats, order, offsets, num_groups, weight, bias, activation)
+    _same_device(feats, grad, stats)
     if grad.shape != feats.shape or grad.dtype != feats.dtype:
         raise ValueError("the gradient must have the features' shape and dtype")
     n, c = feats.shape
-    samples = offsets.shape[0] - 1
-    for t in (mean, rstd):
-        if t.dtype != torch.float32 or tuple(t.shape) != (samples, num_groups) or not t.is_contiguous():
-            raise ValueError("mean and rstd must be what the forward call returned")
+    samples, device = offsets.shape[0] - 1, feats.device
+    if stats.dtype != torch.float32 or tuple(stats.shape) != (2, samples, num_groups) or not stats.is_contiguous():
+        raise ValueError("stats must be what the forward call returned")
+    mean = stats.data_ptr()
     feats, grad = feats.contiguous(), grad.contiguous()
-    weight, bias = (None if p is None else p.contiguous() for p in (weight, bias))
+    weight, bias = weight if weight is None else weight.contiguous(), bias if bias is None else bias.contiguous()
     dx = torch.empty_like(feats)
-    dweight, dbias = (None if p is None else torch.empty_like(p) for p in (weight, bias))
-    ws = _workspace(lib.tsb_group_norm_bwd_workspace_bytes(n, c, num_groups, samples), feats.device)
+    dweight = None if weight is None else torch.empty_like(weight)
+    dbias = None if bias is None else torch.empty_like(bias)
+    nbytes = _norm_bwd_bytes(n, c, num_groups, samples, dtype)
+    ws, at = _scratch(nbytes, device)
     with _on_device_of(feats):
-        check(lib.tsb_group_norm_bwd(_p(feats), _p(grad), _p(order), _p(offsets), _p(weight), _p(bias), _p(mean), _p(rstd), n, c,
-                                     num_groups, samples, act, float(negative_slope), _dtype_code(feats), code, _p(dx),
-                                     _p(dweight), _p(dbias), _p(ws), ws.numel(), _stream()), "group_norm_backward")
+        check(lib.tsb_group_norm_bwd(feats.data_ptr(), grad.data_ptr(), _p(order), offsets.data_ptr(), _p(weight), _p(bias), mean,
+                                     mean + 4 * samples * num_groups, n, c, num_groups, samples, act, negative_slope, dtype, code,
+                                     dx.data_ptr(), _p(dweight), _p(dbias), at, nbytes, _stream()), "group_norm_backward")
     return dx, dweight, dbias
 
 
@@ -1408,8 +1428,8 @@ def embedding_forward_cuda(indices: torch.Tensor, table: torch.Tensor, scale: fl
     table, indices = table.contiguous(), indices.contiguous()
     out = torch.empty((indices.shape[0], table.shape[1]), dtype=table.dtype, device=table.device)
     with _on_device_of(table):
-        check(lib.tsb_embedding_fwd(_p(table), _p(indices), int(indices.dtype == torch.int64), indices.shape[0], table.shape[0],
-                                    table.shape[1], float(scale), dtype, _p(out), _stream()), "embedding")
+        check(lib.tsb_embedding_fwd(table.data_ptr(), indices.data_ptr(), indices.dtype == torch.int64, indices.shape[0],
+                                    table.shape[0], table.shape[1], scale, dtype, out.data_ptr(), _stream()), "embedding")
     return out
 
 
@@ -1426,11 +1446,12 @@ def embedding_backward_cuda(grad: torch.Tensor, indices: torch.Tensor, num_rows:
     grad, indices = grad.contiguous(), indices.contiguous()
     n, c = grad.shape
     out = torch.empty((num_rows, c), dtype=grad.dtype, device=grad.device)
-    ws = _workspace(lib.tsb_embedding_bwd_workspace_bytes(n, num_rows, c, dtype), grad.device)
+    nbytes = _embed_bwd_bytes(n, num_rows, c, dtype)
+    ws, at = _scratch(nbytes, grad.device)
     with _on_device_of(grad):
-        check(lib.tsb_embedding_bwd(_p(grad), _p(indices), int(indices.dtype == torch.int64), n, num_rows, c, float(scale),
-                                    -1 if padding_idx is None else int(padding_idx), dtype, _p(out), _p(ws), ws.numel(),
-                                    _stream()), "embedding_backward")
+        check(lib.tsb_embedding_bwd(grad.data_ptr(), indices.data_ptr(), indices.dtype == torch.int64, n, num_rows, c, scale,
+                                    -1 if padding_idx is None else padding_idx, dtype, out.data_ptr(), at, nbytes, _stream()),
+              "embedding_backward")
     return out
 
 
@@ -1438,9 +1459,9 @@ def _expert_args(inverse: torch.Tensor, offsets: torch.Tensor):
     """(N, k, address of the number of kept choices) of the plan ``group_rows_cuda`` made of [N, k] choices."""
     if inverse.dim() != 2 or inverse.dtype != torch.int32 or not inverse.is_contiguous() or inverse.shape[1] < 1:
         raise ValueError("inverse must be contiguous int32 [N, k]")
-    if offsets.dim() != 1 or offsets.shape[0] < 2:
+    _int32_vector(offsets, None, "offsets")
+    if offsets.shape[0] < 2:
         raise ValueError("offsets must hold the first position of every expert and the end of the last")
-    _int32_vector(offsets, offsets.shape[0], "offsets")
     return inverse.shape[0], inverse.shape[1], offsets.data_ptr() + 4 * (offsets.shape[0] - 1)
 
 

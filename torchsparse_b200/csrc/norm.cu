@@ -593,6 +593,253 @@ __global__ void __launch_bounds__(256) norm_grad_params_kernel(Norm a, const flo
   }
 }
 
+// ------------------------------------------------------------------------------------------------ small samples
+// One block per sample and group, with the group's values in registers between the sums and the result: one launch, one
+// read.  What a long sample has beyond the registers is read again, so every size is served; norm_small() says when.
+constexpr int kSmallThreads = 512;
+constexpr int kSmallVectors = 4096;      // vectors of a sample and group that a block holds at most in the backward pass
+
+// sum over the block, the same bits in every thread; `part`: one float per warp
+__device__ __forceinline__ float block_sum(float v, float* part) {
+  v = warp_sum(v);
+  __syncthreads();      // the last use of part is over
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.f;
+  for (int i = 0; i < (int)(blockDim.x >> 5); ++i) v += part[i];
+  return v;
+}
+
+template <typename T, int VEC, bool ORDERED>
+__global__ void __launch_bounds__(kSmallThreads) norm_small_kernel(Norm a, const T* __restrict__ x, T* __restrict__ y,
+                                                                   float* __restrict__ mean_, float* __restrict__ rstd_) {
+  constexpr int R = 2 * kSmallVectors / kSmallThreads;
+  __shared__ float part[kSmallThreads / 32];
+  const int dv = a.d / VEC, gr = blockIdx.x, s = blockIdx.y;
+  const int lanes = blockDim.x / dv, lane = threadIdx.x / dv, k0 = gr * a.d + (threadIdx.x - lane * dv) * VEC;
+  const bool on = lane < lanes;
+  const T* xc = x + k0;
+  T* yc = y + k0;
+  if (s == 0 && on) clear_outside<T, VEC, ORDERED>(a, 0, a.n, lane, lanes, yc);
+  const int64_t lo = a.b ? offset_of(a, s) : 0, hi = a.b ? offset_of(a, s + 1) : 0, first = on ? lo + lane : hi;
+  const int64_t rest = first + (int64_t)R * lanes;
+  Pack<T, VEC> v[R];
+  float sum = 0.f;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int64_t p = first + r * lanes, row = p < hi ? row_at<ORDERED>(a, p) : -1;
+    v[r].clear();
+    if (row >= 0) v[r].load(xc + row * a.c);
+  }
+  auto each = [&](auto&& f) {      // the rows beyond the registers
+    for (int64_t p = rest; p < hi; p += lanes) {
+      const int64_t row = row_at<ORDERED>(a, p);
+      Pack<T, VEC> q;
+      q.clear();
+      if (row >= 0) q.load(xc + row * a.c);
+      f(q, row);
+    }
+  };
+  const auto add = [&](const Pack<T, VEC>& q) {
+    float f[VEC];
+    q.get(f);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) sum += f[e];
+  };
+#pragma unroll
+  for (int r = 0; r < R; ++r) add(v[r]);      // zeros where there is no row
+  each([&](const Pack<T, VEC>& q, int64_t) { add(q); });
+  const float count = (float)max(hi - lo, (int64_t)1) * a.d;
+  const float mean = block_sum(sum, part) / count;
+  float sq = 0.f;
+  const auto square = [&](const Pack<T, VEC>& q) {
+    float f[VEC];
+    q.get(f);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) sq = fmaf(f[e] - mean, f[e] - mean, sq);
+  };
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    forget(v[r].raw);
+    if (first + r * lanes < hi) square(v[r]);
+  }
+  each([&](const Pack<T, VEC>& q, int64_t) { square(q); });
+  const float rstd = 1.f / sqrtf(block_sum(sq, part) / count + a.eps);
+  if (threadIdx.x == 0 && mean_ && a.b) {
+    mean_[(int64_t)s * a.g + gr] = mean;
+    rstd_[(int64_t)s * a.g + gr] = rstd;
+  }
+  if (!on) return;
+  float w[VEC], b[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    w[e] = rstd * (a.w ? load_any(a.w, a.p_dtype, k0 + e) : 1.f);
+    b[e] = a.bias ? load_any(a.bias, a.p_dtype, k0 + e) : 0.f;
+  }
+  const auto put = [&](Pack<T, VEC>& q, int64_t row) {
+    if (row < 0) return;
+    float z[VEC];
+    q.get(z);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) z[e] = fmaf(z[e] - mean, w[e], b[e]);
+    activate(z, a.act, a.slope);
+    q.set(z);
+    q.store(yc + row * a.c);
+  };
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    forget(v[r].raw);
+    if (first + r * lanes < hi) put(v[r], row_at<ORDERED>(a, first + r * lanes));
+  }
+  each([&](Pack<T, VEC>& q, int64_t row) { put(q, row); });
+}
+
+// by_channel[s][k] receives the sums of dz and dz * xhat where there are several samples; one writes dw and db itself
+template <typename T, int VEC, bool ORDERED>
+__global__ void __launch_bounds__(kSmallThreads) norm_small_grad_kernel(Norm a, const T* __restrict__ x, const T* __restrict__ dy,
+                                                                        const float* __restrict__ mean_,
+                                                                        const float* __restrict__ rstd_,
+                                                                        float2* __restrict__ by_channel, T* __restrict__ dx,
+                                                                        void* __restrict__ dw, void* __restrict__ db) {
+  constexpr int R = kSmallVectors / kSmallThreads;
+  __shared__ float part[kSmallThreads / 32];
+  __shared__ float2 sums[VEC * kSmallThreads];
+  const int dv = a.d / VEC, gr = blockIdx.x, s = blockIdx.y;
+  const int lanes = blockDim.x / dv, lane = threadIdx.x / dv, col = threadIdx.x - lane * dv, k0 = gr * a.d + col * VEC;
+  const bool on = lane < lanes;
+  const T *xc = x + k0, *gc = dy + k0;
+  T* dc = dx + k0;
+  if (s == 0 && on) clear_outside<T, VEC, ORDERED>(a, 0, a.n, lane, lanes, dc);
+  const int64_t lo = a.b ? offset_of(a, s) : 0, hi = a.b ? offset_of(a, s + 1) : 0, first = on ? lo + lane : hi;
+  const int64_t rest = first + (int64_t)R * lanes;
+  const float mean = a.b ? __ldg(mean_ + (int64_t)s * a.g + gr) : 0.f, rstd = a.b ? __ldg(rstd_ + (int64_t)s * a.g + gr) : 0.f;
+  float w[VEC], b[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    w[e] = rstd * (on && a.w ? load_any(a.w, a.p_dtype, k0 + e) : 1.f);
+    b[e] = on && a.bias ? load_any(a.bias, a.p_dtype, k0 + e) : 0.f;
+  }
+  Pack<T, VEC> vx[R], vg[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int64_t p = first + r * lanes, row = p < hi ? row_at<ORDERED>(a, p) : -1;
+    vx[r].clear();
+    vg[r].clear();
+    if (row >= 0) {
+      vx[r].load(xc + row * a.c);
+      vg[r].load(gc + row * a.c);
+    }
+  }
+  auto each = [&](auto&& f) {      // the rows beyond the registers
+    for (int64_t p = rest; p < hi; p += lanes) {
+      const int64_t row = row_at<ORDERED>(a, p);
+      if (row < 0) continue;
+      Pack<T, VEC> qx, qg;
+      qx.load(xc + row * a.c);
+      qg.load(gc + row * a.c);
+      f(qx, qg, row);
+    }
+  };
+  const auto terms = [&](const Pack<T, VEC>& qx, const Pack<T, VEC>& qg, float (&h)[VEC], float (&g)[VEC]) {
+    float z[VEC];
+    qx.get(h);
+    qg.get(g);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      h[e] -= mean;
+      z[e] = fmaf(h[e], w[e], b[e]);
+    }
+    activate_grad(z, g, a.act, a.slope);
+  };
+  float s1[VEC], s2[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) s1[e] = s2[e] = 0.f;
+  const auto add = [&](const Pack<T, VEC>& qx, const Pack<T, VEC>& qg) {
+    float h[VEC], g[VEC];
+    terms(qx, qg, h, g);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      s1[e] += g[e];
+      s2[e] = fmaf(g[e], h[e], s2[e]);
+    }
+  };
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (first + r * lanes < hi) add(vx[r], vg[r]);
+  each([&](const Pack<T, VEC>& qx, const Pack<T, VEC>& qg, int64_t) { add(qx, qg); });
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) sums[e * kSmallThreads + threadIdx.x] = make_float2(s1[e], s2[e]);
+  __syncthreads();
+  // the lanes of a channel: slices of them by several threads, then the slices by one
+  const int slices = max((int)blockDim.x / a.d, 1);
+  float m1 = 0.f, m2 = 0.f;
+  for (int k = threadIdx.x % a.d; k < a.d; k += blockDim.x) {
+    const int slice = threadIdx.x / a.d;
+    float u = 0.f, v = 0.f;
+    if (slice < slices) {
+      for (int l = slice; l < lanes; l += slices) {
+        const float2 f = sums[k % VEC * kSmallThreads + l * dv + k / VEC];
+        u += f.x;
+        v += f.y;
+      }
+      // w of this channel times its sums, over the whole group: m1 and m2
+      const float wk = a.w ? load_any(a.w, a.p_dtype, gr * a.d + k) : 1.f;
+      m1 = fmaf(wk, u, m1);
+      m2 = fmaf(wk * rstd, v, m2);
+    }
+    s1[0] = u;
+    s2[0] = v;
+  }
+  m1 = block_sum(m1, part);      // its barriers also end the reads of sums[]
+  m2 = block_sum(m2, part);
+  const float count = (float)max(hi - lo, (int64_t)1) * a.d;
+  const float k1 = rstd * (m1 / count), k2 = rstd * rstd * (m2 / count);
+  if (slices > 1) {
+    if ((int)threadIdx.x < slices * a.d) sums[threadIdx.x] = make_float2(s1[0], s2[0]);
+    __syncthreads();
+  }
+  for (int k = threadIdx.x; k < a.d; k += blockDim.x) {
+    float u = 0.f, v = 0.f;
+    if (slices > 1) {
+      for (int i = 0; i < slices; ++i) {
+        u += sums[i * a.d + k].x;
+        v += sums[i * a.d + k].y;
+      }
+    } else {      // one slice: all lanes of a channel that this thread summed above
+      for (int l = 0; l < lanes; ++l) {
+        const float2 f = sums[k % VEC * kSmallThreads + l * dv + k / VEC];
+        u += f.x;
+        v += f.y;
+      }
+    }
+    v *= rstd;
+    const int ch = gr * a.d + k;
+    if (a.b > 1) {
+      by_channel[(int64_t)s * a.c + ch] = make_float2(u, v);
+    } else {
+      if (db) store_any(db, a.p_dtype, ch, u);
+      if (dw) store_any(dw, a.p_dtype, ch, v);
+    }
+  }
+  if (!on) return;
+  const auto put = [&](const Pack<T, VEC>& qx, Pack<T, VEC>& qg, int64_t row) {
+    if (row < 0) return;
+    float h[VEC], g[VEC];
+    terms(qx, qg, h, g);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) g[e] = fmaf(g[e], w[e], -fmaf(h[e], k2, k1));
+    qg.set(g);
+    qg.store(dc + row * a.c);
+  };
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    forget(vx[r].raw);
+    forget(vg[r].raw);
+    if (first + r * lanes < hi) put(vx[r], vg[r], row_at<ORDERED>(a, first + r * lanes));
+  }
+  each([&](const Pack<T, VEC>& qx, Pack<T, VEC>& qg, int64_t row) { put(qx, qg, row); });
+}
+
 // ------------------------------------------------------------------------------------------------ host
 bool good_dtype(int dtype) { return dtype == TSB_F32 || dtype == TSB_F16 || dtype == TSB_BF16; }
 
@@ -648,10 +895,43 @@ int norm_vector(int dtype, int64_t c, int64_t g, uintptr_t bits) {
   return vec * (int)dtype_size(dtype) == 16 && d % part != 0 ? vec / 2 : vec;
 }
 
-// slots of the forward statistics for the vector width that needs the most column tiles
+// One block per sample and group where its values fit the block's registers (a sample of twice the mean length still
+// does) and the whole input is small: three launches that pass through memory cost 13 us, one block reads 64 KB in three.
+bool norm_small(int64_t n, int64_t c, int64_t g, int64_t b, int dtype) {
+  const int64_t d = c / g, dv = d / vector_width(dtype, d, 0);
+  const int64_t rows = b > 1 ? 2 * cdiv(n, b) : n;
+  return b <= 65535 && dv <= 64 && rows * dv <= kSmallVectors && n * c * (int64_t)dtype_size(dtype) <= (8 << 20);
+}
+
+// threads of a block of the small kernels: two vectors each for a sample of mean length
+int small_threads(int64_t n, int64_t b, int dv) {
+  const int64_t want = cdiv(cdiv(n, b > 1 ? b : 1) * dv, 2 * 32) * 32;
+  return (int)(want < 128 ? 128 : want > kSmallThreads ? kSmallThreads : want);
+}
+
+template <typename F>
+int dispatch_small(int dtype, int vec, bool ordered, F&& f) {
+  return dispatch_pack(dtype, vec, [&](auto tag) -> int { return ordered ? f(tag, std::true_type()) : f(tag, std::false_type()); });
+}
+
+// parts of the workspaces, for the vector width that needs the most column tiles
 size_t fwd_slot_bytes(int64_t n, int64_t c, int64_t g, int64_t b) {
-  const int64_t tiles = cdiv(c, kNormThreads);
-  return align_up((size_t)tiles * (kNormBlocks + b) * g * sizeof(float2), 256);
+  return align_up((size_t)cdiv(c, kNormThreads) * (kNormBlocks + b) * g * sizeof(float2), 256);
+}
+size_t stat_bytes(int64_t g, int64_t b) { return align_up((size_t)b * g * sizeof(float), 256); }
+size_t channel_bytes(int64_t c, int64_t b) { return align_up((size_t)b * c * sizeof(float2), 256); }
+
+Norm norm_args(Norm a, const int32_t* order, const int32_t* offsets, const void* weight, const void* bias, int param_dtype,
+               float eps, int act, float slope) {
+  a.order = order;
+  a.offsets = offsets;
+  a.w = weight;
+  a.bias = bias;
+  a.p_dtype = param_dtype;
+  a.eps = eps;
+  a.act = act;
+  a.slope = slope;
+  return a;
 }
 
 }  // namespace
@@ -661,9 +941,9 @@ using namespace tsb;
 
 extern "C" {
 
-size_t tsb_group_norm_fwd_workspace_bytes(int64_t n, int64_t c, int64_t g, int64_t b) {
-  if (check_norm(n, c, g, 0, nullptr, 0, 0, 0) != TSB_OK || b < 0) return 0;
-  return fwd_slot_bytes(n, c, g, b);
+size_t tsb_group_norm_fwd_workspace_bytes(int64_t n, int64_t c, int64_t g, int64_t b, int32_t dtype) {
+  if (check_norm(n, c, g, 0, nullptr, dtype, 0, 0) != TSB_OK || b < 0 || norm_small(n, c, g, b, dtype)) return 0;
+  return fwd_slot_bytes(n, c, g, b) + 2 * stat_bytes(g, b);
 }
 
 int tsb_group_norm_fwd(const void* x, const int32_t* order, const int32_t* offsets, const void* weight, const void* bias,
@@ -672,20 +952,31 @@ int tsb_group_norm_fwd(const void* x, const int32_t* order, const int32_t* offse
                        tsb_stream_t stream) {
   const int bad = check_norm(n, c, g, b, offsets, dtype, param_dtype, act);
   if (bad != TSB_OK) return bad;
-  if ((n && (!x || !y)) || (b && (!mean || !rstd))) return TSB_ERR_BAD_ARG;
+  if ((n && (!x || !y)) || !mean != !rstd) return TSB_ERR_BAD_ARG;
   cudaStream_t st = as_stream(stream);
-  if (workspace_bytes < fwd_slot_bytes(n, c, g, b) || !workspace) return TSB_ERR_WORKSPACE;
-  const int vec = norm_vector(dtype, c, g, (uintptr_t)x | (uintptr_t)y);
-  Norm a = norm_shape(n, c, g, b, vec);
-  a.order = order;
-  a.offsets = offsets;
-  a.w = weight;
-  a.bias = bias;
-  a.p_dtype = param_dtype;
-  a.eps = eps;
-  a.act = act;
-  a.slope = slope;
-  float2* slots = static_cast<float2*>(workspace);
+  const uintptr_t bits = (uintptr_t)x | (uintptr_t)y;
+  if (norm_small(n, c, g, b, dtype)) {
+    const int vec = vector_width(dtype, c / g, bits), dv = (int)(c / g) / vec;      // at most 512: 64 of the widest vectors
+    const Norm a = norm_args(norm_shape(n, c, g, b, vec), order, offsets, weight, bias, param_dtype, eps, act, slope);
+    const dim3 grid((unsigned)g, (unsigned)(b > 1 ? b : 1));
+    const int threads = dv > 128 ? kSmallThreads : small_threads(n, b, dv);
+    return dispatch_small(dtype, vec, order != nullptr, [&](auto tag, auto ordered) -> int {
+      using T = typename decltype(tag)::T;
+      norm_small_kernel<T, decltype(tag)::VEC, decltype(ordered)::value>
+          <<<grid, threads, 0, st>>>(a, (const T*)x, (T*)y, mean, rstd);
+      TSB_LAUNCH_CHECK();
+      return TSB_OK;
+    });
+  }
+  if (workspace_bytes < fwd_slot_bytes(n, c, g, b) + 2 * stat_bytes(g, b) || !workspace) return TSB_ERR_WORKSPACE;
+  const int vec = norm_vector(dtype, c, g, bits);
+  const Norm a = norm_args(norm_shape(n, c, g, b, vec), order, offsets, weight, bias, param_dtype, eps, act, slope);
+  char* ws = static_cast<char*>(workspace);
+  float2* slots = reinterpret_cast<float2*>(ws);
+  if (!mean) {
+    mean = reinterpret_cast<float*>(ws + fwd_slot_bytes(n, c, g, b));
+    rstd = reinterpret_cast<float*>(ws + fwd_slot_bytes(n, c, g, b) + stat_bytes(g, b));
+  }
   const int tiles = (int)cdiv(a.cols, a.tile);
   const dim3 grid((unsigned)a.nblk, (unsigned)tiles);
   return dispatch_norm(dtype, vec, a.d, order != nullptr, [&](auto tag, auto each, auto ordered) -> int {
@@ -708,10 +999,10 @@ int tsb_group_norm_fwd(const void* x, const int32_t* order, const int32_t* offse
   });
 }
 
-size_t tsb_group_norm_bwd_workspace_bytes(int64_t n, int64_t c, int64_t g, int64_t b) {
-  if (check_norm(n, c, g, 0, nullptr, 0, 0, 0) != TSB_OK || b < 0) return 0;
-  return align_up((size_t)(kNormBlocks + b) * c * sizeof(float2), 256) + align_up((size_t)b * c * sizeof(float2), 256) +
-         align_up((size_t)b * g * sizeof(float2), 256) + 256;
+size_t tsb_group_norm_bwd_workspace_bytes(int64_t n, int64_t c, int64_t g, int64_t b, int32_t dtype) {
+  if (check_norm(n, c, g, 0, nullptr, dtype, 0, 0) != TSB_OK || b < 0) return 0;
+  if (norm_small(n, c, g, b, dtype)) return b > 1 ? channel_bytes(c, b) : 0;
+  return channel_bytes(c, kNormBlocks + b) + channel_bytes(c, b) + channel_bytes(g, b);
 }
 
 int tsb_group_norm_bwd(const void* x, const void* dy, const int32_t* order, const int32_t* offsets, const void* weight,
@@ -722,21 +1013,33 @@ int tsb_group_norm_bwd(const void* x, const void* dy, const int32_t* order, cons
   if (bad != TSB_OK) return bad;
   if ((n && (!x || !dy || !dx)) || (b && (!mean || !rstd))) return TSB_ERR_BAD_ARG;
   cudaStream_t st = as_stream(stream);
-  if (workspace_bytes < tsb_group_norm_bwd_workspace_bytes(n, c, g, b) || !workspace) return TSB_ERR_WORKSPACE;
-  const int vec = norm_vector(dtype, c, g, (uintptr_t)x | (uintptr_t)dy | (uintptr_t)dx);
-  Norm a = norm_shape(n, c, g, b, vec);
-  a.order = order;
-  a.offsets = offsets;
-  a.w = weight;
-  a.bias = bias;
-  a.p_dtype = param_dtype;
-  a.act = act;
-  a.slope = slope;
+  const size_t need = tsb_group_norm_bwd_workspace_bytes(n, c, g, b, dtype);
+  if (workspace_bytes < need || (need && !workspace)) return TSB_ERR_WORKSPACE;
+  const uintptr_t bits = (uintptr_t)x | (uintptr_t)dy | (uintptr_t)dx;
   char* ws = static_cast<char*>(workspace);
+  if (norm_small(n, c, g, b, dtype)) {
+    const int vec = vector_width(dtype, c / g, bits), dv = (int)(c / g) / vec;      // at most 512: 64 of the widest vectors
+    const Norm a = norm_args(norm_shape(n, c, g, b, vec), order, offsets, weight, bias, param_dtype, 0.f, act, slope);
+    const dim3 grid((unsigned)g, (unsigned)(b > 1 ? b : 1));
+    const int threads = dv > 128 ? kSmallThreads : small_threads(n, b, dv);
+    float2* by_channel = reinterpret_cast<float2*>(ws);
+    return dispatch_small(dtype, vec, order != nullptr, [&](auto tag, auto ordered) -> int {
+      using T = typename decltype(tag)::T;
+      norm_small_grad_kernel<T, decltype(tag)::VEC, decltype(ordered)::value>
+          <<<grid, threads, 0, st>>>(a, (const T*)x, (const T*)dy, mean, rstd, by_channel, (T*)dx, dweight, dbias);
+      TSB_LAUNCH_CHECK();
+      if (b > 1 && (dweight || dbias)) {
+        norm_grad_params_kernel<<<(unsigned)cdiv(a.c, 32), 256, 0, st>>>(a, by_channel, dweight, dbias);
+        TSB_LAUNCH_CHECK();
+      }
+      return TSB_OK;
+    });
+  }
+  const int vec = norm_vector(dtype, c, g, bits);
+  const Norm a = norm_args(norm_shape(n, c, g, b, vec), order, offsets, weight, bias, param_dtype, 0.f, act, slope);
   float2* slots = reinterpret_cast<float2*>(ws);
-  ws += align_up((size_t)(kNormBlocks + b) * c * sizeof(float2), 256);
-  float2* by_channel = reinterpret_cast<float2*>(ws);
-  float2* by_group = reinterpret_cast<float2*>(ws + align_up((size_t)b * c * sizeof(float2), 256));
+  float2* by_channel = reinterpret_cast<float2*>(ws + channel_bytes(c, kNormBlocks + b));
+  float2* by_group = reinterpret_cast<float2*>(ws + channel_bytes(c, kNormBlocks + b) + channel_bytes(c, b));
   const dim3 grid((unsigned)a.nblk, (unsigned)cdiv(a.cols, a.tile));
   return dispatch_norm(dtype, vec, a.d, order != nullptr, [&](auto tag, auto each, auto ordered) -> int {
     using T = typename decltype(tag)::T;
@@ -750,8 +1053,9 @@ int tsb_group_norm_bwd(const void* x, const void* dy, const int32_t* order, cons
       norm_grad_join_kernel<<<grid_for((int64_t)a.b * a.g, 1), kJoinThreads, 0, st>>>(a, slots, by_channel, by_group);
       TSB_LAUNCH_CHECK();
     }
-    if (n && dx) {
-      norm_grad_apply_kernel<T, VEC, A, ORDERED><<<grid, kNormThreads, 0, st>>>(a, (const T*)x, (const T*)dy, mean, rstd, by_group, (T*)dx);
+    if (n) {
+      norm_grad_apply_kernel<T, VEC, A, ORDERED><<<grid, kNormThreads, 0, st>>>(a, (const T*)x, (const T*)dy, mean, rstd, by_group,
+                                                                               (T*)dx);
       TSB_LAUNCH_CHECK();
     }
     if (dweight || dbias) {

@@ -293,8 +293,8 @@ SortPlan sort_plan(int64_t n, int64_t n_groups) {
   p.tiles = cdiv(n, kSortTile);
   p.pairs = align_up((size_t)n * 4, 256);
   p.counts = n <= kClusterKeys ? 0 : align_up(((size_t)(p.tiles + 1) << p.bits) * sizeof(unsigned), 256);
-  // the sorted keys, and two sets of (key, row) beside the tiles' counts
-  p.bytes = p.pairs + (n <= kClusterKeys ? 0 : p.counts + 4 * p.pairs);
+  // the sorted keys where the offsets are searched in them; two sets of (key, row) beside the tiles' counts
+  p.bytes = n <= kClusterKeys ? (p.passes > 1 ? p.pairs : 0) : p.counts + 5 * p.pairs;
   return p;
 }
 
@@ -792,7 +792,8 @@ int tsb_group_rows(const void* keys, int32_t keys_are_i64, int64_t stride, int64
     TSB_CUDA_TRY(cudaMemsetAsync(offsets, 0, (size_t)(n_groups + 1) * sizeof(int32_t), st));
     return TSB_OK;
   }
-  if (!workspace || workspace_bytes < sort_plan(n, n_groups).bytes) return TSB_ERR_WORKSPACE;
+  const size_t need = sort_plan(n, n_groups).bytes;
+  if (workspace_bytes < need || (need && !workspace)) return TSB_ERR_WORKSPACE;
   const KeySource src{keys, stride, keys_are_i64, (unsigned)n_groups, -1};
   return run_sort(src, n, SortOut{order, inverse, nullptr, offsets}, workspace, st);
 }

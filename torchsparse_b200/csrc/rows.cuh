@@ -17,6 +17,13 @@ struct RawOf<4> { using type = unsigned; };
 template <>
 struct RawOf<2> { using type = unsigned short; };
 
+// The compiler forgets what it derived from a value: packed values that are read twice are unpacked twice, instead of being
+// held unpacked in twice or four times the registers.
+__device__ __forceinline__ void forget(uint4& v) { asm volatile("" : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)); }
+__device__ __forceinline__ void forget(uint2& v) { asm volatile("" : "+r"(v.x), "+r"(v.y)); }
+__device__ __forceinline__ void forget(unsigned& v) { asm volatile("" : "+r"(v)); }
+__device__ __forceinline__ void forget(unsigned short& v) { asm volatile("" : "+h"(v)); }
+
 // VEC neighbouring values of a row, moved as one load or store of VEC * sizeof(T) bytes
 template <typename T, int VEC>
 struct Pack {

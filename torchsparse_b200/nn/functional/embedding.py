@@ -39,7 +39,7 @@ def embedding(indices: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
         if not -table.shape[0] <= padding_idx < table.shape[0]:
             raise ValueError(f"padding_idx {padding_idx} is no row of a table of {table.shape[0]}")
         padding_idx = padding_idx % table.shape[0]
-    flat = indices.reshape(-1)
+    flat = indices if indices.dim() == 1 else indices.reshape(-1)
     if torch.is_grad_enabled() and table.requires_grad:
         out = _Embedding.apply(table, flat, scale, padding_idx)
     else:

@@ -52,12 +52,11 @@ def expert_sort(experts: torch.Tensor, num_experts: int) -> ExpertRows:
     want of room) goes to no expert."""
     if experts.dim() not in (1, 2):
         raise ValueError(f"experts must be [N, k] or [N], not {tuple(experts.shape)}")
-    if experts.dim() == 1:
-        experts = experts[:, None]
-    if experts.shape[1] < 1:
+    shape = (experts.shape[0], experts.shape[1] if experts.dim() == 2 else 1)
+    if shape[1] < 1:
         raise ValueError("every row needs at least one choice")
     order, inverse, offsets = backend.group_rows_cuda(experts.reshape(-1), num_experts, want_inverse=True)
-    return ExpertRows(order, inverse.view(experts.shape), offsets)
+    return ExpertRows(order, inverse.view(shape), offsets)
 
 
 def expert_dispatch(feats: torch.Tensor, rows: ExpertRows) -> torch.Tensor:

@@ -39,19 +39,19 @@ class _GroupNorm(Function):
 
     @staticmethod
     def forward(ctx, feats, weight, bias, offsets, order, num_groups, eps, activation, negative_slope):
-        y, mean, rstd = backend.group_norm_forward_cuda(feats, order, offsets, num_groups, weight, bias, eps, activation,
-                                                        negative_slope)
-        ctx.save_for_backward(feats, weight, bias, offsets, order, mean, rstd)
+        y, stats = backend.group_norm_forward_cuda(feats, order, offsets, num_groups, weight, bias, eps, activation,
+                                                   negative_slope)
+        ctx.save_for_backward(feats, weight, bias, offsets, order, stats)
         ctx.args = num_groups, activation, negative_slope
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_output: torch.Tensor):
-        feats, weight, bias, offsets, order, mean, rstd = ctx.saved_tensors
+        feats, weight, bias, offsets, order, stats = ctx.saved_tensors
         num_groups, activation, negative_slope = ctx.args
         dx, dweight, dbias = backend.group_norm_backward_cuda(feats, grad_output, order, offsets, num_groups, weight, bias,
-                                                              mean, rstd, activation, negative_slope)
+                                                              stats, activation, negative_slope)
         return dx, dweight, dbias, None, None, None, None, None, None
 
 
@@ -68,5 +68,5 @@ def group_norm(feats: torch.Tensor, offsets: torch.Tensor, num_groups: int, weig
     if torch.is_grad_enabled() and (feats.requires_grad or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
         return _GroupNorm.apply(feats, weight, bias, offsets, order, num_groups, eps, activation, negative_slope)
-    return backend.group_norm_forward_cuda(feats, order, offsets, num_groups, weight, bias, eps, activation,
-                                           negative_slope)[0]
+    return backend.group_norm_forward_cuda(feats, order, offsets, num_groups, weight, bias, eps, activation, negative_slope,
+                                           want_stats=False)[0]
