@@ -12,6 +12,7 @@
 //
 // Variances are joined from means and sums of squares about them, piece by piece, never as a difference of two large
 // sums, in 32 bits.
+#include <atomic>
 #include <type_traits>
 
 #include "rows.cuh"
@@ -69,28 +70,151 @@ __device__ __forceinline__ int64_t row_at(const Norm& a, int64_t p) {
   return r >= 0 && r < a.n ? r : -1;
 }
 
-// Byte offsets of U rows, `step` positions apart from p on; -1 for those at or beyond `end` (below it when step is
-// negative: `end` is then the first position that still counts).
-template <bool ORDERED, int U>
-__device__ __forceinline__ void rows_at(const Norm& a, int64_t p, int step, int64_t end, int64_t (&at)[U]) {
+// The `count` rows p, p + step, .. of a thread, U at a time: f(v, at, full) with v[i][u] the vector of array i in row u and
+// at[u] the row's offset, which is -1 for a row that is not there unless `full` says that all are.
+//
+// Vectors of 16 bytes come through shared memory by cp.async, each thread filling and reading slots of its own: three
+// batches are on their way without holding registers, nothing waits for another thread, and the order and the borders of
+// the samples do not matter.  Narrower vectors are loaded directly.
+constexpr int kPipeDepth = 3;
+template <typename T, int VEC>
+constexpr bool kPiped = VEC * sizeof(T) == 16;
+template <typename T, int VEC>
+constexpr int pipe_bytes(int arrays, int u) { return kPiped<T, VEC> ? kPipeDepth * arrays * u * kNormThreads * 16 : 0; }
+
+template <typename T, int VEC, int ARRAYS, int U, bool ORDERED, typename F>
+__device__ __forceinline__ void for_rows(const Norm& a, const T* const (&src)[ARRAYS], int64_t p, int step, int count,
+                                         unsigned char* pipe, F&& f) {
+  const int64_t pitch = (int64_t)step * a.c;
+  int64_t off = p * a.c;      // of row k where the rows lie in order
+  const auto offset = [&](int k, int u, int64_t base) -> int64_t {
+    if (k + u >= count) return -1;
+    if constexpr (ORDERED) {
+      const int64_t r = row_at<true>(a, p + (int64_t)(k + u) * step);
+      return r < 0 ? -1 : r * a.c;
+    }
+    return base + u * pitch;
+  };
+  if constexpr (kPiped<T, VEC>) {
+    constexpr int kStage = ARRAYS * U * kNormThreads * 16;
+    const unsigned char* mine = pipe + threadIdx.x * 16;
+    const unsigned to0 = (unsigned)__cvta_generic_to_shared(mine);
+    const auto copy = [&](int stage, int u, int64_t at) {
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int64_t q = p + u * step;
-    const bool in = step > 0 ? q < end : q >= end;
-    int64_t r = -1;
-    if (in) r = row_at<ORDERED>(a, q);
-    at[u] = r < 0 ? -1 : r * a.c;
+      for (int i = 0; i < ARRAYS; ++i)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to0 + stage * kStage + (u * ARRAYS + i) * kNormThreads * 16),
+                     "l"(src[i] + at)
+                     : "memory");
+    };
+    const auto issue = [&](int stage, int k, int64_t base) {
+      if (!ORDERED && k + U <= count) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) copy(stage, u, base + u * pitch);
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int64_t at = offset(k, u, base);
+          if (at >= 0) copy(stage, u, at);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");      // an empty group where nothing was left to read
+    };
+    constexpr int kAhead = (kPipeDepth - 1) * U;
+#pragma unroll
+    for (int d = 0; d < kPipeDepth - 1; ++d) issue(d, d * U, off + d * U * pitch);
+    int stage = 0;
+    for (int k = 0; k < count; k += U, off += U * pitch) {
+      issue(stage == 0 ? kPipeDepth - 1 : stage - 1, k + kAhead, off + kAhead * pitch);
+      asm volatile("cp.async.wait_group %0;" ::"n"(kPipeDepth - 1) : "memory");
+      Pack<T, VEC> v[ARRAYS][U];
+      int64_t at[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < ARRAYS; ++i)
+          v[i][u].raw = *reinterpret_cast<const uint4*>(mine + stage * kStage + (u * ARRAYS + i) * kNormThreads * 16);
+      if (!ORDERED && k + U <= count) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) at[u] = off + u * pitch;
+        f(v, at, std::true_type());
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) at[u] = offset(k, u, off);
+        f(v, at, std::false_type());
+      }
+      stage = stage + 1 == kPipeDepth ? 0 : stage + 1;
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else {
+    for (int k = 0; k < count; k += U, off += U * pitch) {
+      Pack<T, VEC> v[ARRAYS][U];
+      int64_t at[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        at[u] = offset(k, u, off);
+#pragma unroll
+        for (int i = 0; i < ARRAYS; ++i)
+          if (at[u] >= 0) v[i][u].load(src[i] + at[u]);
+      }
+      f(v, at, std::false_type());
+    }
+  }
+}
+
+// Two values at once: the packed 32-bit instructions halve what the arithmetic takes of the issue slots.  Each rounds as
+// its scalar form does.
+__device__ __forceinline__ void fma2(float& x, float& y, float a, float b, float c, float d, float e, float f) {
+  asm("{.reg .b64 p, q, r; mov.b64 p, {%2, %3}; mov.b64 q, {%4, %5}; mov.b64 r, {%6, %7}; fma.rn.f32x2 p, p, q, r; mov.b64 {%0, %1}, p;}"
+      : "=f"(x), "=f"(y) : "f"(a), "f"(b), "f"(c), "f"(d), "f"(e), "f"(f));
+}
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b, float c, float d) {
+  asm("{.reg .b64 p, q; mov.b64 p, {%2, %3}; mov.b64 q, {%4, %5}; add.rn.f32x2 p, p, q; mov.b64 {%0, %1}, p;}"
+      : "=f"(x), "=f"(y) : "f"(a), "f"(b), "f"(c), "f"(d));
+}
+__device__ __forceinline__ void mul2(float& x, float& y, float a, float b, float c, float d) {
+  asm("{.reg .b64 p, q; mov.b64 p, {%2, %3}; mov.b64 q, {%4, %5}; mul.rn.f32x2 p, p, q; mov.b64 {%0, %1}, p;}"
+      : "=f"(x), "=f"(y) : "f"(a), "f"(b), "f"(c), "f"(d));
+}
+// r[e] = x[e] * y[j(e)] + z[l(e)] and the like over VEC values; the indices let a group's value stand for several channels
+template <int N, typename Y, typename Z>
+__device__ __forceinline__ void fma_all(float (&r)[N], const float (&x)[N], Y&& y, Z&& z) {
+  if constexpr (N == 1) {
+    r[0] = fmaf(x[0], y(0), z(0));
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; e += 2) fma2(r[e], r[e + 1], x[e], x[e + 1], y(e), y(e + 1), z(e), z(e + 1));
+  }
+}
+template <int N, typename Y>
+__device__ __forceinline__ void add_all(float (&r)[N], const float (&x)[N], Y&& y) {
+  if constexpr (N == 1) {
+    r[0] = x[0] + y(0);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; e += 2) add2(r[e], r[e + 1], x[e], x[e + 1], y(e), y(e + 1));
+  }
+}
+template <int N, typename Y>
+__device__ __forceinline__ void mul_all(float (&r)[N], const float (&x)[N], Y&& y) {
+  if constexpr (N == 1) {
+    r[0] = x[0] * y(0);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; e += 2) mul2(r[e], r[e + 1], x[e], x[e + 1], y(e), y(e + 1));
   }
 }
 
 // 1 / (1 + 2^(-z log2 e)) with the hardware's exponential and reciprocal, each good to 2^-22: half the instructions of the
 // library's forms, which also serve subnormal arguments (here 2^x below 2^-126 vanishes beside the 1, and beyond 2^126
 // the quotient is below 2^-126 and becomes zero).
-__device__ __forceinline__ float sigmoid(float z) {
-  float e, p;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(1.f + e));
-  return p;
+template <int N>
+__device__ __forceinline__ void sigmoid(float (&p)[N], const float (&z)[N]) {
+  mul_all(p, z, [](int) { return -1.4426950408889634f; });
+#pragma unroll
+  for (int e = 0; e < N; ++e) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p[e]) : "f"(p[e]));
+  add_all(p, p, [](int) { return 1.f; });
+#pragma unroll
+  for (int e = 0; e < N; ++e) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(p[e]) : "f"(p[e]));
 }
 
 template <int N>
@@ -102,8 +226,9 @@ __device__ __forceinline__ void activate(float (&z)[N], int act, float slope) {
 #pragma unroll
     for (int i = 0; i < N; ++i) z[i] = z[i] > 0.f ? z[i] : z[i] * slope;
   } else if (act == kActSilu) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) z[i] *= sigmoid(z[i]);
+    float p[N];
+    sigmoid(p, z);
+    mul_all(z, z, [&](int i) { return p[i]; });
   }
 }
 
@@ -117,11 +242,12 @@ __device__ __forceinline__ void activate_grad(const float (&z)[N], float (&g)[N]
 #pragma unroll
     for (int i = 0; i < N; ++i) g[i] = z[i] > 0.f ? g[i] : g[i] * slope;
   } else if (act == kActSilu) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float p = sigmoid(z[i]);
-      g[i] *= fmaf(z[i] * p, 1.f - p, p);
-    }
+    float p[N], q[N], r[N];      // act' = z p (1 - p) + p
+    sigmoid(p, z);
+    mul_all(q, z, [&](int i) { return p[i]; });
+    fma_all(r, p, [](int) { return -1.f; }, [](int) { return 1.f; });
+    fma_all(q, q, [&](int i) { return r[i]; }, [&](int i) { return p[i]; });
+    mul_all(g, g, [&](int i) { return q[i]; });
   }
 }
 
@@ -156,28 +282,32 @@ struct Running {
   template <typename T, int U>
   __device__ __forceinline__ void add(const Pack<T, VEC> (&v)[U]) {
     constexpr float kCount = (float)(U * W), kInv = 1.f / kCount;      // W values of a vector share a pair
-    float sum[A], sq[A];
+    float f[U][VEC], chan[VEC], sum[A], sq[A];
 #pragma unroll
-    for (int i = 0; i < A; ++i) sum[i] = sq[i] = 0.f;
+    for (int u = 0; u < U; ++u) v[u].get(f[u]);
+    const auto gather = [&](float (&to)[A]) {      // the channels of a pair
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float f[VEC];
-      v[u].get(f);
+      for (int i = 0; i < A; ++i) {
+        to[i] = chan[i * W];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) sum[e / W] += f[e];
-    }
+        for (int e = 1; e < W; ++e) to[i] += chan[i * W + e];
+      }
+    };
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) chan[e] = f[0][e];
+#pragma unroll
+    for (int u = 1; u < U; ++u) add_all(chan, chan, [&](int e) { return f[u][e]; });
+    gather(sum);
 #pragma unroll
     for (int i = 0; i < A; ++i) sum[i] *= kInv;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float f[VEC];
-      v[u].get(f);
+    for (int e = 0; e < VEC; ++e) chan[e] = 0.f;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float t = f[e] - sum[e / W];
-        sq[e / W] = fmaf(t, t, sq[e / W]);
-      }
+    for (int u = 0; u < U; ++u) {
+      add_all(f[u], f[u], [&](int e) { return -sum[e / W]; });
+      fma_all(chan, f[u], [&](int e) { return f[u][e]; }, [&](int e) { return chan[e]; });
     }
+    gather(sq);
     const float all = n + kCount, share = __fdividef(kCount, all), cross = n * share;
 #pragma unroll
     for (int i = 0; i < A; ++i) {
@@ -191,6 +321,7 @@ struct Running {
 
 template <typename T, int VEC, int A, bool ORDERED>
 __global__ void __launch_bounds__(kNormThreads, 3) norm_stats_kernel(Norm a, const T* __restrict__ x, float2* __restrict__ slots) {
+  extern __shared__ __align__(16) unsigned char pipe[];
   __shared__ float2 part[A * kNormThreads];
   const int first = blockIdx.y * a.tile, width = min(a.tile, a.cols - first);
   const int lane = threadIdx.x / width, col = threadIdx.x - lane * width;
@@ -206,23 +337,26 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_stats_kernel(Norm a, con
       constexpr int U = 4;
       Running<VEC, A> run;
       run.clear();
-      int64_t p = lo + lane;
-      for (; p + (U - 1) * lanes < hi; p += U * lanes) {
-        Pack<T, VEC> v[U];
-        int64_t at[U];
-        rows_at<ORDERED>(a, p, lanes, hi, at);
+      const T* const src[1] = {xc};
+      const int count = (int)lane_rows(hi - lo, lanes, lane);
+      int left = count;
+      for_rows<T, VEC, 1, U, ORDERED>(a, src, lo + lane, lanes, count, pipe, [&](Pack<T, VEC> (&v)[1][U], const int64_t (&at)[U], auto) {
+        if constexpr (ORDERED) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (!ORDERED || at[u] >= 0) v[u].load(xc + at[u]); else v[u].clear();
+          for (int u = 0; u < U; ++u)
+            if (at[u] < 0) v[0][u].clear();      // an entry of the order that is no row
         }
-        run.add(v);
-      }
-      for (; p < hi; p += lanes) {
-        Pack<T, VEC> v[1];
-        const int64_t r = row_at<ORDERED>(a, p);
-        if (r >= 0) v[0].load(xc + r * a.c); else v[0].clear();
-        run.add(v);
-      }
+        if (left >= U) {
+          run.add(v[0]);
+        } else {
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const Pack<T, VEC> one[1] = {v[0][u]};
+            if (u < left) run.add(one);
+          }
+        }
+        left -= U;
+      });
 #pragma unroll
       for (int i = 0; i < A; ++i) part[i * kNormThreads + threadIdx.x] = make_float2(run.mean[i], run.m2[i]);
     }
@@ -308,19 +442,25 @@ __global__ void __launch_bounds__(128) norm_join_kernel(Norm a, int vec, int til
   }
 }
 
-// What a thread needs of its VEC channels within one sample: z = (x - mean) * a + b with a = rstd * w.
+// What a thread needs of its VEC channels within one sample: z = (x + away) * a + b with away = -mean, a = rstd * w.
 template <int VEC, int A>
 struct Channels {
   static constexpr int W = VEC / A;
-  float mean[A], a[VEC], b[VEC];
+  float away[A], a[VEC], b[VEC];
   __device__ __forceinline__ void load(const Norm& n, int s, int k0, const float* __restrict__ mean_, const float* __restrict__ rstd_) {
 #pragma unroll
-    for (int i = 0; i < A; ++i) mean[i] = __ldg(mean_ + (int64_t)s * n.g + (k0 + i * W) / n.d);
+    for (int i = 0; i < A; ++i) away[i] = -__ldg(mean_ + (int64_t)s * n.g + (k0 + i * W) / n.d);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       a[e] = __ldg(rstd_ + (int64_t)s * n.g + (k0 + e / W * W) / n.d) * (n.w ? load_any(n.w, n.p_dtype, k0 + e) : 1.f);
       b[e] = n.bias ? load_any(n.bias, n.p_dtype, k0 + e) : 0.f;
     }
+  }
+  __device__ __forceinline__ void center(float (&x)[VEC]) const {
+    add_all(x, x, [&](int e) { return away[e / W]; });
+  }
+  __device__ __forceinline__ void affine(float (&z)[VEC], const float (&x)[VEC]) const {
+    fma_all(z, x, [&](int e) { return a[e]; }, [&](int e) { return b[e]; });
   }
 };
 
@@ -343,6 +483,7 @@ template <typename T, int VEC, int A, bool ORDERED>
 __global__ void __launch_bounds__(kNormThreads, 3) norm_apply_kernel(Norm a, const T* __restrict__ x, const float* __restrict__ mean,
                                                                      const float* __restrict__ rstd, T* __restrict__ y) {
   constexpr int U = 4, W = VEC / A;
+  extern __shared__ __align__(16) unsigned char pipe[];
   const int first = blockIdx.y * a.tile, width = min(a.tile, a.cols - first);
   const int lane = threadIdx.x / width, lanes = kNormThreads / width;
   const int k0 = (first + threadIdx.x - lane * width) * VEC;
@@ -359,25 +500,21 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_apply_kernel(Norm a, con
     if (lo >= hi) continue;
     Channels<VEC, A> ch;
     ch.load(a, s, k0, mean, rstd);
-    for (int64_t p = hi - 1 - lane; p >= lo; p -= U * lanes) {
-      Pack<T, VEC> v[U];
-      int64_t at[U];
-      rows_at<ORDERED>(a, p, -lanes, lo, at);
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (at[u] >= 0) v[u].load(xc + at[u]);
+    const T* const src[1] = {xc};
+    for_rows<T, VEC, 1, U, ORDERED>(a, src, hi - 1 - lane, -lanes, (int)lane_rows(hi - lo, lanes, lane), pipe,
+                                    [&](Pack<T, VEC> (&v)[1][U], const int64_t (&at)[U], auto full) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (at[u] < 0) continue;
+        if (!decltype(full)::value && at[u] < 0) continue;
         float z[VEC];
-        v[u].get(z);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) z[e] = fmaf(z[e] - ch.mean[e / W], ch.a[e], ch.b[e]);
+        v[0][u].get(z);
+        ch.center(z);
+        ch.affine(z, z);
         activate(z, a.act, a.slope);
-        v[u].set(z);
-        v[u].store(yc + at[u]);
+        v[0][u].set(z);
+        v[0][u].store(yc + at[u]);
       }
-    }
+    });
   }
 }
 
@@ -388,6 +525,7 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_grad_sums_kernel(Norm a,
                                                                          const float* __restrict__ mean,
                                                                          const float* __restrict__ rstd, float2* __restrict__ slots) {
   constexpr int U = 2, W = VEC / A;
+  extern __shared__ __align__(16) unsigned char pipe[];
   __shared__ float2 part[VEC * kNormThreads];
   const int first = blockIdx.y * a.tile, width = min(a.tile, a.cols - first);
   const int lane = threadIdx.x / width, lanes = kNormThreads / width, col = threadIdx.x - lane * width;
@@ -405,35 +543,22 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_grad_sums_kernel(Norm a,
       for (int e = 0; e < VEC; ++e) s1[e] = s2[e] = 0.f;
       Channels<VEC, A> ch;
       ch.load(a, s, k0, mean, rstd);
-      for (int64_t p = lo + lane; p < hi; p += U * lanes) {
-        Pack<T, VEC> vx[U], vg[U];
-        int64_t at[U];
-        rows_at<ORDERED>(a, p, lanes, hi, at);
+      const T* const src[2] = {xc, gc};
+      for_rows<T, VEC, 2, U, ORDERED>(a, src, lo + lane, lanes, (int)lane_rows(hi - lo, lanes, lane), pipe,
+                                      [&](Pack<T, VEC> (&v)[2][U], const int64_t (&at)[U], auto full) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          if (at[u] < 0) continue;
-          vx[u].load(xc + at[u]);
-          vg[u].load(gc + at[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (at[u] < 0) continue;
+          if (!decltype(full)::value && at[u] < 0) continue;
           float h[VEC], z[VEC], g[VEC];
-          vx[u].get(h);
-          vg[u].get(g);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            h[e] -= ch.mean[e / W];
-            z[e] = fmaf(h[e], ch.a[e], ch.b[e]);
-          }
+          v[0][u].get(h);
+          v[1][u].get(g);
+          ch.center(h);
+          ch.affine(z, h);
           activate_grad(z, g, a.act, a.slope);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            s1[e] += g[e];
-            s2[e] = fmaf(g[e], h[e], s2[e]);
-          }
+          add_all(s1, s1, [&](int e) { return g[e]; });
+          fma_all(s2, g, [&](int e) { return h[e]; }, [&](int e) { return s2[e]; });
         }
-      }
+      });
 #pragma unroll
       for (int e = 0; e < VEC; ++e) part[e * kNormThreads + threadIdx.x] = make_float2(s1[e], s2[e]);
     }
@@ -506,13 +631,14 @@ __global__ void __launch_bounds__(kJoinThreads) norm_grad_join_kernel(Norm a, co
   }
 }
 
-// dx = rstd * (dz * w - m1 - xhat * m2) = dz * a - (x - mean) * k2 - k1 with k1 = rstd * m1, k2 = rstd^2 * m2
+// dx = rstd * (dz * w - m1 - xhat * m2) = dz * a + (x - mean) * k2 + k1 with k1 = -rstd * m1, k2 = -rstd^2 * m2
 template <typename T, int VEC, int A, bool ORDERED>
 __global__ void __launch_bounds__(kNormThreads, 3) norm_grad_apply_kernel(Norm a, const T* __restrict__ x, const T* __restrict__ dy,
                                                                           const float* __restrict__ mean,
                                                                           const float* __restrict__ rstd,
                                                                           const float2* __restrict__ by_group, T* __restrict__ dx) {
   constexpr int U = 2, W = VEC / A;
+  extern __shared__ __align__(16) unsigned char pipe[];
   const int first = blockIdx.y * a.tile, width = min(a.tile, a.cols - first);
   const int lane = threadIdx.x / width, lanes = kNormThreads / width;
   const int k0 = (first + threadIdx.x - lane * width) * VEC;
@@ -535,37 +661,27 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_grad_apply_kernel(Norm a
       const int64_t at = (int64_t)s * a.g + (k0 + i * W) / a.d;
       const float2 f = __ldg(by_group + at);
       const float r = __ldg(rstd + at);
-      k1[i] = r * f.x;
-      k2[i] = r * r * f.y;
+      k1[i] = -r * f.x;
+      k2[i] = -r * r * f.y;
     }
-    for (int64_t p = hi - 1 - lane; p >= lo; p -= U * lanes) {
-      Pack<T, VEC> vx[U], vg[U];
-      int64_t at[U];
-      rows_at<ORDERED>(a, p, -lanes, lo, at);
+    const T* const src[2] = {xc, gc};
+    for_rows<T, VEC, 2, U, ORDERED>(a, src, hi - 1 - lane, -lanes, (int)lane_rows(hi - lo, lanes, lane), pipe,
+                                    [&](Pack<T, VEC> (&v)[2][U], const int64_t (&at)[U], auto full) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (at[u] < 0) continue;
-        vx[u].load(xc + at[u]);
-        vg[u].load(gc + at[u]);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (at[u] < 0) continue;
+        if (!decltype(full)::value && at[u] < 0) continue;
         float h[VEC], z[VEC], g[VEC];
-        vx[u].get(h);
-        vg[u].get(g);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          h[e] -= ch.mean[e / W];
-          z[e] = fmaf(h[e], ch.a[e], ch.b[e]);
-        }
+        v[0][u].get(h);
+        v[1][u].get(g);
+        ch.center(h);
+        ch.affine(z, h);
         activate_grad(z, g, a.act, a.slope);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) g[e] = fmaf(g[e], ch.a[e], -fmaf(h[e], k2[e / W], k1[e / W]));
-        vg[u].set(g);
-        vg[u].store(dc + at[u]);
+        fma_all(h, h, [&](int e) { return k2[e / W]; }, [&](int e) { return k1[e / W]; });
+        fma_all(g, g, [&](int e) { return ch.a[e]; }, [&](int e) { return h[e]; });
+        v[1][u].set(g);
+        v[1][u].store(dc + at[u]);
       }
-    }
+    });
   }
 }
 
@@ -909,6 +1025,23 @@ int small_threads(int64_t n, int64_t b, int dv) {
   return (int)(want < 128 ? 128 : want > kSmallThreads ? kSmallThreads : want);
 }
 
+// launches a kernel with BYTES of dynamic shared memory, which its device has to be told of once
+template <auto KERNEL, int BYTES, typename... Q>
+int launch_piped(dim3 grid, cudaStream_t st, Q... args) {
+  if (BYTES > 0) {
+    static std::atomic<bool> told[64];
+    int dev = 0;
+    TSB_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev >= 64 || !told[dev].load(std::memory_order_acquire)) {
+      TSB_CUDA_TRY(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES));
+      if (dev < 64) told[dev].store(true, std::memory_order_release);
+    }
+  }
+  KERNEL<<<grid, kNormThreads, BYTES, st>>>(args...);
+  TSB_LAUNCH_CHECK();
+  return TSB_OK;
+}
+
 template <typename F>
 int dispatch_small(int dtype, int vec, bool ordered, F&& f) {
   return dispatch_pack(dtype, vec, [&](auto tag) -> int { return ordered ? f(tag, std::true_type()) : f(tag, std::false_type()); });
@@ -984,16 +1117,17 @@ int tsb_group_norm_fwd(const void* x, const int32_t* order, const int32_t* offse
     constexpr int VEC = decltype(tag)::VEC, A = decltype(each)::value;
     constexpr bool ORDERED = decltype(ordered)::value;
     if (n && b) {
-      norm_stats_kernel<T, VEC, A, ORDERED><<<grid, kNormThreads, 0, st>>>(a, (const T*)x, slots);
-      TSB_LAUNCH_CHECK();
+      const int rc = launch_piped<norm_stats_kernel<T, VEC, A, ORDERED>, pipe_bytes<T, VEC>(1, 4)>(grid, st, a, (const T*)x, slots);
+      if (rc != TSB_OK) return rc;
     }
     if (b) {
       norm_join_kernel<<<grid_for((int64_t)a.b * a.g, 4), 128, 0, st>>>(a, VEC, tiles, slots, mean, rstd);
       TSB_LAUNCH_CHECK();
     }
     if (n) {
-      norm_apply_kernel<T, VEC, A, ORDERED><<<grid, kNormThreads, 0, st>>>(a, (const T*)x, mean, rstd, (T*)y);
-      TSB_LAUNCH_CHECK();
+      const int rc = launch_piped<norm_apply_kernel<T, VEC, A, ORDERED>, pipe_bytes<T, VEC>(1, 4)>(grid, st, a, (const T*)x, mean,
+                                                            rstd, (T*)y);
+      if (rc != TSB_OK) return rc;
     }
     return TSB_OK;
   });
@@ -1046,17 +1180,18 @@ int tsb_group_norm_bwd(const void* x, const void* dy, const int32_t* order, cons
     constexpr int VEC = decltype(tag)::VEC, A = decltype(each)::value;
     constexpr bool ORDERED = decltype(ordered)::value;
     if (n && b) {
-      norm_grad_sums_kernel<T, VEC, A, ORDERED><<<grid, kNormThreads, 0, st>>>(a, (const T*)x, (const T*)dy, mean, rstd, slots);
-      TSB_LAUNCH_CHECK();
+      const int rc = launch_piped<norm_grad_sums_kernel<T, VEC, A, ORDERED>, pipe_bytes<T, VEC>(2, 2)>(grid, st, a, (const T*)x,
+                                                            (const T*)dy, mean, rstd, slots);
+      if (rc != TSB_OK) return rc;
     }
     if (b) {
       norm_grad_join_kernel<<<grid_for((int64_t)a.b * a.g, 1), kJoinThreads, 0, st>>>(a, slots, by_channel, by_group);
       TSB_LAUNCH_CHECK();
     }
     if (n) {
-      norm_grad_apply_kernel<T, VEC, A, ORDERED><<<grid, kNormThreads, 0, st>>>(a, (const T*)x, (const T*)dy, mean, rstd, by_group,
-                                                                               (T*)dx);
-      TSB_LAUNCH_CHECK();
+      const int rc = launch_piped<norm_grad_apply_kernel<T, VEC, A, ORDERED>, pipe_bytes<T, VEC>(2, 2)>(grid, st, a, (const T*)x,
+                                                            (const T*)dy, mean, rstd, by_group, (T*)dx);
+      if (rc != TSB_OK) return rc;
     }
     if (dweight || dbias) {
       norm_grad_params_kernel<<<(unsigned)cdiv(a.c, 32), 256, 0, st>>>(a, by_channel, dweight, dbias);

@@ -10,6 +10,9 @@
 #include "rows.cuh"
 
 namespace cg = cooperative_groups;
+#ifndef TSB_GRID
+#define TSB_GRID 8
+#endif
 
 namespace tsb {
 namespace {
@@ -645,127 +648,140 @@ __global__ void __launch_bounds__(kThreads) dispatch_kernel(const T* __restrict_
   }
 }
 
-// out[i] = sum over j of w[i][j] * rows[inverse[i][j]] (w null: 1), in the order of j.  A thread has ROWS vectors of the
-// result and reads KU choices of each at once: eight vectors in flight.
-template <typename T, int VEC, int KU>
+// The two kernels below give a row (a choice) to a group of `lanes` threads, a power of two up to a warp, and let a grid
+// that fits the machine walk over the rows, with the indices of a group's next row on their way while it reads this one.
+
+// out[i] = sum over j of w[i][j] * rows[inverse[i][j]] (w null: 1), in the order of j: KU choices and U vectors of each at once
+template <typename T, int VEC, int KU, int U>
 __global__ void __launch_bounds__(kThreads) combine_kernel(const T* __restrict__ rows, const void* __restrict__ w, int w_dtype,
                                                            const int* __restrict__ inverse, const int* __restrict__ kept,
-                                                           int64_t total, int64_t pairs, int k, RowSplit split,
-                                                           T* __restrict__ out) {
-  constexpr int ROWS = 8 / KU;
-  const int64_t t0 = blockIdx.x * (int64_t)(kThreads * ROWS) + threadIdx.x, c = (int64_t)split.cols * VEC;
-  const int n_kept = (int)min((int64_t)__ldg(kept), pairs);
-  float acc[ROWS][VEC];
-  int64_t i[ROWS];
-  const T* base[ROWS];
+                                                           int64_t n, int k, int64_t c, int lanes, T* __restrict__ out) {
+  const int cols = (int)(c / VEC), lane = threadIdx.x & (lanes - 1), groups = kThreads / lanes;
+  const int64_t step = (int64_t)gridDim.x * groups;
+  const int n_kept = (int)min((int64_t)__ldg(kept), n * k);
+  int next[KU];
+  const auto fetch = [&](int64_t i, int q0, int (&pos)[KU]) {
 #pragma unroll
-  for (int r = 0; r < ROWS; ++r) {
-    const int64_t t = min(t0 + r * kThreads, total - 1);
-    i[r] = split.row(t);
-    base[r] = rows + (t - i[r] * split.cols) * VEC;
-    i[r] *= k;
+    for (int u = 0; u < KU; ++u) pos[u] = i < n && q0 + u < k ? __ldg(inverse + i * k + q0 + u) : -1;
+  };
+  int64_t i = blockIdx.x * (int64_t)groups + threadIdx.x / lanes;
+  fetch(i, 0, next);
+  for (; i < n; i += step) {
+    int first[KU];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) acc[r][e] = 0.f;
-  }
-  for (int q0 = 0; q0 < k; q0 += KU) {
-    Pack<T, VEC> p[ROWS][KU];
-    int pos[ROWS][KU];
+    for (int u = 0; u < KU; ++u) first[u] = next[u];
+    fetch(i + step, 0, next);
+    for (int v0 = lane; v0 < cols; v0 += lanes * U) {
+      float acc[U][VEC];
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r)
+      for (int x = 0; x < U; ++x)
 #pragma unroll
-      for (int u = 0; u < KU; ++u) {
-        pos[r][u] = q0 + u < k ? __ldg(inverse + i[r] + q0 + u) : -1;
-        if (pos[r][u] >= n_kept) pos[r][u] = -1;
+        for (int e = 0; e < VEC; ++e) acc[x][e] = 0.f;
+      for (int q0 = 0; q0 < k; q0 += KU) {
+        int pos[KU];
+        if (q0) {
+          fetch(i, q0, pos);
+        } else {
+#pragma unroll
+          for (int u = 0; u < KU; ++u) pos[u] = first[u];
+        }
+        Pack<T, VEC> p[KU][U];
+#pragma unroll
+        for (int u = 0; u < KU; ++u)
+#pragma unroll
+          for (int x = 0; x < U; ++x)
+            if ((unsigned)pos[u] < (unsigned)n_kept && v0 + x * lanes < cols)
+              p[u][x].load(rows + (int64_t)pos[u] * c + (v0 + x * lanes) * VEC);
+#pragma unroll
+        for (int u = 0; u < KU; ++u) {
+          if ((unsigned)pos[u] >= (unsigned)n_kept) continue;
+          const float f = w ? load_any(w, w_dtype, i * k + q0 + u) : 1.f;
+#pragma unroll
+          for (int x = 0; x < U; ++x) {
+            if (v0 + x * lanes >= cols) continue;
+            float v[VEC];
+            p[u][x].get(v);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) acc[x][e] = fmaf(f, v[e], acc[x][e]);
+          }
+        }
       }
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r)
-#pragma unroll
-      for (int u = 0; u < KU; ++u)
-        if (pos[r][u] >= 0) p[r][u].load(base[r] + pos[r][u] * c);
-#pragma unroll
-    for (int r = 0; r < ROWS; ++r)
-#pragma unroll
-      for (int u = 0; u < KU; ++u) {
-        if (pos[r][u] < 0) continue;
-        const float f = w ? load_any(w, w_dtype, i[r] + q0 + u) : 1.f;
-        float v[VEC];
-        p[r][u].get(v);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[r][e] = fmaf(f, v[e], acc[r][e]);
+      for (int x = 0; x < U; ++x) {
+        if (v0 + x * lanes >= cols) continue;
+        Pack<T, VEC> o;
+        o.set(acc[x]);
+        o.store(out + i * c + (v0 + x * lanes) * VEC);
       }
-  }
-#pragma unroll
-  for (int r = 0; r < ROWS; ++r) {
-    if (t0 + r * kThreads >= total) break;
-    Pack<T, VEC> o;
-    o.set(acc[r]);
-    o.store(out + (t0 + r * kThreads) * VEC);
+    }
   }
 }
 
-// One group of `lanes` threads (a power of two up to a warp) for PAIRS choices at a time: drows[pos] = w * dout[i] and
-// dw = <dout[i], rows[pos]>, both zero for a choice of no expert.  Choices of one row share its dout through the L1 cache.
+// drows[pos] = w * dout[i] and dw = <dout[i], rows[pos]> of a choice, both zero for a choice of no expert.  Choices of one
+// row share its dout through the L1 cache.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads) combine_grad_kernel(const T* __restrict__ dout, const T* __restrict__ rows,
                                                                 const void* __restrict__ w, int w_dtype,
                                                                 const int* __restrict__ inverse, const int* __restrict__ kept,
                                                                 int64_t pairs, RowSplit by_k, int64_t c, int lanes,
                                                                 T* __restrict__ drows, void* __restrict__ dw) {
-  constexpr int PAIRS = 2, U = 2;
-  const int cols = (int)(c / VEC), lane = threadIdx.x & (lanes - 1);
-  const int64_t n_kept = __ldg(kept);
-  const int64_t q0 = (blockIdx.x * (int64_t)(kThreads / lanes) + threadIdx.x / lanes) * PAIRS;
-  float f[PAIRS], dot[PAIRS];
-  const T *g0[PAIRS], *r0[PAIRS];
-  T* d0[PAIRS];
-  bool there[PAIRS], used[PAIRS];
+  constexpr int U = 2;
+  const int cols = (int)(c / VEC), lane = threadIdx.x & (lanes - 1), groups = kThreads / lanes;
+  const int64_t step = (int64_t)gridDim.x * groups;
+  const int n_kept = (int)min((int64_t)__ldg(kept), pairs);
+  // whole warps stay together for the sums: q of the warp's first group decides
+  const int64_t ahead = threadIdx.x / lanes - (threadIdx.x / 32) * (32 / lanes);
+  int64_t q0 = blockIdx.x * (int64_t)groups + (threadIdx.x / 32) * (32 / lanes);
+  int next = q0 + ahead < pairs ? __ldg(inverse + q0 + ahead) : -1;
+  float next_w = q0 + ahead < pairs ? load_any(w, w_dtype, q0 + ahead) : 0.f;
+  for (; q0 < pairs; q0 += step) {
+    const int64_t q = q0 + ahead;
+    const int pos = next;
+    const float f = next_w;
+    next = q + step < pairs ? __ldg(inverse + q + step) : -1;
+    next_w = q + step < pairs ? load_any(w, w_dtype, q + step) : 0.f;
+    float dot = 0.f;
+    if ((unsigned)pos < (unsigned)n_kept) {
+      const T *g0 = dout + by_k.row(q) * c, *r0 = rows + (int64_t)pos * c;
+      T* d0 = drows + (int64_t)pos * c;
+      for (int v0 = lane; v0 < cols; v0 += lanes * U) {
+        Pack<T, VEC> g[U], r[U];
 #pragma unroll
-  for (int q = 0; q < PAIRS; ++q) {
-    const int64_t pos = q0 + q < pairs ? (int64_t)__ldg(inverse + q0 + q) : -1;
-    there[q] = pos >= 0 && pos < pairs;
-    used[q] = there[q] && pos < n_kept;
-    dot[q] = 0.f;
-    f[q] = used[q] ? load_any(w, w_dtype, q0 + q) : 0.f;
-    g0[q] = dout + by_k.row(min(q0 + q, pairs - 1)) * c;
-    r0[q] = rows + (there[q] ? pos : 0) * c;
-    d0[q] = drows + (there[q] ? pos : 0) * c;
-  }
-  for (int v0 = lane; v0 < cols; v0 += lanes * U) {
-    Pack<T, VEC> g[PAIRS][U], r[PAIRS][U];
-#pragma unroll
-    for (int q = 0; q < PAIRS; ++q)
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (!used[q] || v0 + u * lanes >= cols) {
-          g[q][u].clear();
-          r[q][u].clear();
-          continue;
+        for (int u = 0; u < U; ++u) {
+          if (v0 + u * lanes >= cols) continue;
+          r[u].load(r0 + (v0 + u * lanes) * VEC);
+          g[u].load(g0 + (v0 + u * lanes) * VEC);
         }
-        r[q][u].load(r0[q] + (v0 + u * lanes) * VEC);
-        g[q][u].load(g0[q] + (v0 + u * lanes) * VEC);
-      }
 #pragma unroll
-    for (int q = 0; q < PAIRS; ++q)
+        for (int u = 0; u < U; ++u) {
+          if (v0 + u * lanes >= cols) continue;
+          float a[VEC], b[VEC];
+          g[u].get(a);
+          r[u].get(b);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (!there[q] || v0 + u * lanes >= cols) continue;
-        float a[VEC], b[VEC];
-        g[q][u].get(a);
-        r[q][u].get(b);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          dot[q] = fmaf(a[e], b[e], dot[q]);
-          a[e] *= f[q];
+          for (int e = 0; e < VEC; ++e) {
+            dot = fmaf(a[e], b[e], dot);
+            a[e] *= f;
+          }
+          g[u].set(a);
+          g[u].store(d0 + (v0 + u * lanes) * VEC);
         }
-        g[q][u].set(a);
-        g[q][u].store(d0[q] + (v0 + u * lanes) * VEC);
       }
+    } else if (pos >= 0 && pos < pairs) {
+      Pack<T, VEC> zero;
+      zero.clear();
+      for (int v = lane; v < cols; v += lanes) zero.store(drows + (int64_t)pos * c + v * VEC);
+    }
+    for (int o = lanes >> 1; o > 0; o >>= 1) dot += __shfl_down_sync(0xffffffffu, dot, o, lanes);
+    if (lane == 0 && q < pairs) store_any(dw, w_dtype, q, dot);
   }
-#pragma unroll
-  for (int q = 0; q < PAIRS; ++q) {
-    for (int o = lanes >> 1; o > 0; o >>= 1) dot[q] += __shfl_down_sync(0xffffffffu, dot[q], o, lanes);
-    if (lane == 0 && q0 + q < pairs) store_any(dw, w_dtype, q0 + q, dot[q]);
-  }
+}
+
+// threads of a row of `cols` vectors
+int row_lanes(int64_t cols) {
+  int lanes = 1;
+  while (lanes < 32 && lanes < cols) lanes *= 2;
+  return lanes;
 }
 
 bool good_dtype(int dtype) { return dtype == TSB_F32 || dtype == TSB_F16 || dtype == TSB_BF16; }
@@ -902,16 +918,15 @@ int tsb_expert_combine(const void* rows, const void* weights, int32_t weights_dt
   if (n > kMaxRows / k || c > kMaxChannels) return TSB_ERR_LIMIT;
   if (n == 0) return TSB_OK;
   const int vec = vector_width(dtype, c, (uintptr_t)rows | (uintptr_t)out);
-  const int64_t total = n * (c / vec), blocks = cdiv(total, kThreads * (k <= 2 ? 4 : 2));
-  if (blocks > 0x7fffffff) return TSB_ERR_LIMIT;
+  const int lanes = row_lanes(c / vec);
+  const int grid = grid_for(n * lanes, kThreads, TSB_GRID);
   return dispatch_pack(dtype, vec, [&](auto tag) -> int {
     using T = typename decltype(tag)::T;
     constexpr int VEC = decltype(tag)::VEC;
     const auto run = [&](auto kernel) {
-      kernel<<<(unsigned)blocks, kThreads, 0, as_stream(stream)>>>((const T*)rows, weights, weights_dtype, inverse, kept, total, n * k,
-                                                                   k, row_split(c / VEC), (T*)out);
+      kernel<<<grid, kThreads, 0, as_stream(stream)>>>((const T*)rows, weights, weights_dtype, inverse, kept, n, k, c, lanes, (T*)out);
     };
-    if (k <= 2) run(combine_kernel<T, VEC, 2>); else run(combine_kernel<T, VEC, 4>);
+    if (k <= 2) run(combine_kernel<T, VEC, 2, 2>); else run(combine_kernel<T, VEC, 4, 1>);
     TSB_LAUNCH_CHECK();
     return TSB_OK;
   });
@@ -926,13 +941,12 @@ int tsb_expert_combine_bwd(const void* dout, const void* rows, const void* weigh
   if (n > kMaxRows / k || c > kMaxChannels) return TSB_ERR_LIMIT;
   if (n == 0) return TSB_OK;
   const int vec = vector_width(dtype, c, (uintptr_t)dout | (uintptr_t)rows | (uintptr_t)drows);
-  int lanes = 1;
-  while (lanes < 32 && lanes < c / vec) lanes *= 2;
-  const int64_t blocks = cdiv(n * k, 2 * (kThreads / lanes));
+  const int lanes = row_lanes(c / vec);
+  const int grid = grid_for(n * k * lanes, kThreads, TSB_GRID);
   return dispatch_pack(dtype, vec, [&](auto tag) -> int {
     using T = typename decltype(tag)::T;
     constexpr int VEC = decltype(tag)::VEC;
-    combine_grad_kernel<T, VEC><<<(unsigned)blocks, kThreads, 0, as_stream(stream)>>>(
+    combine_grad_kernel<T, VEC><<<grid, kThreads, 0, as_stream(stream)>>>(
         (const T*)dout, (const T*)rows, weights, weights_dtype, inverse, kept, n * k, row_split(k), c, lanes, (T*)drows, dweights);
     TSB_LAUNCH_CHECK();
     return TSB_OK;
