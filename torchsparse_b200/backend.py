@@ -16,7 +16,6 @@ Differences from the reference that callers can see:
 """
 from __future__ import annotations
 
-from functools import lru_cache
 from typing import List, Optional, Sequence, Tuple
 
 import torch
@@ -36,8 +35,6 @@ __all__ = [
     "conv_forward_fetch_on_demand_no_fusion_cuda", "voxelize_forward_cuda", "devoxelize_forward_cuda",
     "voxelize_backward_cuda", "devoxelize_backward_cuda", "hash_cuda", "kernel_hash_cuda", "hash_query_cuda", "count_cuda", "to_dense_forward_cuda", "to_dense_backward_cuda",
     "pairs_from_out_in_map", "quantize_unique_cuda", "tile_mask_cuda", "sorted_cm_artefacts_cuda", "SortedMap",
-    "group_rows_cuda", "group_norm_forward_cuda", "group_norm_backward_cuda", "embedding_forward_cuda",
-    "embedding_backward_cuda", "expert_dispatch_cuda", "expert_combine_cuda", "expert_combine_backward_cuda",
 ]
 
 _DTYPES = {torch.float32: _lib.TSB_F32, torch.float16: _lib.TSB_F16, torch.bfloat16: _lib.TSB_BF16}
@@ -1258,263 +1255,3 @@ def quantize_unique_cuda(xyz: torch.Tensor, voxel_size: Sequence[float], return_
     nv = res[0]
     bounds = (tuple(res[1:4]), tuple(res[4:7])) if nv else ((0, 0, 0), (0, 0, 0))
     return uniq[:nv], (first[:nv] if first is not None else None), inv, bounds
-
-
-# --------------------------------------------------------------------------- rows grouped by an index
-# These have no counterpart in the reference's pybind module.  Launches go to the current stream of the tensors'
-# device, which need not be the current device.
-ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "leaky_relu": 2, "silu": 3}
-_MAX_ROWS = 2 ** 31 - 1
-# workspace sizes depend on sizes alone; at small ones the call costs as much as a lookup saves
-_group_rows_bytes = lru_cache(1024)(lib.tsb_group_rows_workspace_bytes)
-_norm_fwd_bytes = lru_cache(1024)(lib.tsb_group_norm_fwd_workspace_bytes)
-_norm_bwd_bytes = lru_cache(1024)(lib.tsb_group_norm_bwd_workspace_bytes)
-_embed_bwd_bytes = lru_cache(1024)(lib.tsb_embedding_bwd_workspace_bytes)
-
-
-class _Here:
-    """``with`` block of the case that needs no device switch."""
-
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
-
-
-_HERE = _Here()
-
-
-def _on_device_of(t: torch.Tensor):
-    return _HERE if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
-
-
-def _scratch(nbytes: int, device):
-    """(tensor or None, address or None) of a workspace that may be empty."""
-    if nbytes == 0:
-        return None, None
-    t = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    return t, t.data_ptr()
-
-
-def _same_device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
-    if not first.is_cuda:
-        _need_cuda(first)
-    device = first.device
-    for t in others:
-        if t is not None and t.device != device:
-            _need_cuda(t)
-            raise ValueError(f"tensors live on {device} and {t.device}")
-
-
-def _index_tensor(t: torch.Tensor, what: str) -> torch.Tensor:
-    if t.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"{what} must be int32 or int64, not {t.dtype}")
-    return t
-
-
-def _int32_vector(t: torch.Tensor, length: Optional[int], what: str) -> None:
-    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or (length is not None and t.shape[0] != length):
-        raise ValueError(f"{what} must be a contiguous int32 vector" + ("" if length is None else f" of length {length}"))
-
-
-def group_rows_cuda(keys: torch.Tensor, num_groups: int, want_inverse: bool = False):
-    """Stable grouping of ``keys`` (int32 or int64 [N], any stride): ``(order, inverse or None, offsets)``, all int32.
-    Keys outside [0, num_groups) come last, from position ``offsets[num_groups]`` on."""
-    _need_cuda(keys)
-    _index_tensor(keys, "keys")
-    if keys.dim() != 1:
-        raise ValueError(f"keys must be a vector, not {tuple(keys.shape)}")
-    num_groups, n = int(num_groups), keys.shape[0]
-    if not 1 <= num_groups <= _MAX_ROWS:
-        raise ValueError(f"num_groups must be in [1, 2^31), not {num_groups}")
-    dev = keys.device
-    order = torch.empty(n, dtype=torch.int32, device=dev)
-    inverse = torch.empty(n, dtype=torch.int32, device=dev) if want_inverse else None
-    offsets = torch.empty(num_groups + 1, dtype=torch.int32, device=dev)
-    nbytes = _group_rows_bytes(n, num_groups)
-    ws, at = _scratch(nbytes, dev)
-    with _on_device_of(keys):
-        check(lib.tsb_group_rows(keys.data_ptr(), keys.dtype == torch.int64, keys.stride(0), n, num_groups, order.data_ptr(),
-                                 _p(inverse), offsets.data_ptr(), at, nbytes, _stream()), "group_rows")
-    return order, inverse, offsets
-
-
-def _norm_args(feats, order, offsets, num_groups, weight, bias, activation):
-    """Checked arguments of the two group norm calls: (activation code, feature dtype code, parameter dtype code)."""
-    _same_device(feats, order, offsets, weight, bias)
-    if feats.dim() != 2 or feats.shape[1] < 1:
-        raise ValueError(f"group_norm expects features [N, C], not {tuple(feats.shape)}")
-    n, c = feats.shape
-    if num_groups < 1 or c % num_groups != 0:
-        raise ValueError(f"{c} channels do not divide into {num_groups} groups")
-    _int32_vector(offsets, None, "offsets")
-    if offsets.shape[0] < 1:
-        raise ValueError("offsets must hold the first row of every sample and the end of the last")
-    if order is not None:
-        _int32_vector(order, n, "order")
-    code = None
-    for p in (weight, bias):
-        if p is not None:
-            if p.dim() != 1 or p.shape[0] != c:
-                raise ValueError(f"weight and bias must be vectors of {c} values, not {tuple(p.shape)}")
-            if code is not None and _dtype_code(p) != code:
-                raise ValueError("weight and bias must have one dtype")
-            code = _dtype_code(p)
-    if activation not in ACTIVATIONS:
-        raise ValueError(f"unknown activation {activation!r}: one of {sorted(k for k in ACTIVATIONS if k)}")
-    return ACTIVATIONS[activation], _dtype_code(feats), _lib.TSB_F32 if code is None else code
-
-
-def group_norm_forward_cuda(feats: torch.Tensor, order: Optional[torch.Tensor], offsets: torch.Tensor, num_groups: int,
-                            weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5,
-                            activation: Optional[str] = None, negative_slope: float = 0.01, want_stats: bool = True):
-    """``(y, stats)`` of ``act(group_norm(feats))`` over the samples ``offsets`` delimits; stats is fp32
-    [2, samples, num_groups], the means and the reciprocal deviations (None unless wanted)."""
-    act, dtype, code = _norm_args(feats, order, offsets, num_groups, weight, bias, activation)
-    feats = feats.contiguous()
-    weight, bias = weight if weight is None else weight.contiguous(), bias if bias is None else bias.contiguous()
-    n, c = feats.shape
-    samples, device = offsets.shape[0] - 1, feats.device
-    y = torch.empty_like(feats)
-    stats = mean = rstd = None
-    if want_stats:
-        stats = torch.empty((2, samples, num_groups), dtype=torch.float32, device=device)
-        mean = stats.data_ptr()
-        rstd = mean + 4 * samples * num_groups
-    nbytes = _norm_fwd_bytes(n, c, num_groups, samples, dtype)
-    ws, at = _scratch(nbytes, device)
-    with _on_device_of(feats):
-        check(lib.tsb_group_norm_fwd(feats.data_ptr(), _p(order), offsets.data_ptr(), _p(weight), _p(bias), n, c, num_groups,
-                                     samples, eps, act, negative_slope, dtype, code, y.data_ptr(), mean, rstd, at, nbytes,
-                                     _stream()), "group_norm")
-    return y, stats
-
-
-def group_norm_backward_cuda(feats: torch.Tensor, grad: torch.Tensor, order: Optional[torch.Tensor], offsets: torch.Tensor,
-                             num_groups: int, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor],
-                             stats: torch.Tensor, activation: Optional[str] = None, negative_slope: float = 0.01):
-    """``(dfeats, dweight or None, dbias or None)`` of ``group_norm_forward_cuda``."""
-    act, dtype, code = _norm_args(feats, order, offsets, num_groups, weight, bias, activation)
-    _same_device(feats, grad, stats)
-    if grad.shape != feats.shape or grad.dtype != feats.dtype:
-        raise ValueError("the gradient must have the features' shape and dtype")
-    n, c = feats.shape
-    samples, device = offsets.shape[0] - 1, feats.device
-    if stats.dtype != torch.float32 or tuple(stats.shape) != (2, samples, num_groups) or not stats.is_contiguous():
-        raise ValueError("stats must be what the forward call returned")
-    mean = stats.data_ptr()
-    feats, grad = feats.contiguous(), grad.contiguous()
-    weight, bias = weight if weight is None else weight.contiguous(), bias if bias is None else bias.contiguous()
-    dx = torch.empty_like(feats)
-    dweight = None if weight is None else torch.empty_like(weight)
-    dbias = None if bias is None else torch.empty_like(bias)
-    nbytes = _norm_bwd_bytes(n, c, num_groups, samples, dtype)
-    ws, at = _scratch(nbytes, device)
-    with _on_device_of(feats):
-        check(lib.tsb_group_norm_bwd(feats.data_ptr(), grad.data_ptr(), _p(order), offsets.data_ptr(), _p(weight), _p(bias), mean,
-                                     mean + 4 * samples * num_groups, n, c, num_groups, samples, act, negative_slope, dtype, code,
-                                     dx.data_ptr(), _p(dweight), _p(dbias), at, nbytes, _stream()), "group_norm_backward")
-    return dx, dweight, dbias
-
-
-def embedding_forward_cuda(indices: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
-    """``scale * table[indices]`` for a vector of int32 or int64 indices; an index that is no row gives zeros."""
-    _same_device(table, indices)
-    _index_tensor(indices, "indices")
-    if table.dim() != 2 or table.shape[1] < 1 or indices.dim() != 1:
-        raise ValueError("embedding expects a table [rows, channels] and a vector of indices")
-    dtype = _dtype_code(table)
-    table, indices = table.contiguous(), indices.contiguous()
-    out = torch.empty((indices.shape[0], table.shape[1]), dtype=table.dtype, device=table.device)
-    with _on_device_of(table):
-        check(lib.tsb_embedding_fwd(table.data_ptr(), indices.data_ptr(), indices.dtype == torch.int64, indices.shape[0],
-                                    table.shape[0], table.shape[1], scale, dtype, out.data_ptr(), _stream()), "embedding")
-    return out
-
-
-def embedding_backward_cuda(grad: torch.Tensor, indices: torch.Tensor, num_rows: int, scale: float = 1.0,
-                            padding_idx: Optional[int] = None) -> torch.Tensor:
-    """The gradient of the table, [num_rows, C] in the gradient's dtype, summed in fp32 in the order of the rows."""
-    _same_device(grad, indices)
-    _index_tensor(indices, "indices")
-    if grad.dim() != 2 or indices.dim() != 1 or grad.shape[0] != indices.shape[0] or grad.shape[1] < 1:
-        raise ValueError("embedding_backward expects a gradient [N, C] and N indices")
-    dtype, num_rows = _dtype_code(grad), int(num_rows)
-    if not 0 <= num_rows <= _MAX_ROWS:
-        raise ValueError(f"num_rows must be in [0, 2^31), not {num_rows}")
-    grad, indices = grad.contiguous(), indices.contiguous()
-    n, c = grad.shape
-    out = torch.empty((num_rows, c), dtype=grad.dtype, device=grad.device)
-    nbytes = _embed_bwd_bytes(n, num_rows, c, dtype)
-    ws, at = _scratch(nbytes, grad.device)
-    with _on_device_of(grad):
-        check(lib.tsb_embedding_bwd(grad.data_ptr(), indices.data_ptr(), indices.dtype == torch.int64, n, num_rows, c, scale,
-                                    -1 if padding_idx is None else padding_idx, dtype, out.data_ptr(), at, nbytes, _stream()),
-              "embedding_backward")
-    return out
-
-
-def _expert_args(inverse: torch.Tensor, offsets: torch.Tensor):
-    """(N, k, address of the number of kept choices) of the plan ``group_rows_cuda`` made of [N, k] choices."""
-    if inverse.dim() != 2 or inverse.dtype != torch.int32 or not inverse.is_contiguous() or inverse.shape[1] < 1:
-        raise ValueError("inverse must be contiguous int32 [N, k]")
-    _int32_vector(offsets, None, "offsets")
-    if offsets.shape[0] < 2:
-        raise ValueError("offsets must hold the first position of every expert and the end of the last")
-    return inverse.shape[0], inverse.shape[1], offsets.data_ptr() + 4 * (offsets.shape[0] - 1)
-
-
-def expert_dispatch_cuda(feats: torch.Tensor, inverse: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
-    """[N * k, C]: row i of ``feats`` at every position ``inverse[i, j]``, zeros behind the kept choices."""
-    _same_device(feats, inverse, offsets)
-    n, k, kept = _expert_args(inverse, offsets)
-    if feats.dim() != 2 or feats.shape[0] != n or feats.shape[1] < 1:
-        raise ValueError(f"expert_dispatch expects features [{n}, C], not {tuple(feats.shape)}")
-    dtype = _dtype_code(feats)
-    feats = feats.contiguous()
-    out = torch.empty((n * k, feats.shape[1]), dtype=feats.dtype, device=feats.device)
-    with _on_device_of(feats):
-        check(lib.tsb_expert_dispatch(_p(feats), _p(inverse), kept, n, k, feats.shape[1], dtype, _p(out), _stream()),
-              "expert_dispatch")
-    return out
-
-
-def _expert_rows(rows, n, k, weights):
-    if rows.dim() != 2 or rows.shape[0] != n * k or rows.shape[1] < 1:
-        raise ValueError(f"expert_combine expects sorted rows [{n * k}, C], not {tuple(rows.shape)}")
-    if weights is not None and tuple(weights.shape) != (n, k):
-        raise ValueError(f"expert_combine expects weights [{n}, {k}], not {tuple(weights.shape)}")
-
-
-def expert_combine_cuda(rows: torch.Tensor, weights: Optional[torch.Tensor], inverse: torch.Tensor,
-                        offsets: torch.Tensor) -> torch.Tensor:
-    """[N, C]: the sum over j of ``weights[i, j] * rows[inverse[i, j]]`` (no weights: 1)."""
-    _same_device(rows, weights, inverse, offsets)
-    n, k, kept = _expert_args(inverse, offsets)
-    _expert_rows(rows, n, k, weights)
-    dtype, w_dtype = _dtype_code(rows), _lib.TSB_F32 if weights is None else _dtype_code(weights)
-    rows = rows.contiguous()
-    weights = None if weights is None else weights.contiguous()
-    out = torch.empty((n, rows.shape[1]), dtype=rows.dtype, device=rows.device)
-    with _on_device_of(rows):
-        check(lib.tsb_expert_combine(_p(rows), _p(weights), w_dtype, _p(inverse), kept, n, k, rows.shape[1], dtype, _p(out),
-                                     _stream()), "expert_combine")
-    return out
-
-
-def expert_combine_backward_cuda(grad: torch.Tensor, rows: torch.Tensor, weights: torch.Tensor, inverse: torch.Tensor,
-                                 offsets: torch.Tensor):
-    """``(drows, dweights)`` of ``expert_combine_cuda``."""
-    _same_device(grad, rows, weights, inverse, offsets)
-    n, k, kept = _expert_args(inverse, offsets)
-    _expert_rows(rows, n, k, weights)
-    if tuple(grad.shape) != (n, rows.shape[1]) or grad.dtype != rows.dtype:
-        raise ValueError("the gradient must be [N, C] in the rows' dtype")
-    dtype, w_dtype = _dtype_code(rows), _dtype_code(weights)
-    grad, rows, weights = grad.contiguous(), rows.contiguous(), weights.contiguous()
-    drows, dweights = torch.empty_like(rows), torch.empty_like(weights)
-    with _on_device_of(rows):
-        check(lib.tsb_expert_combine_bwd(_p(grad), _p(rows), _p(weights), w_dtype, _p(inverse), kept, n, k, rows.shape[1], dtype,
-                                         _p(drows), _p(dweights), _stream()), "expert_combine_backward")
-    return drows, dweights

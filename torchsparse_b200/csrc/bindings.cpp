@@ -1,0 +1,360 @@
+// The operators over grouped rows as torch operators with gradients: argument checks, allocation and the autograd nodes, in
+// C++ because at the sizes of one resolution level a call through ctypes and Python autograd costs several times what
+// its kernels take (embedding with its gradient, smallest sizes: 97 us a pass there, 58 us here).
+//
+// Every call goes to the C entries of include/tsb200.h, on the current stream of the tensors' device.
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/extension.h>
+
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+
+#include "../../include/tsb200.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::Function;
+using torch::autograd::variable_list;
+
+void check_status(int status, const char* what) {
+  if (status == TSB_OK) return;
+  std::string text = std::string(what) + ": " + tsb_status_string(status);
+  if (status == TSB_ERR_CUDA) text += std::string(": ") + tsb_last_cuda_error();
+  TORCH_CHECK_VALUE(status != TSB_ERR_BAD_ARG && status != TSB_ERR_LIMIT, text);
+  TORCH_CHECK(false, text);
+}
+
+void need_cuda(const Tensor& t) {
+  TORCH_CHECK(!t.defined() || t.is_cuda(), "torchsparse_b200: CUDA tensors required (there is no CPU fallback)");
+}
+
+void same_device(const Tensor& first, std::initializer_list<Tensor> others) {
+  need_cuda(first);
+  for (const Tensor& t : others) {
+    if (!t.defined()) continue;
+    need_cuda(t);
+    TORCH_CHECK_VALUE(t.device() == first.device(), "tensors live on ", first.device(), " and ", t.device());
+  }
+}
+
+int dtype_code(const Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return TSB_F32;
+    case at::kHalf: return TSB_F16;
+    case at::kBFloat16: return TSB_BF16;
+    default: TORCH_CHECK(false, "unsupported feature dtype ", t.scalar_type());
+  }
+}
+
+void check_index(const Tensor& t, const char* what) {
+  TORCH_CHECK_VALUE(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, what, " must be int32 or int64, not ",
+                    t.scalar_type());
+}
+
+void check_int32(const Tensor& t, int64_t length, const char* what) {
+  TORCH_CHECK_VALUE(t.scalar_type() == at::kInt && t.dim() == 1 && t.is_contiguous() && (length < 0 || t.size(0) == length), what,
+                    " must be a contiguous int32 vector", length < 0 ? std::string() : " of length " + std::to_string(length));
+}
+
+const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+void* out_ptr(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
+const int32_t* ints(const Tensor& t) { return t.defined() ? t.const_data_ptr<int32_t>() : nullptr; }
+Tensor packed(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+std::optional<Tensor> given(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
+
+// device guard, stream and an optional workspace of one call
+struct Call {
+  c10::cuda::CUDAGuard guard;
+  Tensor scratch;
+  size_t bytes = 0;
+  explicit Call(const Tensor& t) : guard(t.device()) {}
+  void* workspace(size_t n, const Tensor& like) {
+    bytes = n;
+    if (n) scratch = at::empty({(int64_t)n}, like.options().dtype(at::kByte));
+    return n ? scratch.mutable_data_ptr() : nullptr;
+  }
+  tsb_stream_t stream() const { return c10::cuda::getCurrentCUDAStream().stream(); }
+};
+
+bool wants_grad(std::initializer_list<Tensor> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor& t : ts)
+    if (t.defined() && t.requires_grad()) return true;
+  return false;
+}
+
+// What a backward call returns: its kernels have no gradient of their own, and asking for one is an error, not a zero.
+variable_list once(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  int n = 0;
+  for (const Tensor& t : grads) n += t.defined();
+  auto refuse = std::make_shared<torch::autograd::DelayedError>(
+      "this operator of torchsparse_b200 can be differentiated once only", n);
+  variable_list in;
+  for (const Tensor& t : grads)
+    if (t.defined()) in.push_back(t.detach().requires_grad_());
+  variable_list made = (*refuse)(std::move(in));
+  size_t k = 0;
+  for (Tensor& t : grads)
+    if (t.defined()) t = made[k++];
+  return grads;
+}
+
+// ------------------------------------------------------------------------------------------------ grouping
+std::tuple<Tensor, Tensor, Tensor> group_rows(const Tensor& keys, int64_t num_groups, bool want_inverse) {
+  need_cuda(keys);
+  check_index(keys, "keys");
+  TORCH_CHECK_VALUE(keys.dim() == 1, "keys must be a vector, not ", keys.sizes());
+  TORCH_CHECK_VALUE(num_groups >= 1 && num_groups < (1ll << 31), "the number of groups must be in [1, 2^31), not ", num_groups);
+  Call call(keys);
+  const int64_t n = keys.size(0);
+  const auto opts = keys.options().dtype(at::kInt);
+  Tensor order = at::empty({n}, opts), offsets = at::empty({num_groups + 1}, opts), inverse;
+  if (want_inverse) inverse = at::empty({n}, opts);
+  void* ws = call.workspace(tsb_group_rows_workspace_bytes(n, num_groups), keys);
+  check_status(tsb_group_rows(keys.const_data_ptr(), keys.scalar_type() == at::kLong, keys.stride(0), n, num_groups,
+                              order.mutable_data_ptr<int32_t>(), (int32_t*)out_ptr(inverse), offsets.mutable_data_ptr<int32_t>(), ws,
+                              call.bytes, call.stream()),
+               "group_rows");
+  return {order, inverse, offsets};
+}
+
+// ------------------------------------------------------------------------------------------------ group norm
+struct NormArgs {
+  int64_t groups;
+  double eps, slope;
+  int64_t act;
+};
+
+int check_norm(const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& offsets, const Tensor& order, int64_t groups) {
+  same_device(x, {weight, bias, offsets, order});
+  TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) >= 1, "group_norm expects features [N, C], not ", x.sizes());
+  const int64_t c = x.size(1);
+  TORCH_CHECK_VALUE(groups >= 1 && c % groups == 0, c, " channels do not divide into ", groups, " groups");
+  check_int32(offsets, -1, "offsets");
+  TORCH_CHECK_VALUE(offsets.size(0) >= 1, "offsets must hold the first row of every sample and the end of the last");
+  if (order.defined()) check_int32(order, x.size(0), "order");
+  dtype_code(x);
+  int code = -1;
+  for (const Tensor* p : {&weight, &bias}) {
+    if (!p->defined()) continue;
+    TORCH_CHECK_VALUE(p->dim() == 1 && p->size(0) == c, "weight and bias must be vectors of ", c, " values, not ", p->sizes());
+    TORCH_CHECK_VALUE(code < 0 || code == dtype_code(*p), "weight and bias must have one dtype");
+    code = dtype_code(*p);
+  }
+  return code < 0 ? (int)TSB_F32 : code;
+}
+
+// (y, [2, samples, groups] of means and reciprocal deviations, or an undefined tensor)
+std::pair<Tensor, Tensor> norm_forward(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& offsets, const Tensor& order,
+                                       const NormArgs& a, int p_code, bool want_stats) {
+  Call call(x);
+  const int64_t n = x.size(0), c = x.size(1), samples = offsets.size(0) - 1;
+  Tensor y = at::empty_like(x), stats;
+  float *mean = nullptr, *rstd = nullptr;
+  if (want_stats) {
+    stats = at::empty({2, samples, a.groups}, x.options().dtype(at::kFloat));
+    mean = stats.mutable_data_ptr<float>();
+    rstd = mean + samples * a.groups;
+  }
+  const int dtype = dtype_code(x);
+  void* ws = call.workspace(tsb_group_norm_fwd_workspace_bytes(n, c, a.groups, samples, dtype), x);
+  check_status(tsb_group_norm_fwd(ptr(x), ints(order), ints(offsets), ptr(w), ptr(b), n, c, a.groups, samples, (float)a.eps,
+                                  (int)a.act, (float)a.slope, dtype, p_code, out_ptr(y), mean, rstd, ws, call.bytes, call.stream()),
+               "group_norm");
+  return {y, stats};
+}
+
+struct GroupNorm : Function<GroupNorm> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias,
+                        const Tensor& offsets, const std::optional<Tensor>& order, int64_t groups, double eps, int64_t act,
+                        double slope, int64_t p_code) {
+    const NormArgs a{groups, eps, slope, act};
+    const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor()), o = order.value_or(Tensor());
+    auto [y, stats] = norm_forward(x, w, b, offsets, o, a, (int)p_code, true);
+    ctx->save_for_backward({x, w, b, offsets, o, stats});
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["slope"] = slope;
+    ctx->saved_data["code"] = p_code;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &w = saved[1], &b = saved[2], &offsets = saved[3], &order = saved[4], &stats = saved[5];
+    const int64_t n = x.size(0), c = x.size(1), samples = offsets.size(0) - 1, groups = ctx->saved_data["groups"].toInt();
+    Call call(x);
+    const Tensor dy = grads[0].contiguous();
+    Tensor dx = at::empty_like(x), dw, db;
+    if (w.defined()) dw = at::empty_like(w);
+    if (b.defined()) db = at::empty_like(b);
+    const float* mean = stats.const_data_ptr<float>();
+    const int dtype = dtype_code(x);
+    void* ws = call.workspace(tsb_group_norm_bwd_workspace_bytes(n, c, groups, samples, dtype), x);
+    check_status(tsb_group_norm_bwd(ptr(x), ptr(dy), ints(order), ints(offsets), ptr(w), ptr(b), mean, mean + samples * groups, n, c,
+                                    groups, samples, (int)ctx->saved_data["act"].toInt(), (float)ctx->saved_data["slope"].toDouble(),
+                                    dtype, (int)ctx->saved_data["code"].toInt(), out_ptr(dx), out_ptr(dw), out_ptr(db), ws, call.bytes,
+                                    call.stream()),
+                 "group_norm_backward");
+    auto made = once({dx, dw, db});
+    made.resize(10);
+    return made;
+  }
+};
+
+Tensor group_norm(const Tensor& feats, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, const Tensor& offsets,
+                  const std::optional<Tensor>& order, int64_t groups, double eps, int64_t act, double slope) {
+  const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor()), o = order.value_or(Tensor());
+  const int code = check_norm(feats, w, b, offsets, o, groups);
+  if (wants_grad({feats, w, b}))
+    return GroupNorm::apply(packed(feats), given(packed(w)), given(packed(b)), offsets, given(o), groups, eps, act, slope,
+                            (int64_t)code);
+  return norm_forward(packed(feats), packed(w), packed(b), offsets, o, NormArgs{groups, eps, slope, act}, code, false).first;
+}
+
+// ------------------------------------------------------------------------------------------------ embedding
+Tensor embedding_forward(const Tensor& table, const Tensor& indices, double scale) {
+  Call call(table);
+  const int64_t n = indices.size(0), c = table.size(1);
+  Tensor out = at::empty({n, c}, table.options());
+  check_status(tsb_embedding_fwd(ptr(table), ptr(indices), indices.scalar_type() == at::kLong, n, table.size(0), c, (float)scale,
+                                 dtype_code(table), out_ptr(out), call.stream()),
+               "embedding");
+  return out;
+}
+
+struct Embedding : Function<Embedding> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& table, const Tensor& indices, double scale, int64_t padding) {
+    ctx->save_for_backward({indices});
+    ctx->saved_data["rows"] = table.size(0);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding"] = padding;
+    return embedding_forward(table, indices, scale);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const Tensor indices = ctx->get_saved_variables()[0], dy = grads[0].contiguous();
+    const int64_t n = indices.size(0), rows = ctx->saved_data["rows"].toInt(), c = dy.size(1);
+    Call call(dy);
+    Tensor dtable = at::empty({rows, c}, dy.options());
+    const int dtype = dtype_code(dy);
+    void* ws = call.workspace(tsb_embedding_bwd_workspace_bytes(n, rows, c, dtype), dy);
+    check_status(tsb_embedding_bwd(ptr(dy), ptr(indices), indices.scalar_type() == at::kLong, n, rows, c,
+                                   (float)ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt(), dtype,
+                                   out_ptr(dtable), ws, call.bytes, call.stream()),
+                 "embedding_backward");
+    auto made = once({dtable});
+    made.resize(4);
+    return made;
+  }
+};
+
+// padding: the row that gets no gradient, -1 for none
+Tensor embedding(const Tensor& table, const Tensor& indices, double scale, int64_t padding) {
+  same_device(table, {indices});
+  check_index(indices, "indices");
+  dtype_code(table);
+  TORCH_CHECK_VALUE(table.dim() == 2 && table.size(1) >= 1, "embedding expects a table [rows, channels], not ", table.sizes());
+  const Tensor flat = (indices.dim() == 1 ? indices : indices.reshape(-1)).contiguous();
+  const Tensor out = wants_grad({table}) ? Embedding::apply(packed(table), flat, scale, padding)
+                                         : embedding_forward(packed(table), flat, scale);
+  if (indices.dim() == 1) return out;
+  auto shape = indices.sizes().vec();
+  shape.push_back(table.size(1));
+  return out.view(shape);
+}
+
+// ------------------------------------------------------------------------------------------------ experts
+// the plan of [N, k] choices: (N, k, address of the number of kept choices)
+std::tuple<int64_t, int32_t, const int32_t*> plan(const Tensor& inverse, const Tensor& offsets) {
+  TORCH_CHECK_VALUE(inverse.dim() == 2 && inverse.scalar_type() == at::kInt && inverse.is_contiguous() && inverse.size(1) >= 1 &&
+                        inverse.size(1) < (1ll << 31),
+                    "inverse must be contiguous int32 [N, k]");
+  check_int32(offsets, -1, "offsets");
+  TORCH_CHECK_VALUE(offsets.size(0) >= 2, "offsets must hold the first position of every expert and the end of the last");
+  return {inverse.size(0), (int32_t)inverse.size(1), ints(offsets) + offsets.size(0) - 1};
+}
+
+Tensor dispatch(const Tensor& x, const Tensor& inverse, const Tensor& offsets) {
+  const auto [n, k, kept] = plan(inverse, offsets);
+  Call call(x);
+  Tensor out = at::empty({n * k, x.size(1)}, x.options());
+  check_status(tsb_expert_dispatch(ptr(x), ints(inverse), kept, n, k, x.size(1), dtype_code(x), out_ptr(out), call.stream()),
+               "expert_dispatch");
+  return out;
+}
+
+Tensor combine(const Tensor& rows, const Tensor& weights, const Tensor& inverse, const Tensor& offsets) {
+  const auto [n, k, kept] = plan(inverse, offsets);
+  Call call(rows);
+  Tensor out = at::empty({n, rows.size(1)}, rows.options());
+  check_status(tsb_expert_combine(ptr(rows), ptr(weights), weights.defined() ? dtype_code(weights) : (int)TSB_F32, ints(inverse), kept,
+                                  n, k, rows.size(1), dtype_code(rows), out_ptr(out), call.stream()),
+               "expert_combine");
+  return out;
+}
+
+struct Dispatch : Function<Dispatch> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& inverse, const Tensor& offsets) {
+    ctx->save_for_backward({inverse, offsets});
+    return dispatch(x, inverse, offsets);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    auto made = once({combine(grads[0].contiguous(), Tensor(), saved[0], saved[1])});
+    made.resize(3);
+    return made;
+  }
+};
+
+struct Combine : Function<Combine> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& weights, const Tensor& inverse, const Tensor& offsets) {
+    ctx->save_for_backward({rows, weights, inverse, offsets});
+    return combine(rows, weights, inverse, offsets);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &rows = saved[0], &weights = saved[1], dout = grads[0].contiguous();
+    const auto [n, k, kept] = plan(saved[2], saved[3]);
+    Call call(rows);
+    Tensor drows = at::empty_like(rows), dweights = at::empty_like(weights);
+    check_status(tsb_expert_combine_bwd(ptr(dout), ptr(rows), ptr(weights), dtype_code(weights), ints(saved[2]), kept, n, k,
+                                        rows.size(1), dtype_code(rows), out_ptr(drows), out_ptr(dweights), call.stream()),
+                 "expert_combine_backward");
+    auto made = once({drows, dweights});
+    made.resize(4);
+    return made;
+  }
+};
+
+Tensor expert_dispatch(const Tensor& x, const Tensor& inverse, const Tensor& offsets) {
+  same_device(x, {inverse, offsets});
+  const int64_t n = std::get<0>(plan(inverse, offsets));
+  TORCH_CHECK_VALUE(x.dim() == 2 && x.size(0) == n && x.size(1) >= 1, "expert_dispatch expects features [", n, ", C], not ", x.sizes());
+  dtype_code(x);
+  return wants_grad({x}) ? Dispatch::apply(packed(x), inverse, offsets) : dispatch(packed(x), inverse, offsets);
+}
+
+Tensor expert_combine(const Tensor& rows, const Tensor& weights, const Tensor& inverse, const Tensor& offsets) {
+  same_device(rows, {weights, inverse, offsets});
+  const auto [n, k, kept] = plan(inverse, offsets);
+  TORCH_CHECK_VALUE(rows.dim() == 2 && rows.size(0) == n * k && rows.size(1) >= 1, "expert_combine expects sorted rows [", n * k,
+                    ", C], not ", rows.sizes());
+  TORCH_CHECK_VALUE(weights.dim() == 2 && weights.size(0) == n && weights.size(1) == k, "expert_combine expects weights [", n, ", ", k,
+                    "], not ", weights.sizes());
+  dtype_code(rows);
+  dtype_code(weights);
+  return wants_grad({rows, weights}) ? Combine::apply(packed(rows), packed(weights), inverse, offsets)
+                                     : combine(packed(rows), packed(weights), inverse, offsets);
+}
+
+}  // namespace
+
+PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  m.def("group_rows", &group_rows);
+  m.def("group_norm", &group_norm);
+  m.def("embedding", &embedding);
+  m.def("expert_dispatch", &expert_dispatch);
+  m.def("expert_combine", &expert_combine);
+}

@@ -24,6 +24,33 @@ def _newer(a: str, b: str) -> bool:
     return (not os.path.exists(b)) or os.path.getmtime(a) > os.path.getmtime(b)
 
 
+BINDINGS = os.path.join(HERE, "_bindings.so")
+
+
+def build_bindings(force: bool = False) -> str:
+    """The torch operators of bindings.cpp (autograd nodes over the C ABI), a Python module beside the library."""
+    import sysconfig
+
+    src, hdr = os.path.join(HERE, "bindings.cpp"), os.path.join(HERE, "..", "..", "include", "tsb200.h")
+    if not force and not _newer(src, BINDINGS) and not _newer(hdr, BINDINGS):
+        return BINDINGS
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    cuda = os.path.dirname(os.path.dirname(os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")))
+    incs = include_paths() + [os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
+    libs = library_paths()
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", src, "-o", BINDINGS, "-DTORCH_EXTENSION_NAME=_bindings",
+           "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    cmd += [f"-isystem{p}" for p in incs] + [f"-L{p}" for p in libs] + [f"-L{HERE}"]
+    cmd += ["-l:libtsb200.so", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda",
+            "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {src}:\n{r.stderr}")
+    return BINDINGS
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
     hdrs = [os.path.join(HERE, h) for h in HEADERS]
@@ -52,6 +79,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         list(ex.map(cc, jobs))
     if jobs or not os.path.exists(LIB):
         subprocess.check_call([nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-o", LIB, *objs, "-lcudart"])
+    build_bindings(force)
     return LIB
 
 

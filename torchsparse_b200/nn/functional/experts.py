@@ -1,10 +1,8 @@
 from typing import NamedTuple
 
 import torch
-from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
-from ... import backend
+from ... import _ops
 
 __all__ = ["ExpertRows", "expert_sort", "expert_dispatch", "expert_combine"]
 
@@ -19,33 +17,6 @@ class ExpertRows(NamedTuple):
     offsets: torch.Tensor
 
 
-class _Dispatch(Function):
-    @staticmethod
-    def forward(ctx, feats: torch.Tensor, inverse: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
-        ctx.save_for_backward(inverse, offsets)
-        return backend.expert_dispatch_cuda(feats, inverse, offsets)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_output: torch.Tensor):
-        inverse, offsets = ctx.saved_tensors
-        return backend.expert_combine_cuda(grad_output, None, inverse, offsets), None, None
-
-
-class _Combine(Function):
-    @staticmethod
-    def forward(ctx, rows: torch.Tensor, weights: torch.Tensor, inverse: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
-        ctx.save_for_backward(rows, weights, inverse, offsets)
-        return backend.expert_combine_cuda(rows, weights, inverse, offsets)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_output: torch.Tensor):
-        rows, weights, inverse, offsets = ctx.saved_tensors
-        drows, dweights = backend.expert_combine_backward_cuda(grad_output, rows, weights, inverse, offsets)
-        return drows, dweights, None, None
-
-
 def expert_sort(experts: torch.Tensor, num_experts: int) -> ExpertRows:
     """Sort the choices of a router: ``experts`` int32 or int64 [N, k] (or [N]) names the weight matrices that row i is
     sent to.  Choices of one expert keep their order; a choice outside [0, num_experts) (-1, say, for one dropped for
@@ -55,22 +26,18 @@ def expert_sort(experts: torch.Tensor, num_experts: int) -> ExpertRows:
     shape = (experts.shape[0], experts.shape[1] if experts.dim() == 2 else 1)
     if shape[1] < 1:
         raise ValueError("every row needs at least one choice")
-    order, inverse, offsets = backend.group_rows_cuda(experts.reshape(-1), num_experts, want_inverse=True)
+    order, inverse, offsets = _ops.group_rows(experts.reshape(-1), num_experts, True)
     return ExpertRows(order, inverse.view(shape), offsets)
 
 
 def expert_dispatch(feats: torch.Tensor, rows: ExpertRows) -> torch.Tensor:
     """[N * k, C]: the rows of ``feats`` sorted by expert, those of expert e at positions ``offsets[e]`` to
     ``offsets[e + 1]``; zeros behind the last expert.  The gradient adds up a row's k copies in their order."""
-    if torch.is_grad_enabled() and feats.requires_grad:
-        return _Dispatch.apply(feats, rows.inverse, rows.offsets)
-    return backend.expert_dispatch_cuda(feats, rows.inverse, rows.offsets)
+    return _ops.expert_dispatch(feats, rows.inverse, rows.offsets)
 
 
 def expert_combine(feats: torch.Tensor, weights: torch.Tensor, rows: ExpertRows) -> torch.Tensor:
     """[N, C]: row i is the sum over its choices of ``weights[i, j]`` times the sorted row of that choice (``feats``
     [N * k, C], what the experts made of the dispatched rows); a choice without an expert adds nothing.  Products and
     sums are fp32.  ``weights`` fp32, fp16 or bf16 [N, k]."""
-    if torch.is_grad_enabled() and (feats.requires_grad or weights.requires_grad):
-        return _Combine.apply(feats, weights, rows.inverse, rows.offsets)
-    return backend.expert_combine_cuda(feats, weights, rows.inverse, rows.offsets)
+    return _ops.expert_combine(feats, weights, rows.inverse, rows.offsets)

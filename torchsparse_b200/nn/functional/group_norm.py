@@ -1,10 +1,8 @@
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
-from ... import backend
+from ... import _ops
 from ...tensor import SparseTensor
 
 __all__ = ["RowGroups", "group_rows", "sample_rows", "group_norm"]
@@ -21,7 +19,7 @@ class RowGroups(NamedTuple):
 def group_rows(keys: torch.Tensor, num_groups: int) -> RowGroups:
     """Group rows by ``keys`` (int32 or int64 [N]); rows of one group keep their order, a key outside
     [0, num_groups) belongs to no group."""
-    order, _, offsets = backend.group_rows_cuda(keys, num_groups)
+    order, _, offsets = _ops.group_rows(keys, num_groups, False)
     return RowGroups(order, offsets)
 
 
@@ -34,25 +32,15 @@ def sample_rows(input: SparseTensor, batch_size: Optional[int] = None) -> RowGro
     return group_rows(batch, max(int(batch_size), 1))
 
 
-class _GroupNorm(Function):
-    """Group norm with an activation (torchsparse/nn/modules/norm.py:25-57) and its gradient."""
+_ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "leaky_relu": 2, "silu": 3}
 
-    @staticmethod
-    def forward(ctx, feats, weight, bias, offsets, order, num_groups, eps, activation, negative_slope):
-        y, stats = backend.group_norm_forward_cuda(feats, order, offsets, num_groups, weight, bias, eps, activation,
-                                                   negative_slope)
-        ctx.save_for_backward(feats, weight, bias, offsets, order, stats)
-        ctx.args = num_groups, activation, negative_slope
-        return y
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_output: torch.Tensor):
-        feats, weight, bias, offsets, order, stats = ctx.saved_tensors
-        num_groups, activation, negative_slope = ctx.args
-        dx, dweight, dbias = backend.group_norm_backward_cuda(feats, grad_output, order, offsets, num_groups, weight, bias,
-                                                              stats, activation, negative_slope)
-        return dx, dweight, dbias, None, None, None, None, None, None
+def activation_code(activation: Optional[str]) -> int:
+    """The library's number of an activation that a norm can be fused with."""
+    try:
+        return _ACTIVATIONS[activation]
+    except KeyError:
+        raise ValueError(f"unknown activation {activation!r}: one of {sorted(k for k in _ACTIVATIONS if k)}") from None
 
 
 def group_norm(feats: torch.Tensor, offsets: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] = None,
@@ -65,8 +53,4 @@ def group_norm(feats: torch.Tensor, offsets: torch.Tensor, num_groups: int, weig
     rows of no sample become zero.  A group with one value becomes ``act(bias)``.  ``weight`` and ``bias`` [C] may have a
     dtype of their own (fp32 beside 16-bit features).  ``activation``: None, "relu", "leaky_relu" or "silu".
     Statistics and sums are fp32 and run in a fixed order."""
-    if torch.is_grad_enabled() and (feats.requires_grad or (weight is not None and weight.requires_grad)
-                                    or (bias is not None and bias.requires_grad)):
-        return _GroupNorm.apply(feats, weight, bias, offsets, order, num_groups, eps, activation, negative_slope)
-    return backend.group_norm_forward_cuda(feats, order, offsets, num_groups, weight, bias, eps, activation, negative_slope,
-                                           want_stats=False)[0]
+    return _ops.group_norm(feats, weight, bias, offsets, order, num_groups, eps, activation_code(activation), negative_slope)

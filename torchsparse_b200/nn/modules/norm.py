@@ -3,9 +3,9 @@ from typing import Optional
 import torch
 from torch import nn
 
-from ... import backend
 from ...tensor import SparseTensor
 from .. import functional as F
+from ..functional.group_norm import activation_code
 from ..utils import fapply
 
 __all__ = ["BatchNorm", "GroupNorm", "InstanceNorm"]
@@ -37,8 +37,7 @@ class GroupNorm(nn.GroupNorm):
     def __init__(self, num_groups: int, num_channels: int, eps: float = 1e-5, affine: bool = True, device=None, dtype=None,
                  *, activation: Optional[str] = None, negative_slope: float = 0.01) -> None:
         super().__init__(num_groups, num_channels, eps, affine, device, dtype)
-        if activation not in backend.ACTIVATIONS:
-            raise ValueError(f"unknown activation {activation!r}")
+        activation_code(activation)      # refuses an unknown one
         self.activation, self.negative_slope = activation, negative_slope
 
     def forward(self, input: SparseTensor, rows: Optional[F.RowGroups] = None) -> SparseTensor:
