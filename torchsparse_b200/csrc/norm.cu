@@ -12,7 +12,6 @@
 //
 // Variances are joined from means and sums of squares about them, piece by piece, never as a difference of two large
 // sums, in 32 bits.
-#include <atomic>
 #include <type_traits>
 
 #include "rows.cuh"
@@ -1025,23 +1024,6 @@ int small_threads(int64_t n, int64_t b, int dv) {
   return (int)(want < 128 ? 128 : want > kSmallThreads ? kSmallThreads : want);
 }
 
-// launches a kernel with BYTES of dynamic shared memory, which its device has to be told of once
-template <auto KERNEL, int BYTES, typename... Q>
-int launch_piped(dim3 grid, cudaStream_t st, Q... args) {
-  if (BYTES > 0) {
-    static std::atomic<bool> told[64];
-    int dev = 0;
-    TSB_CUDA_TRY(cudaGetDevice(&dev));
-    if (dev >= 64 || !told[dev].load(std::memory_order_acquire)) {
-      TSB_CUDA_TRY(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES));
-      if (dev < 64) told[dev].store(true, std::memory_order_release);
-    }
-  }
-  KERNEL<<<grid, kNormThreads, BYTES, st>>>(args...);
-  TSB_LAUNCH_CHECK();
-  return TSB_OK;
-}
-
 template <typename F>
 int dispatch_small(int dtype, int vec, bool ordered, F&& f) {
   return dispatch_pack(dtype, vec, [&](auto tag) -> int { return ordered ? f(tag, std::true_type()) : f(tag, std::false_type()); });
@@ -1117,7 +1099,7 @@ int tsb_group_norm_fwd(const void* x, const int32_t* order, const int32_t* offse
     constexpr int VEC = decltype(tag)::VEC, A = decltype(each)::value;
     constexpr bool ORDERED = decltype(ordered)::value;
     if (n && b) {
-      const int rc = launch_piped<norm_stats_kernel<T, VEC, A, ORDERED>, pipe_bytes<T, VEC>(1, 4)>(grid, st, a, (const T*)x, slots);
+      const int rc = launch_wide<norm_stats_kernel<T, VEC, A, ORDERED>, pipe_bytes<T, VEC>(1, 4)>(grid, kNormThreads, st, a, (const T*)x, slots);
       if (rc != TSB_OK) return rc;
     }
     if (b) {
@@ -1125,7 +1107,7 @@ int tsb_group_norm_fwd(const void* x, const int32_t* order, const int32_t* offse
       TSB_LAUNCH_CHECK();
     }
     if (n) {
-      const int rc = launch_piped<norm_apply_kernel<T, VEC, A, ORDERED>, pipe_bytes<T, VEC>(1, 4)>(grid, st, a, (const T*)x, mean,
+      const int rc = launch_wide<norm_apply_kernel<T, VEC, A, ORDERED>, pipe_bytes<T, VEC>(1, 4)>(grid, kNormThreads, st, a, (const T*)x, mean,
                                                             rstd, (T*)y);
       if (rc != TSB_OK) return rc;
     }
@@ -1180,7 +1162,7 @@ int tsb_group_norm_bwd(const void* x, const void* dy, const int32_t* order, cons
     constexpr int VEC = decltype(tag)::VEC, A = decltype(each)::value;
     constexpr bool ORDERED = decltype(ordered)::value;
     if (n && b) {
-      const int rc = launch_piped<norm_grad_sums_kernel<T, VEC, A, ORDERED>, pipe_bytes<T, VEC>(2, 2)>(grid, st, a, (const T*)x,
+      const int rc = launch_wide<norm_grad_sums_kernel<T, VEC, A, ORDERED>, pipe_bytes<T, VEC>(2, 2)>(grid, kNormThreads, st, a, (const T*)x,
                                                             (const T*)dy, mean, rstd, slots);
       if (rc != TSB_OK) return rc;
     }
@@ -1189,7 +1171,7 @@ int tsb_group_norm_bwd(const void* x, const void* dy, const int32_t* order, cons
       TSB_LAUNCH_CHECK();
     }
     if (n) {
-      const int rc = launch_piped<norm_grad_apply_kernel<T, VEC, A, ORDERED>, pipe_bytes<T, VEC>(2, 2)>(grid, st, a, (const T*)x,
+      const int rc = launch_wide<norm_grad_apply_kernel<T, VEC, A, ORDERED>, pipe_bytes<T, VEC>(2, 2)>(grid, kNormThreads, st, a, (const T*)x,
                                                             (const T*)dy, mean, rstd, by_group, (T*)dx);
       if (rc != TSB_OK) return rc;
     }

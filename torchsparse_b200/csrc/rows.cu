@@ -23,6 +23,7 @@ namespace {
 // keys keep their order; sums over the warps of a tile and over the tiles make the ranks global.
 constexpr int kItems = 8;                        // keys of a thread
 constexpr int kMaxDigits = 512;
+static_assert(32 * kItems * sizeof(uint2) == kMaxDigits * sizeof(unsigned), "a warp's pairs and its masks share memory");
 constexpr int kSortThreads = 256;                // of a tile of the sort of many keys
 constexpr int kSortTile = kSortThreads * kItems;
 constexpr int kClusterThreads = 1024;            // of a block of the sort of few keys, at most
@@ -45,24 +46,39 @@ __device__ __forceinline__ unsigned read_key(const KeySource& s, int64_t i) {
 
 // Ranks of the keys of a tile among equal digits of the same warp; whist[w][d] ends as the exclusive sum over the
 // warps before w and total[d] as the tile's count.  Item `it` of lane l is key w * 256 + it * 32 + l of the tile.
+// Which lanes of a warp have the same digit is found by setting their bits in a word per digit (masks, kMaxDigits words
+// per warp; the same memory may serve scatter_tile): for 8192 keys in a block __match_any_sync took 12000 cycles, one
+// vote per bit 9000, this 3600.
 __device__ __forceinline__ void rank_tile(const unsigned (&digit)[kItems], const bool (&on)[kItems], unsigned (&rank)[kItems],
-                                          unsigned short (*whist)[kMaxDigits], unsigned* total, int n_digits) {
+                                          unsigned short (*whist)[kMaxDigits], unsigned* masks, unsigned* total, int n_digits) {
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  for (int d = lane; d < n_digits; d += 32) whist[w][d] = 0;
+  unsigned* mask = masks + w * kMaxDigits;
+  for (int d = lane; d < n_digits; d += 32) {
+    whist[w][d] = 0;
+    mask[d] = 0;
+  }
   __syncwarp();
 #pragma unroll
   for (int it = 0; it < kItems; ++it) {
-    const unsigned d = on[it] ? digit[it] : (unsigned)kMaxDigits;      // keys beyond the end match only one another
-    const unsigned same = __match_any_sync(0xffffffffu, d);
-    const unsigned before = on[it] ? whist[w][d] : 0u;
+    if (on[it]) atomicOr(mask + digit[it], 1u << lane);
+    __syncwarp();
+    unsigned same = 0, before = 0;
+    if (on[it]) {
+      same = mask[digit[it]];
+      before = whist[w][digit[it]];
+    }
     rank[it] = before + __popc(same & ((1u << lane) - 1));
     __syncwarp();
-    if (on[it] && lane == __ffs(same) - 1) whist[w][d] = (unsigned short)(before + __popc(same));
+    if (on[it] && lane == __ffs(same) - 1) {
+      whist[w][digit[it]] = (unsigned short)(before + __popc(same));
+      mask[digit[it]] = 0;
+    }
     __syncwarp();
   }
   __syncthreads();
   for (int d = threadIdx.x; d < n_digits; d += blockDim.x) {
     unsigned sum = 0;
+#pragma unroll 8
     for (int i = 0; i < warps; ++i) {
       const unsigned v = whist[i][d];
       whist[i][d] = (unsigned short)sum;
@@ -73,28 +89,55 @@ __device__ __forceinline__ void rank_tile(const unsigned (&digit)[kItems], const
   __syncthreads();
 }
 
-// in place: v[0..n) -> exclusive sums, by the whole block; wsum: one word per warp
-__device__ __forceinline__ void scan_digits(unsigned* v, int n, unsigned* wsum) {
+// In place: v[0..n) -> exclusive sums, by the whole block.  A word holds two 32-bit sums that are scanned at once.
+// wsum: 33 words.
+__device__ __forceinline__ void scan_digits(unsigned long long* v, int n, unsigned long long* wsum) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  unsigned carry = 0;
-  for (int d0 = 0; d0 < n; d0 += blockDim.x) {
-    const int d = d0 + threadIdx.x;
-    const unsigned own = d < n ? v[d] : 0u;
-    unsigned inc = own;
+  const auto inclusive = [&](unsigned long long x) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const unsigned up = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += up;
+      const unsigned long long up = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += up;
     }
+    return x;
+  };
+  unsigned long long carry = 0;
+  for (int d0 = 0; d0 < n; d0 += blockDim.x) {
+    const int d = d0 + threadIdx.x;
+    const unsigned long long own = d < n ? v[d] : 0ull, inc = inclusive(own);
     if (lane == 31) wsum[w] = inc;
     __syncthreads();
-    unsigned before = carry;
-    for (int i = 0; i < warps; ++i) {
-      if (i < w) before += wsum[i];
-      carry += wsum[i];
+    if (w == 0) {
+      const unsigned long long x = lane < warps ? wsum[lane] : 0ull, sum = inclusive(x);
+      wsum[lane] = sum - x;
+      if (lane == 31) wsum[32] = sum;
     }
-    if (d < n) v[d] = before + inc - own;
     __syncthreads();
+    if (d < n) v[d] = carry + wsum[w] + inc - own;
+    carry += wsum[32];
+    __syncthreads();
+  }
+}
+
+// The keys of a tile leave it in the order of their digits: neighbours then go to neighbouring places, in runs instead of
+// one by one.  both[d]: place of digit d in the tile (high) and, all tiles before it and `before[d]` keys of earlier tiles
+// added, in the sorted rows (low).  put(position, key, row).
+template <typename Put>
+__device__ __forceinline__ void scatter_tile(const unsigned (&key)[kItems], const unsigned (&row)[kItems], const bool (&on)[kItems],
+                                             const unsigned (&digit)[kItems], const unsigned (&rank)[kItems],
+                                             const unsigned short (*whist)[kMaxDigits], unsigned long long* both,
+                                             const unsigned* before, uint2* local, int count, int shift, int n_digits, Put&& put) {
+  const int w = threadIdx.x >> 5;
+#pragma unroll
+  for (int it = 0; it < kItems; ++it)
+    if (on[it]) local[(unsigned)(both[digit[it]] >> 32) + whist[w][digit[it]] + rank[it]] = make_uint2(key[it], row[it]);
+  __syncthreads();
+#pragma unroll 4
+  for (int t = threadIdx.x; t < count; t += blockDim.x) {
+    const uint2 v = local[t];
+    const unsigned d = (v.x >> shift) & (n_digits - 1);
+    const unsigned long long b = both[d];
+    put((unsigned)b + before[d] + (unsigned)t - (unsigned)(b >> 32), v.x, v.y);
   }
 }
 
@@ -109,68 +152,72 @@ struct SortOut {
 // stay in registers, the counts and the sorted pairs cross through the blocks' shared memory, the last pass writes the
 // result.
 size_t cluster_smem(int threads) {
-  return (size_t)threads * kItems * 8 + (2 * kMaxDigits + 32) * sizeof(unsigned) + (size_t)(threads / 32) * kMaxDigits * 2;
+  return (size_t)threads * kItems * 16 + (kMaxDigits + 33) * 8 + 2 * kMaxDigits * 4 + (size_t)(threads / 32) * kMaxDigits * 2;
 }
 
 __global__ void __launch_bounds__(kClusterThreads) sort_cluster_kernel(KeySource src, int n, int passes, int bits, SortOut out) {
   extern __shared__ __align__(16) unsigned char smem[];
   const int tile = blockDim.x * kItems;
   uint2* pairs = reinterpret_cast<uint2*>(smem);
-  unsigned* total = reinterpret_cast<unsigned*>(pairs + tile);
-  unsigned* start = total + kMaxDigits;
-  unsigned* wsum = start + kMaxDigits;
-  auto whist = reinterpret_cast<unsigned short(*)[kMaxDigits]>(wsum + 32);
+  uint2* local = pairs + tile;
+  unsigned long long* both = reinterpret_cast<unsigned long long*>(local + tile);
+  unsigned long long* wsum = both + kMaxDigits;
+  unsigned* total = reinterpret_cast<unsigned*>(wsum + 33);
+  unsigned* before = total + kMaxDigits;
+  auto whist = reinterpret_cast<unsigned short(*)[kMaxDigits]>(before + kMaxDigits);
   cg::cluster_group cluster = cg::this_cluster();
   const int w = threadIdx.x >> 5, blocks = (int)gridDim.x;
-  const int local = w * 32 * kItems + (threadIdx.x & 31), base = (int)blockIdx.x * tile + local;
+  const int at = w * 32 * kItems + (threadIdx.x & 31), base = (int)blockIdx.x * tile, count = min(tile, n - base);
   const unsigned per = 0xffffffffu / (unsigned)tile + 1;      // pos / tile = pos * per >> 32 for pos, tile <= 65536
   unsigned key[kItems], row[kItems], digit[kItems], rank[kItems];
   bool on[kItems];
 #pragma unroll
   for (int it = 0; it < kItems; ++it) {
-    row[it] = (unsigned)(base + it * 32);
-    on[it] = (int)row[it] < n;
+    row[it] = (unsigned)(base + at + it * 32);
+    on[it] = at + it * 32 < count;
     key[it] = on[it] ? read_key(src, row[it]) : 0u;
   }
   const int n_digits = 1 << bits;
   for (int p = 0; p < passes; ++p) {
 #pragma unroll
     for (int it = 0; it < kItems; ++it) digit[it] = (key[it] >> (p * bits)) & (n_digits - 1);
-    rank_tile(digit, on, rank, whist, total, n_digits);
+    rank_tile(digit, on, rank, whist, reinterpret_cast<unsigned*>(local), total, n_digits);
     if (blocks > 1) cluster.sync();      // every block's counts are there
     for (int d = threadIdx.x; d < n_digits; d += blockDim.x) {
       unsigned sum = 0, mine = 0;
-      for (int q = 0; q < blocks; ++q) {
+#pragma unroll
+      for (int q = 0; q < kClusterBlocks; ++q) {
+        if (q >= blocks) break;
         if (q == (int)blockIdx.x) mine = sum;      // what earlier blocks have of this digit
         sum += *cluster.map_shared_rank(total + d, q);
       }
-      start[d] = sum;
-      for (int i = 0; i < (int)(blockDim.x >> 5); ++i) whist[i][d] += (unsigned short)mine;      // below 65536: fewer than n
+      both[d] = (unsigned long long)total[d] << 32 | sum;
+      before[d] = mine;
     }
     __syncthreads();
-    scan_digits(start, n_digits, wsum);
+    scan_digits(both, n_digits, wsum);
     if (out.offsets && blockIdx.x == 0)
-      for (int d = threadIdx.x; d <= (int)src.n_groups; d += blockDim.x) out.offsets[d] = (int)start[d];
-    const bool end = p + 1 == passes;
-#pragma unroll
-    for (int it = 0; it < kItems; ++it) {
-      if (!on[it]) continue;
-      const unsigned pos = start[digit[it]] + whist[w][digit[it]] + rank[it];
-      if (end) {
-        out.order[pos] = (int)row[it];
-        if (out.inverse) out.inverse[row[it]] = (int)pos;
-        if (out.keys) out.keys[pos] = key[it];
-      } else {
-        const unsigned to = __umulhi(pos, per);
-        cluster.map_shared_rank(pairs, (int)to)[pos - to * tile] = make_uint2(key[it], row[it]);
-      }
+      for (int d = threadIdx.x; d <= (int)src.n_groups; d += blockDim.x) out.offsets[d] = (int)(unsigned)both[d];
+    if (p + 1 == passes) {
+      scatter_tile(key, row, on, digit, rank, whist, both, before, local, count, p * bits, n_digits,
+                   [&](unsigned pos, unsigned k, unsigned r) {
+                     out.order[pos] = (int)r;
+                     if (out.inverse) out.inverse[r] = (int)pos;
+                     if (out.keys) out.keys[pos] = k;
+                   });
+      if (blocks > 1) cluster.sync();      // no block reads this one's counts any more
+      break;
     }
-    if (blocks > 1) cluster.sync(); else __syncthreads();      // the pairs are there, and no block reads counts any more
-    if (end) break;
+    scatter_tile(key, row, on, digit, rank, whist, both, before, local, count, p * bits, n_digits,
+                 [&](unsigned pos, unsigned k, unsigned r) {
+                   const unsigned to = __umulhi(pos, per);
+                   cluster.map_shared_rank(pairs, (int)to)[pos - to * tile] = make_uint2(k, r);
+                 });
+    if (blocks > 1) cluster.sync(); else __syncthreads();      // the pairs are there
 #pragma unroll
     for (int it = 0; it < kItems; ++it) {
       if (!on[it]) continue;
-      const uint2 v = pairs[local + it * 32];
+      const uint2 v = pairs[at + it * 32];
       key[it] = v.x;
       row[it] = v.y;
     }
@@ -196,14 +243,14 @@ __device__ __forceinline__ void load_tile(const PassIn& in, int64_t n, unsigned 
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(PassIn in, int64_t n, int shift, int bits, int64_t tiles,
                                                                   unsigned* __restrict__ counts) {
   __shared__ unsigned short whist[kSortThreads / 32][kMaxDigits];
-  __shared__ unsigned total[kMaxDigits];
+  __shared__ unsigned total[kMaxDigits], masks[kSortThreads / 32 * kMaxDigits];
   const int64_t first = (int64_t)blockIdx.x * kSortTile + (threadIdx.x >> 5) * 32 * kItems + (threadIdx.x & 31);
   unsigned key[kItems], digit[kItems], rank[kItems];
   bool on[kItems];
   load_tile(in, n, key, on, first);
 #pragma unroll
   for (int it = 0; it < kItems; ++it) digit[it] = (key[it] >> shift) & ((1u << bits) - 1);
-  rank_tile(digit, on, rank, whist, total, 1 << bits);
+  rank_tile(digit, on, rank, whist, masks, total, 1 << bits);
   for (int d = threadIdx.x; d < (1 << bits); d += kSortThreads) counts[d * tiles + blockIdx.x] = total[d];
 }
 
@@ -239,32 +286,35 @@ __global__ void __launch_bounds__(256) sort_scan_kernel(unsigned* __restrict__ c
 __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(PassIn in, int64_t n, int shift, int bits, int64_t tiles,
                                                                     const unsigned* __restrict__ counts, SortOut out) {
   __shared__ unsigned short whist[kSortThreads / 32][kMaxDigits];
-  __shared__ unsigned total[kMaxDigits];
-  __shared__ unsigned start[kMaxDigits];
-  __shared__ unsigned wsum[kSortThreads / 32];
-  const int w = threadIdx.x >> 5;
-  const int64_t first = (int64_t)blockIdx.x * kSortTile + w * 32 * kItems + (threadIdx.x & 31);
-  unsigned key[kItems], digit[kItems], rank[kItems];
+  __shared__ unsigned total[kMaxDigits], before[kMaxDigits];
+  __shared__ unsigned long long both[kMaxDigits], wsum[33];
+  __shared__ uint2 local[kSortTile];
+  const int at = (threadIdx.x >> 5) * 32 * kItems + (threadIdx.x & 31), n_digits = 1 << bits;
+  const int64_t base = (int64_t)blockIdx.x * kSortTile;
+  unsigned key[kItems], row[kItems], digit[kItems], rank[kItems];
   bool on[kItems];
-  load_tile(in, n, key, on, first);
-  for (int d = threadIdx.x; d < (1 << bits); d += kSortThreads) start[d] = counts[(int64_t)(1 << bits) * tiles + d];
-#pragma unroll
-  for (int it = 0; it < kItems; ++it) digit[it] = (key[it] >> shift) & ((1u << bits) - 1);
-  rank_tile(digit, on, rank, whist, total, 1 << bits);      // its barriers also publish start[]
-  scan_digits(start, 1 << bits, wsum);
-  if (out.offsets && blockIdx.x == 0)
-    for (int d = threadIdx.x; d <= (int)in.src.n_groups; d += kSortThreads) out.offsets[d] = (int)start[d];
+  load_tile(in, n, key, on, base + at);
 #pragma unroll
   for (int it = 0; it < kItems; ++it) {
-    if (!on[it]) continue;
-    const unsigned d = digit[it];
-    const int64_t pos = (int64_t)start[d] + counts[d * tiles + blockIdx.x] + whist[w][d] + rank[it];
-    const int64_t i = first + it * 32;
-    const int row = in.keys ? __ldg(in.rows + i) : (int)i;
-    out.order[pos] = row;
-    if (out.keys) out.keys[pos] = key[it];
-    if (out.inverse) out.inverse[row] = (int)pos;
+    const int64_t i = base + at + it * 32;
+    row[it] = !on[it] ? 0u : in.keys ? (unsigned)__ldg(in.rows + i) : (unsigned)i;
+    digit[it] = (key[it] >> shift) & (n_digits - 1);
   }
+  rank_tile(digit, on, rank, whist, reinterpret_cast<unsigned*>(local), total, n_digits);
+  for (int d = threadIdx.x; d < n_digits; d += kSortThreads) {
+    both[d] = (unsigned long long)total[d] << 32 | counts[(int64_t)n_digits * tiles + d];
+    before[d] = counts[d * tiles + blockIdx.x];
+  }
+  __syncthreads();
+  scan_digits(both, n_digits, wsum);
+  if (out.offsets && blockIdx.x == 0)
+    for (int d = threadIdx.x; d <= (int)in.src.n_groups; d += kSortThreads) out.offsets[d] = (int)(unsigned)both[d];
+  scatter_tile(key, row, on, digit, rank, whist, both, before, local, (int)min((int64_t)kSortTile, n - base), shift, n_digits,
+               [&](unsigned pos, unsigned k, unsigned r) {
+                 out.order[pos] = (int)r;
+                 if (out.keys) out.keys[pos] = k;
+                 if (out.inverse) out.inverse[r] = (int)pos;
+               });
 }
 
 __device__ __forceinline__ int64_t lower_bound(const unsigned* __restrict__ keys, int64_t n, unsigned g) {
@@ -371,17 +421,20 @@ int run_sort(const KeySource& src, int64_t n, SortOut out, void* workspace, cuda
 
 // ------------------------------------------------------------------------------------------------ embedding
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;      // vectors of a thread in the row copies: 64 bytes in flight for each
+// y[i] = scale * table[token[i]], zeros where the token is no row of the table: a thread has U vectors of the result, and the
+// blocks follow one another.  (A grid that stays and reads the tokens of its next vectors ahead took 27 us where this
+// takes 20, for 500009 x 64 bf16: waiting blocks are replaced sooner than waiting loops go round.)
+template <typename T, int VEC>
+constexpr int kTokenVectors = VEC * sizeof(T) >= 8 ? 4 : 8;
 
-// y[i] = scale * table[token[i]], zeros where the token is no row of the table.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads) embed_kernel(const T* __restrict__ table, KeySource src, int64_t total, RowSplit split,
                                                          float scale, T* __restrict__ out) {
-  const int64_t t0 = blockIdx.x * (int64_t)(kThreads * kUnroll) + threadIdx.x;
-  const int64_t c = (int64_t)split.cols * VEC;
-  Pack<T, VEC> v[kUnroll];
+  constexpr int U = kTokenVectors<T, VEC>;
+  const int64_t t0 = blockIdx.x * (int64_t)(kThreads * U) + threadIdx.x, c = (int64_t)split.cols * VEC;
+  Pack<T, VEC> v[U];
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
+  for (int u = 0; u < U; ++u) {
     const int64_t t = t0 + u * kThreads;
     v[u].clear();
     if (t < total) {
@@ -391,7 +444,7 @@ __global__ void __launch_bounds__(kThreads) embed_kernel(const T* __restrict__ t
     }
   }
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
+  for (int u = 0; u < U; ++u) {
     const int64_t t = t0 + u * kThreads;
     if (t >= total) break;
     float f[VEC];
@@ -424,6 +477,10 @@ struct EmbedGrad {
   float* tail;
 };
 
+constexpr int kGradRows = 4, kGradAhead = 2;      // rows of a batch, batches on their way
+template <typename T, int VEC>
+constexpr int kGradBytes = VEC * sizeof(T) == 16 ? (kGradAhead + 1) * kGradRows * kThreads * 16 : 0;
+
 template <typename T, int VEC>
 __device__ __forceinline__ void write_row(const EmbedGrad& a, float (&acc)[VEC], T* __restrict__ to) {
   Pack<T, VEC> o;
@@ -434,8 +491,9 @@ __device__ __forceinline__ void write_row(const EmbedGrad& a, float (&acc)[VEC],
 }
 
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads, 4) embed_grad_kernel(EmbedGrad a, const T* __restrict__ grad, T* __restrict__ dtable,
+__global__ void __launch_bounds__(kThreads, kGradBytes<T, VEC> > 0 ? 3 : 4) embed_grad_kernel(EmbedGrad a, const T* __restrict__ grad, T* __restrict__ dtable,
                                                               int zero_rows) {
+  extern __shared__ __align__(16) unsigned char pipe[];
   __shared__ float s_head[VEC][kThreads], s_tail[VEC][kThreads];
   __shared__ unsigned char s_flags[kThreads];      // of a worker: 1 = it has a tail, 2 = its head goes on behind it
   const int first = blockIdx.y * a.tile, width = min(a.tile, (int)(a.c / VEC) - first);
@@ -473,35 +531,86 @@ __global__ void __launch_bounds__(kThreads, 4) embed_grad_kernel(EmbedGrad a, co
     cur = __ldg(a.keys + p0);
     bool goes_on = cur != none && p0 > 0 && __ldg(a.keys + p0 - 1) == cur;      // the run began in an earlier worker
     has_head = goes_on;
-    constexpr int U = 4;
-    for (int64_t p = p0; p < p1 && cur != none; p += U) {
-      Pack<T, VEC> v[U];
-      unsigned key[U];
+    const auto take = [&](unsigned key, const Pack<T, VEC>& v) {
+      if (cur == none) return;
+      if (key != cur) {      // the run of `cur` ended inside this worker
+        if (goes_on) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        key[u] = p + u < p1 ? __ldg(a.keys + p + u) : none;
-        if (key[u] != none) v[u].load(grad + (int64_t)__ldg(a.order + p + u) * a.c + j);
+          for (int e = 0; e < VEC; ++e) s_head[e][threadIdx.x] = acc[e];
+        } else {
+          write_row(a, acc, dtable + (int64_t)cur * a.c + j);
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+        cur = key;
+        goes_on = false;
+        if (cur == none) return;
+      }
+      float g[VEC];
+      v.get(g);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) acc[e] += g[e];
+    };
+    const int count = (int)(p1 - p0);
+    const unsigned* keys = a.keys + p0;
+    const int* order = a.order + p0;
+    if constexpr (kGradBytes<T, VEC> > 0) {
+      // Rows come through shared memory by cp.async, kGradAhead batches ahead, in slots of this thread's own; the rows'
+      // numbers are read one batch before they are needed, the keys one batch before they are compared.
+      constexpr int U = kGradRows, D = kGradAhead + 1;
+      unsigned char* mine = pipe + threadIdx.x * 16;
+      const auto slot = [&](int stage, int u) { return mine + (stage * U + u) * kThreads * 16; };
+      int row[U];
+      unsigned key[U], next[U];
+      const auto rows_of = [&](int k) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) row[u] = k + u < count ? __ldg(order + k + u) : -1;
+      };
+      const auto issue = [&](int stage) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (row[u] >= 0) async_copy(slot(stage, u), grad + (int64_t)row[u] * a.c + j);
+        async_commit();
+      };
+      rows_of(0);
+#pragma unroll
+      for (int d = 0; d < kGradAhead; ++d) {
+        issue(d);
+        rows_of((d + 1) * U);
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (p + u >= p1 || cur == none) continue;
-        if (key[u] != cur) {      // the run of `cur` ended inside this worker
-          if (goes_on) {
+      for (int u = 0; u < U; ++u) key[u] = u < count ? __ldg(keys + u) : none;
+      int stage = 0;
+      for (int k = 0; k < count && cur != none; k += U) {
+        issue(stage == 0 ? D - 1 : stage - 1);
+        rows_of(k + D * U);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) s_head[e][threadIdx.x] = acc[e];
-          } else {
-            write_row(a, acc, dtable + (int64_t)cur * a.c + j);
-          }
+        for (int u = 0; u < U; ++u) next[u] = k + U + u < count ? __ldg(keys + k + U + u) : none;
+        async_wait<kGradAhead>();
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
-          cur = key[u];
-          goes_on = false;
-          if (cur == none) continue;
+        for (int u = 0; u < U; ++u) {
+          Pack<T, VEC> v;
+          v.raw = *reinterpret_cast<const typename Pack<T, VEC>::Raw*>(slot(stage, u));
+          if (k + u < count) take(key[u], v);
         }
-        float g[VEC];
-        v[u].get(g);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[e] += g[e];
+        for (int u = 0; u < U; ++u) key[u] = next[u];
+        stage = stage + 1 == D ? 0 : stage + 1;
+      }
+      async_wait<0>();
+    } else {
+      constexpr int U = 8;
+      for (int k = 0; k < count && cur != none; k += U) {
+        Pack<T, VEC> v[U];
+        unsigned key[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          key[u] = k + u < count ? __ldg(keys + k + u) : none;
+          if (key[u] != none) v[u].load(grad + (int64_t)__ldg(order + k + u) * a.c + j);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (k + u < count) take(key[u], v[u]);
       }
     }
     if (cur != none) {
@@ -602,7 +711,7 @@ __global__ void __launch_bounds__(kJoinThreads) embed_join_kernel(EmbedGrad a, T
   }
 }
 
-EmbedGrad embed_plan(int64_t n, int64_t n_rows, int64_t c, int vec) {
+EmbedGrad embed_plan(int64_t n, int64_t n_rows, int64_t c, int vec, int size) {
   EmbedGrad a{};
   a.n = n;
   a.n_rows = n_rows;
@@ -610,8 +719,8 @@ EmbedGrad embed_plan(int64_t n, int64_t n_rows, int64_t c, int vec) {
   const int64_t vecs = c / vec;
   a.tile = (int)cdiv(vecs, cdiv(vecs, kThreads));
   a.per_block = kThreads / a.tile;
-  // one wave of four blocks an SM where that leaves workers of 8 to 64 positions
-  int64_t len = cdiv(n, cdiv(4 * kSmCount, cdiv(vecs, a.tile)) * a.per_block);
+  // one wave of resident blocks where that leaves workers of 8 to 64 positions
+  int64_t len = cdiv(n, cdiv((vec * size == 16 ? 3 : 4) * kSmCount, cdiv(vecs, a.tile)) * a.per_block);
   len = len < 8 ? 8 : len > 64 ? 64 : len;
   a.len = (int)len;
   a.span = len * a.per_block;
@@ -822,11 +931,12 @@ int tsb_embedding_fwd(const void* table, const void* tokens, int32_t tokens_are_
   if (n == 0) return TSB_OK;
   const KeySource src{tokens, 1, tokens_are_i64, (unsigned)n_rows, -1};
   const int vec = vector_width(dtype, c, (uintptr_t)table | (uintptr_t)out);
-  const int64_t total = n * (c / vec), blocks = cdiv(total, kThreads * kUnroll);
-  if (blocks > 0x7fffffff) return TSB_ERR_LIMIT;
+  const int64_t total = n * (c / vec);
   return dispatch_pack(dtype, vec, [&](auto tag) -> int {
     using T = typename decltype(tag)::T;
     constexpr int VEC = decltype(tag)::VEC;
+    const int64_t blocks = cdiv(total, kThreads * kTokenVectors<T, VEC>);
+    if (blocks > 0x7fffffff) return TSB_ERR_LIMIT;
     embed_kernel<T, VEC><<<(unsigned)blocks, kThreads, 0, as_stream(stream)>>>((const T*)table, src, total, row_split(c / VEC), scale,
                                                                                (T*)out);
     TSB_LAUNCH_CHECK();
@@ -839,7 +949,7 @@ size_t tsb_embedding_bwd_workspace_bytes(int64_t n, int64_t n_rows, int64_t c, i
   size_t partials = 0;      // of the vector width that leaves the most
   for (int vec = 1; vec <= 16 / (int)dtype_size(dtype); vec *= 2) {
     if (c % vec) continue;
-    const size_t b = align_up((size_t)embed_plan(n, n_rows, c, vec).blocks * c * sizeof(float), 256);
+    const size_t b = align_up((size_t)embed_plan(n, n_rows, c, vec, (int)dtype_size(dtype)).blocks * c * sizeof(float), 256);
     if (b > partials) partials = b;
   }
   return sort_plan(n, n_rows).bytes + 2 * align_up((size_t)n * 4, 256) + 2 * partials;
@@ -859,7 +969,7 @@ int tsb_embedding_bwd(const void* grad, const void* tokens, int32_t tokens_are_i
   }
   if (!workspace || workspace_bytes < tsb_embedding_bwd_workspace_bytes(n, n_rows, c, dtype)) return TSB_ERR_WORKSPACE;
   const int vec = vector_width(dtype, c, (uintptr_t)grad | (uintptr_t)dtable);
-  EmbedGrad a = embed_plan(n, n_rows, c, vec);
+  EmbedGrad a = embed_plan(n, n_rows, c, vec, (int)dtype_size(dtype));
   const int zero_rows = c >= 256 ? 64 : 256;      // rows that a block looks up and clears
   const int64_t blocks = a.blocks + cdiv(n_rows, zero_rows);
   if (blocks > 0x7fffffff) return TSB_ERR_LIMIT;
@@ -874,14 +984,15 @@ int tsb_embedding_bwd(const void* grad, const void* tokens, int32_t tokens_are_i
   a.head = reinterpret_cast<float*>(ws);
   a.tail = reinterpret_cast<float*>(ws + align_up((size_t)a.blocks * c * sizeof(float), 256));
   const KeySource src{tokens, 1, tokens_are_i64, (unsigned)n_rows, padding_row};
-  const int rc = run_sort(src, n, SortOut{order, nullptr, keys, nullptr}, workspace, st);
-  if (rc != TSB_OK) return rc;
+  const int sorted = run_sort(src, n, SortOut{order, nullptr, keys, nullptr}, workspace, st);
+  if (sorted != TSB_OK) return sorted;
   return dispatch_pack(dtype, vec, [&](auto tag) -> int {
     using T = typename decltype(tag)::T;
     constexpr int VEC = decltype(tag)::VEC;
     const dim3 grid((unsigned)blocks, (unsigned)cdiv(c / VEC, a.tile));
-    embed_grad_kernel<T, VEC><<<grid, kThreads, 0, st>>>(a, (const T*)grad, (T*)dtable, zero_rows);
-    TSB_LAUNCH_CHECK();
+    const int rc = launch_wide<embed_grad_kernel<T, VEC>, kGradBytes<T, VEC>>(grid, kThreads, st, a, (const T*)grad, (T*)dtable,
+                                                                             zero_rows);
+    if (rc != TSB_OK) return rc;
     if (a.blocks > 1) {
       const dim3 join((unsigned)(a.blocks - 1), (unsigned)cdiv(c, 256));
       if (c % 4 == 0) embed_join_kernel<T, 4><<<join, kJoinThreads, 0, st>>>(a, (T*)dtable);

@@ -2,6 +2,8 @@
 // activations and the parameter loads whose type is only known at run time.
 #pragma once
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace tsb {
@@ -107,6 +109,33 @@ __device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float v
   if (dtype == TSB_F32) reinterpret_cast<float*>(p)[i] = v;
   else if (dtype == TSB_F16) reinterpret_cast<__half*>(p)[i] = from_f32<__half>(v);
   else reinterpret_cast<__nv_bfloat16*>(p)[i] = from_f32<__nv_bfloat16>(v);
+}
+
+// launches a kernel with BYTES of dynamic shared memory, which its device has to be told of once
+template <auto KERNEL, int BYTES, typename... Q>
+inline int launch_wide(dim3 grid, int threads, cudaStream_t st, Q... args) {
+  if (BYTES > 0) {
+    static std::atomic<bool> told[64];
+    int dev = 0;
+    TSB_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev >= 64 || !told[dev].load(std::memory_order_acquire)) {
+      TSB_CUDA_TRY(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES));
+      if (dev < 64) told[dev].store(true, std::memory_order_release);
+    }
+  }
+  KERNEL<<<grid, threads, BYTES, st>>>(args...);
+  TSB_LAUNCH_CHECK();
+  return TSB_OK;
+}
+
+// 16 bytes into shared memory without passing through registers; commit closes a group, wait<N> leaves the N newest open
+__device__ __forceinline__ void async_copy(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 }  // namespace tsb
