@@ -460,8 +460,8 @@ def check_experts(choice, e, c, dtype, w_dtype=torch.float32, seed=0, shift=lamb
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("n,k,e", [(1, 1, 1), (1, 8, 256), (16, 2, 8), (1500, 6, 130), (4097, 1, 3), (700, 3, 70000)])
-@pytest.mark.parametrize("c", [8, 99, 1024])
+@pytest.mark.parametrize("n,k,e", [(1, 1, 1), (1, 8, 256), (16, 2, 8), (1500, 6, 130), (4097, 1, 3), (700, 3, 70000), (90, 13, 40)])
+@pytest.mark.parametrize("c", [8, 99, 200, 1024, 2600])
 def test_experts_there_and_back(dtype, n, k, e, c):
     choice = torch.randint(-1, e + 1, (n, k), generator=torch.Generator(device="cuda").manual_seed(n + e), device="cuda")
     check_experts(choice, e, c, dtype)

@@ -630,14 +630,44 @@ __global__ void __launch_bounds__(kJoinThreads) norm_grad_join_kernel(Norm a, co
   }
 }
 
+// dw and db of the 32 channels of this block: their sums over the samples, in order
+__device__ __forceinline__ void sum_params(const Norm& a, const float2* __restrict__ by_channel, void* __restrict__ dw,
+                                           void* __restrict__ db, float2* part) {
+  const int k = blockIdx.x * 32 + (threadIdx.x & 31), lane = threadIdx.x >> 5;      // 32 channels x 8 slices of the samples
+  float u = 0.f, v = 0.f;
+  if (k < a.c)
+    for (int s = lane; s < a.b; s += kNormWarps) {
+      const float2 f = by_channel[(int64_t)s * a.c + k];
+      u += f.x;
+      v += f.y;
+    }
+  part[threadIdx.x] = make_float2(u, v);
+  __syncthreads();
+  if (lane == 0 && k < a.c) {
+    for (int l = 1; l < kNormWarps; ++l) {
+      u += part[l * 32 + threadIdx.x].x;
+      v += part[l * 32 + threadIdx.x].y;
+    }
+    if (db) store_any(db, a.p_dtype, k, u);
+    if (dw) store_any(dw, a.p_dtype, k, v);
+  }
+}
+
 // dx = rstd * (dz * w - m1 - xhat * m2) = dz * a + (x - mean) * k2 + k1 with k1 = -rstd * m1, k2 = -rstd^2 * m2
 template <typename T, int VEC, int A, bool ORDERED>
 __global__ void __launch_bounds__(kNormThreads, 3) norm_grad_apply_kernel(Norm a, const T* __restrict__ x, const T* __restrict__ dy,
                                                                           const float* __restrict__ mean,
                                                                           const float* __restrict__ rstd,
-                                                                          const float2* __restrict__ by_group, T* __restrict__ dx) {
+                                                                          const float2* __restrict__ by_group,
+                                                                          const float2* __restrict__ by_channel,
+                                                                          T* __restrict__ dx, void* __restrict__ dw,
+                                                                          void* __restrict__ db) {
   constexpr int U = 2, W = VEC / A;
   extern __shared__ __align__(16) unsigned char pipe[];
+  if ((dw || db) && blockIdx.y == 0 && blockIdx.x * 32 < a.c) {      // the first blocks also write the parameters' gradients
+    __shared__ float2 part[kNormThreads];
+    sum_params(a, by_channel, dw, db, part);
+  }
   const int first = blockIdx.y * a.tile, width = min(a.tile, a.cols - first);
   const int lane = threadIdx.x / width, lanes = kNormThreads / width;
   const int k0 = (first + threadIdx.x - lane * width) * VEC;
@@ -684,28 +714,10 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_grad_apply_kernel(Norm a
   }
 }
 
-// dw and db: the channels' sums over the samples, in their order
-__global__ void __launch_bounds__(256) norm_grad_params_kernel(Norm a, const float2* __restrict__ by_channel, void* __restrict__ dw,
-                                                               void* __restrict__ db) {
-  __shared__ float2 part[256];
-  const int k = blockIdx.x * 32 + (threadIdx.x & 31), lane = threadIdx.x >> 5;      // 32 channels x 8 slices of the samples
-  float u = 0.f, v = 0.f;
-  if (k < a.c)
-    for (int s = lane; s < a.b; s += 8) {
-      const float2 f = by_channel[(int64_t)s * a.c + k];
-      u += f.x;
-      v += f.y;
-    }
-  part[threadIdx.x] = make_float2(u, v);
-  __syncthreads();
-  if (lane == 0 && k < a.c) {
-    for (int l = 1; l < 8; ++l) {
-      u += part[l * 32 + threadIdx.x].x;
-      v += part[l * 32 + threadIdx.x].y;
-    }
-    if (db) store_any(db, a.p_dtype, k, u);
-    if (dw) store_any(dw, a.p_dtype, k, v);
-  }
+__global__ void __launch_bounds__(kNormThreads) norm_grad_params_kernel(Norm a, const float2* __restrict__ by_channel,
+                                                                        void* __restrict__ dw, void* __restrict__ db) {
+  __shared__ float2 part[kNormThreads];
+  sum_params(a, by_channel, dw, db, part);
 }
 
 // ------------------------------------------------------------------------------------------------ small samples
@@ -1145,7 +1157,7 @@ int tsb_group_norm_bwd(const void* x, const void* dy, const int32_t* order, cons
           <<<grid, threads, 0, st>>>(a, (const T*)x, (const T*)dy, mean, rstd, by_channel, (T*)dx, dweight, dbias);
       TSB_LAUNCH_CHECK();
       if (b > 1 && (dweight || dbias)) {
-        norm_grad_params_kernel<<<(unsigned)cdiv(a.c, 32), 256, 0, st>>>(a, by_channel, dweight, dbias);
+        norm_grad_params_kernel<<<(unsigned)cdiv(a.c, 32), kNormThreads, 0, st>>>(a, by_channel, dweight, dbias);
         TSB_LAUNCH_CHECK();
       }
       return TSB_OK;
@@ -1157,6 +1169,7 @@ int tsb_group_norm_bwd(const void* x, const void* dy, const int32_t* order, cons
   float2* by_channel = reinterpret_cast<float2*>(ws + channel_bytes(c, kNormBlocks + b));
   float2* by_group = reinterpret_cast<float2*>(ws + channel_bytes(c, kNormBlocks + b) + channel_bytes(c, b));
   const dim3 grid((unsigned)a.nblk, (unsigned)cdiv(a.cols, a.tile));
+  const bool fold = (int64_t)a.nblk * 32 >= c;      // enough blocks for the parameters: no launch of their own
   return dispatch_norm(dtype, vec, a.d, order != nullptr, [&](auto tag, auto each, auto ordered) -> int {
     using T = typename decltype(tag)::T;
     constexpr int VEC = decltype(tag)::VEC, A = decltype(each)::value;
@@ -1172,11 +1185,12 @@ int tsb_group_norm_bwd(const void* x, const void* dy, const int32_t* order, cons
     }
     if (n) {
       const int rc = launch_wide<norm_grad_apply_kernel<T, VEC, A, ORDERED>, pipe_bytes<T, VEC>(2, 2)>(grid, kNormThreads, st, a, (const T*)x,
-                                                            (const T*)dy, mean, rstd, by_group, (T*)dx);
+                                                            (const T*)dy, mean, rstd, by_group, by_channel, (T*)dx,
+                                                            fold ? dweight : nullptr, fold ? dbias : nullptr);
       if (rc != TSB_OK) return rc;
     }
-    if (dweight || dbias) {
-      norm_grad_params_kernel<<<(unsigned)cdiv(a.c, 32), 256, 0, st>>>(a, by_channel, dweight, dbias);
+    if (!fold && (dweight || dbias)) {
+      norm_grad_params_kernel<<<(unsigned)cdiv(a.c, 32), kNormThreads, 0, st>>>(a, by_channel, dweight, dbias);
       TSB_LAUNCH_CHECK();
     }
     return TSB_OK;

@@ -6,13 +6,11 @@
 #include <cooperative_groups.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "rows.cuh"
 
 namespace cg = cooperative_groups;
-#ifndef TSB_GRID
-#define TSB_GRID 8
-#endif
 
 namespace tsb {
 namespace {
@@ -655,10 +653,10 @@ __global__ void __launch_bounds__(kThreads, kGradBytes<T, VEC> > 0 ? 3 : 4) embe
   }
 }
 
-// A block per block of embed_grad_kernel in which a run begins that goes on behind it, and per 256 channels: its tail and
+// A block per block of embed_grad_kernel in which a run begins that goes on behind it, and per 128 JV channels: its tail and
 // the heads of the blocks that follow (those whose first key is the same), threads = channels (JV a thread) x slices of
 // those blocks.
-constexpr int kJoinThreads = 512;
+constexpr int kJoinThreads = 512, kJoinColumns = 128;
 template <typename T, int JV>
 __global__ void __launch_bounds__(kJoinThreads) embed_join_kernel(EmbedGrad a, T* __restrict__ dtable) {
   __shared__ float part[JV][kJoinThreads];
@@ -667,8 +665,8 @@ __global__ void __launch_bounds__(kJoinThreads) embed_join_kernel(EmbedGrad a, T
   const unsigned key = __ldg(a.keys + p1 - 1);
   if (key == (unsigned)a.n_rows || __ldg(a.keys + p1) != key) return;
   if (p0 > 0 && __ldg(a.keys + p0 - 1) == key) return;      // it began before (the keys are sorted)
-  const int64_t j0 = blockIdx.y * 256;
-  const int cols = (int)((min(a.c - j0, (int64_t)256) + JV - 1) / JV), slices = kJoinThreads / cols;
+  const int64_t j0 = (int64_t)blockIdx.y * kJoinColumns * JV;
+  const int cols = (int)min((a.c - j0) / JV, (int64_t)kJoinColumns), slices = kJoinThreads / cols;
   const int slice = threadIdx.x / cols, q = threadIdx.x - slice * cols;
   const int64_t j = j0 + q * JV;
   float s[JV];
@@ -757,133 +755,243 @@ __global__ void __launch_bounds__(kThreads) dispatch_kernel(const T* __restrict_
   }
 }
 
-// The two kernels below give a row (a choice) to a group of `lanes` threads, a power of two up to a warp, and let a grid
-// that fits the machine walk over the rows, with the indices of a group's next row on their way while it reads this one.
+// The two kernels below give a row (a choice) to a group of `lanes` threads and let a grid that fits the machine walk over
+// the rows.  A step is what a thread reads at once: of 16-byte vectors, two steps more are on their way through shared
+// memory by cp.async, in slots of the thread's own, and the indices of the step behind them; narrower vectors are loaded
+// when they are needed, with the next step's indices on their way.  (131072 x 2 of 512 bf16: combined in 79 us with loads
+// into registers, in 64 us so; the gradient in 132 and 104 us.)
+constexpr int kStepAhead = 2, kStepVectors = 4;      // vectors of a thread and step
+constexpr int kRowBlocks = 3 * kSmCount;             // resident: 48 KB of slots each
+template <typename T, int VEC>
+constexpr int kStepBytes = VEC * sizeof(T) == 16 ? (kStepAhead + 1) * kStepVectors * kThreads * 16 : 0;
 
-// out[i] = sum over j of w[i][j] * rows[inverse[i][j]] (w null: 1), in the order of j: KU choices and U vectors of each at once
-template <typename T, int VEC, int KU, int U>
+// out[i] = sum over j of w[i][j] * rows[inverse[i][j]] (w null: 1), in the order of j.  A step: KU choices of a row, U vectors
+// of each.
+template <typename T, int VEC, int KU>
 __global__ void __launch_bounds__(kThreads) combine_kernel(const T* __restrict__ rows, const void* __restrict__ w, int w_dtype,
                                                            const int* __restrict__ inverse, const int* __restrict__ kept,
                                                            int64_t n, int k, int64_t c, int lanes, T* __restrict__ out) {
-  const int cols = (int)(c / VEC), lane = threadIdx.x & (lanes - 1), groups = kThreads / lanes;
+  constexpr int U = kStepVectors / KU;      // 4, 2, 1, 1
+  constexpr bool kAsync = kStepBytes<T, VEC> > 0;
+  constexpr int D = kAsync ? kStepAhead + 1 : 1;
+  extern __shared__ __align__(16) unsigned char pipe[];
+  const int cols = (int)(c / VEC), groups = kThreads / lanes, group = threadIdx.x / lanes, lane = threadIdx.x - group * lanes;
   const int64_t step = (int64_t)gridDim.x * groups;
-  const int n_kept = (int)min((int64_t)__ldg(kept), n * k);
-  int next[KU];
-  const auto fetch = [&](int64_t i, int q0, int (&pos)[KU]) {
-#pragma unroll
-    for (int u = 0; u < KU; ++u) pos[u] = i < n && q0 + u < k ? __ldg(inverse + i * k + q0 + u) : -1;
+  const unsigned n_kept = (unsigned)min((int64_t)__ldg(kept), n * k);
+  struct Place {      // row, first vector, first choice
+    int64_t i;
+    int v, q;
   };
-  int64_t i = blockIdx.x * (int64_t)groups + threadIdx.x / lanes;
-  fetch(i, 0, next);
-  for (; i < n; i += step) {
-    int first[KU];
+  const auto advance = [&](Place& p) {
+    p.q += KU;
+    if (p.q < k) return;
+    p.q = 0;
+    p.v += lanes * U;
+    if (p.v < cols) return;
+    p.v = lane;
+    p.i += step;
+  };
+  // positions (no expert: none) and weights of a step
+  const unsigned none = 0xffffffffu;
+  const auto fetch = [&](const Place& p, unsigned (&pos)[KU], float (&f)[KU]) {
 #pragma unroll
-    for (int u = 0; u < KU; ++u) first[u] = next[u];
-    fetch(i + step, 0, next);
-    for (int v0 = lane; v0 < cols; v0 += lanes * U) {
-      float acc[U][VEC];
+    for (int u = 0; u < KU; ++u) {
+      const bool in = p.i < n && p.q + u < k;
+      pos[u] = in ? (unsigned)__ldg(inverse + p.i * k + p.q + u) : none;
+      f[u] = in && w ? load_any(w, w_dtype, p.i * k + p.q + u) : 1.f;
+    }
+  };
+  const auto slot = [&](int stage, int u, int x) { return pipe + (((stage * KU + u) * U + x) * kThreads + threadIdx.x) * 16; };
+  const auto issue = [&](int stage, const Place& p, const unsigned (&pos)[KU]) {
+#pragma unroll
+    for (int u = 0; u < KU; ++u)
+#pragma unroll
+      for (int x = 0; x < U; ++x)
+        if (pos[u] < n_kept && p.v + x * lanes < cols) async_copy(slot(stage, u, x), rows + (int64_t)pos[u] * c + (p.v + x * lanes) * VEC);
+    async_commit();
+  };
+  Place now{blockIdx.x * (int64_t)groups + group, lane, 0}, ahead = now;
+  if (group >= groups || lane >= cols) now.i = ahead.i = n;      // threads left over
+  unsigned pos[D + 1][KU];      // of the steps from `now` on; the last is on its way
+  float f[D + 1][KU];
+  fetch(ahead, pos[0], f[0]);
+#pragma unroll
+  for (int d = 0; d < D - 1; ++d) {
+    if constexpr (kAsync) issue(d, ahead, pos[d]);
+    advance(ahead);
+    fetch(ahead, pos[d + 1], f[d + 1]);
+  }
+  float acc[U][VEC];
+  int stage = 0;
+  while (now.i < n) {
+    if constexpr (kAsync) issue(stage == 0 ? D - 1 : stage - 1, ahead, pos[D - 1]);
+    advance(ahead);
+    fetch(ahead, pos[D], f[D]);
+    Pack<T, VEC> p[KU][U];
+    if constexpr (kAsync) {
+      async_wait<kStepAhead>();
+    } else {
+#pragma unroll
+      for (int u = 0; u < KU; ++u)
+#pragma unroll
+        for (int x = 0; x < U; ++x)
+          if (pos[0][u] < n_kept && now.v + x * lanes < cols) p[u][x].load(rows + (int64_t)pos[0][u] * c + (now.v + x * lanes) * VEC);
+    }
+    if (now.q == 0) {
 #pragma unroll
       for (int x = 0; x < U; ++x)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) acc[x][e] = 0.f;
-      for (int q0 = 0; q0 < k; q0 += KU) {
-        int pos[KU];
-        if (q0) {
-          fetch(i, q0, pos);
-        } else {
+    }
 #pragma unroll
-          for (int u = 0; u < KU; ++u) pos[u] = first[u];
-        }
-        Pack<T, VEC> p[KU][U];
-#pragma unroll
-        for (int u = 0; u < KU; ++u)
-#pragma unroll
-          for (int x = 0; x < U; ++x)
-            if ((unsigned)pos[u] < (unsigned)n_kept && v0 + x * lanes < cols)
-              p[u][x].load(rows + (int64_t)pos[u] * c + (v0 + x * lanes) * VEC);
-#pragma unroll
-        for (int u = 0; u < KU; ++u) {
-          if ((unsigned)pos[u] >= (unsigned)n_kept) continue;
-          const float f = w ? load_any(w, w_dtype, i * k + q0 + u) : 1.f;
-#pragma unroll
-          for (int x = 0; x < U; ++x) {
-            if (v0 + x * lanes >= cols) continue;
-            float v[VEC];
-            p[u][x].get(v);
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[x][e] = fmaf(f, v[e], acc[x][e]);
-          }
-        }
-      }
+    for (int u = 0; u < KU; ++u) {
+      if (pos[0][u] >= n_kept) continue;
 #pragma unroll
       for (int x = 0; x < U; ++x) {
-        if (v0 + x * lanes >= cols) continue;
-        Pack<T, VEC> o;
-        o.set(acc[x]);
-        o.store(out + i * c + (v0 + x * lanes) * VEC);
+        if (now.v + x * lanes >= cols) continue;
+        if constexpr (kAsync) p[u][x].raw = *reinterpret_cast<const typename Pack<T, VEC>::Raw*>(slot(stage, u, x));
+        float v[VEC];
+        p[u][x].get(v);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) acc[x][e] = fmaf(f[0][u], v[e], acc[x][e]);
       }
     }
+    if (now.q + KU >= k) {
+#pragma unroll
+      for (int x = 0; x < U; ++x) {
+        if (now.v + x * lanes >= cols) continue;
+        Pack<T, VEC> o;
+        o.set(acc[x]);
+        o.store(out + now.i * c + (now.v + x * lanes) * VEC);
+      }
+    }
+    advance(now);
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+#pragma unroll
+      for (int u = 0; u < KU; ++u) {
+        pos[d][u] = pos[d + 1][u];
+        f[d][u] = f[d + 1][u];
+      }
+    stage = stage + 1 == D ? 0 : stage + 1;
   }
+  if constexpr (kAsync) async_wait<0>();
 }
 
-// drows[pos] = w * dout[i] and dw = <dout[i], rows[pos]> of a choice, both zero for a choice of no expert.  Choices of one
-// row share its dout through the L1 cache.
+// drows[pos] = w * dout[i] and dw = <dout[i], rows[pos]> of a choice, both zero for a choice of no expert.  A step: two vectors
+// of both rows; `lanes` is a power of two up to a warp.  Choices of one row share its dout through the caches.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads) combine_grad_kernel(const T* __restrict__ dout, const T* __restrict__ rows,
                                                                 const void* __restrict__ w, int w_dtype,
                                                                 const int* __restrict__ inverse, const int* __restrict__ kept,
                                                                 int64_t pairs, RowSplit by_k, int64_t c, int lanes,
                                                                 T* __restrict__ drows, void* __restrict__ dw) {
-  constexpr int U = 2;
+  constexpr int U = kStepVectors / 2;
+  constexpr bool kAsync = kStepBytes<T, VEC> > 0;
+  constexpr int D = kAsync ? kStepAhead + 1 : 1;
+  extern __shared__ __align__(16) unsigned char pipe[];
   const int cols = (int)(c / VEC), lane = threadIdx.x & (lanes - 1), groups = kThreads / lanes;
   const int64_t step = (int64_t)gridDim.x * groups;
-  const int n_kept = (int)min((int64_t)__ldg(kept), pairs);
-  // whole warps stay together for the sums: q of the warp's first group decides
-  const int64_t ahead = threadIdx.x / lanes - (threadIdx.x / 32) * (32 / lanes);
-  int64_t q0 = blockIdx.x * (int64_t)groups + (threadIdx.x / 32) * (32 / lanes);
-  int next = q0 + ahead < pairs ? __ldg(inverse + q0 + ahead) : -1;
-  float next_w = q0 + ahead < pairs ? load_any(w, w_dtype, q0 + ahead) : 0.f;
-  for (; q0 < pairs; q0 += step) {
-    const int64_t q = q0 + ahead;
-    const int pos = next;
-    const float f = next_w;
-    next = q + step < pairs ? __ldg(inverse + q + step) : -1;
-    next_w = q + step < pairs ? load_any(w, w_dtype, q + step) : 0.f;
-    float dot = 0.f;
-    if ((unsigned)pos < (unsigned)n_kept) {
-      const T *g0 = dout + by_k.row(q) * c, *r0 = rows + (int64_t)pos * c;
-      T* d0 = drows + (int64_t)pos * c;
-      for (int v0 = lane; v0 < cols; v0 += lanes * U) {
-        Pack<T, VEC> g[U], r[U];
+  const unsigned n_kept = (unsigned)min((int64_t)__ldg(kept), pairs);
+  struct Place {      // choice, first vector
+    int64_t q;
+    int v;
+  };
+  const auto advance = [&](Place& p) {
+    p.v += lanes * U;
+    if (p.v - lane < cols) return;      // the same for all threads of a warp, which sum together
+    p.v = lane;
+    p.q += step;
+  };
+  const unsigned none = 0xffffffffu;
+  const auto fetch = [&](const Place& p, unsigned& pos, float& f) {
+    pos = p.q < pairs ? (unsigned)__ldg(inverse + p.q) : none;
+    f = p.q < pairs ? load_any(w, w_dtype, p.q) : 0.f;
+  };
+  const auto slot = [&](int stage, int i, int u) { return pipe + (((stage * 2 + i) * U + u) * kThreads + threadIdx.x) * 16; };
+  const auto issue = [&](int stage, const Place& p, unsigned pos) {
+    if (pos < n_kept) {
+      const T* g = dout + by_k.row(p.q) * c + p.v * VEC;
+      const T* r = rows + (int64_t)pos * c + p.v * VEC;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (p.v + u * lanes >= cols) continue;
+        async_copy(slot(stage, 0, u), r + u * lanes * VEC);
+        async_copy(slot(stage, 1, u), g + u * lanes * VEC);
+      }
+    }
+    async_commit();
+  };
+  const int64_t warp_q = blockIdx.x * (int64_t)groups + (threadIdx.x / 32) * (32 / lanes);      // of the warp's first group
+  const int64_t own = threadIdx.x / lanes - (threadIdx.x / 32) * (32 / lanes);
+  Place now{warp_q + own, lane}, ahead = now;
+  unsigned pos[D + 1];
+  float f[D + 1];
+  fetch(ahead, pos[0], f[0]);
+#pragma unroll
+  for (int d = 0; d < D - 1; ++d) {
+    if constexpr (kAsync) issue(d, ahead, pos[d]);
+    advance(ahead);
+    fetch(ahead, pos[d + 1], f[d + 1]);
+  }
+  float dot = 0.f;
+  int stage = 0;
+  while (now.q - own < pairs) {      // the same for all threads of a warp
+    if constexpr (kAsync) issue(stage == 0 ? D - 1 : stage - 1, ahead, pos[D - 1]);
+    advance(ahead);
+    fetch(ahead, pos[D], f[D]);
+    const bool used = pos[0] < n_kept;
+    T* d0 = drows + (int64_t)pos[0] * c;
+    if constexpr (kAsync) async_wait<kStepAhead>();
+    if (used) {
+      Pack<T, VEC> r[U], g[U];
+      if constexpr (!kAsync) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          if (v0 + u * lanes >= cols) continue;
-          r[u].load(r0 + (v0 + u * lanes) * VEC);
-          g[u].load(g0 + (v0 + u * lanes) * VEC);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (v0 + u * lanes >= cols) continue;
-          float a[VEC], b[VEC];
-          g[u].get(a);
-          r[u].get(b);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            dot = fmaf(a[e], b[e], dot);
-            a[e] *= f;
-          }
-          g[u].set(a);
-          g[u].store(d0 + (v0 + u * lanes) * VEC);
+          if (now.v + u * lanes >= cols) continue;
+          r[u].load(rows + (int64_t)pos[0] * c + (now.v + u * lanes) * VEC);
+          g[u].load(dout + by_k.row(now.q) * c + (now.v + u * lanes) * VEC);
         }
       }
-    } else if (pos >= 0 && pos < pairs) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (now.v + u * lanes >= cols) continue;
+        if constexpr (kAsync) {
+          r[u].raw = *reinterpret_cast<const typename Pack<T, VEC>::Raw*>(slot(stage, 0, u));
+          g[u].raw = *reinterpret_cast<const typename Pack<T, VEC>::Raw*>(slot(stage, 1, u));
+        }
+        float a[VEC], b[VEC];
+        g[u].get(a);
+        r[u].get(b);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          dot = fmaf(a[e], b[e], dot);
+          a[e] *= f[0];
+        }
+        g[u].set(a);
+        g[u].store(d0 + (now.v + u * lanes) * VEC);
+      }
+    } else if ((int64_t)pos[0] < pairs) {
       Pack<T, VEC> zero;
       zero.clear();
-      for (int v = lane; v < cols; v += lanes) zero.store(drows + (int64_t)pos * c + v * VEC);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (now.v + u * lanes < cols) zero.store(d0 + (now.v + u * lanes) * VEC);
     }
-    for (int o = lanes >> 1; o > 0; o >>= 1) dot += __shfl_down_sync(0xffffffffu, dot, o, lanes);
-    if (lane == 0 && q < pairs) store_any(dw, w_dtype, q, dot);
+    if (now.v - lane + lanes * U >= cols) {      // the choice's last step
+      for (int o = lanes >> 1; o > 0; o >>= 1) dot += __shfl_down_sync(0xffffffffu, dot, o, lanes);
+      if (lane == 0 && now.q < pairs) store_any(dw, w_dtype, now.q, dot);
+      dot = 0.f;
+    }
+    advance(now);
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      pos[d] = pos[d + 1];
+      f[d] = f[d + 1];
+    }
+    stage = stage + 1 == D ? 0 : stage + 1;
   }
+  if constexpr (kAsync) async_wait<0>();
 }
 
 // threads of a row of `cols` vectors
@@ -994,9 +1102,9 @@ int tsb_embedding_bwd(const void* grad, const void* tokens, int32_t tokens_are_i
                                                                              zero_rows);
     if (rc != TSB_OK) return rc;
     if (a.blocks > 1) {
-      const dim3 join((unsigned)(a.blocks - 1), (unsigned)cdiv(c, 256));
-      if (c % 4 == 0) embed_join_kernel<T, 4><<<join, kJoinThreads, 0, st>>>(a, (T*)dtable);
-      else embed_join_kernel<T, 1><<<join, kJoinThreads, 0, st>>>(a, (T*)dtable);
+      const auto join = [&](int jv) { return dim3((unsigned)(a.blocks - 1), (unsigned)cdiv(c, kJoinColumns * jv)); };
+      if (c % 4 == 0) embed_join_kernel<T, 4><<<join(4), kJoinThreads, 0, st>>>(a, (T*)dtable);
+      else embed_join_kernel<T, 1><<<join(1), kJoinThreads, 0, st>>>(a, (T*)dtable);
       TSB_LAUNCH_CHECK();
     }
     return TSB_OK;
@@ -1029,17 +1137,27 @@ int tsb_expert_combine(const void* rows, const void* weights, int32_t weights_dt
   if (n > kMaxRows / k || c > kMaxChannels) return TSB_ERR_LIMIT;
   if (n == 0) return TSB_OK;
   const int vec = vector_width(dtype, c, (uintptr_t)rows | (uintptr_t)out);
-  const int lanes = row_lanes(c / vec);
-  const int grid = grid_for(n * lanes, kThreads, TSB_GRID);
+  // choices of a step: as few steps as four at once need, evenly filled; threads of a row: as many as its vectors need
+  const int ku = (int)cdiv(k, cdiv(k, kStepVectors)), u = kStepVectors / ku;
+  const int64_t vecs = c / vec;
+  const int lanes = (int)cdiv(vecs, u * cdiv(vecs, kThreads * u));
+  const int64_t want = cdiv(n, kThreads / lanes);
   return dispatch_pack(dtype, vec, [&](auto tag) -> int {
     using T = typename decltype(tag)::T;
-    constexpr int VEC = decltype(tag)::VEC;
-    const auto run = [&](auto kernel) {
-      kernel<<<grid, kThreads, 0, as_stream(stream)>>>((const T*)rows, weights, weights_dtype, inverse, kept, n, k, c, lanes, (T*)out);
+    constexpr int VEC = decltype(tag)::VEC, BYTES = kStepBytes<T, VEC>;
+    const int64_t most = BYTES > 0 ? kRowBlocks : 8 * kSmCount;
+    const dim3 grid((unsigned)(want < most ? want : most));
+    const auto run = [&](auto choices) -> int {
+      return launch_wide<combine_kernel<T, VEC, decltype(choices)::value>, BYTES>(grid, kThreads, as_stream(stream), (const T*)rows,
+                                                                                 weights, weights_dtype, inverse, kept, n, k, c, lanes,
+                                                                                 (T*)out);
     };
-    if (k <= 2) run(combine_kernel<T, VEC, 2, 2>); else run(combine_kernel<T, VEC, 4, 1>);
-    TSB_LAUNCH_CHECK();
-    return TSB_OK;
+    switch (ku) {
+      case 1: return run(std::integral_constant<int, 1>());
+      case 2: return run(std::integral_constant<int, 2>());
+      case 3: return run(std::integral_constant<int, 3>());
+      default: return run(std::integral_constant<int, 4>());
+    }
   });
 }
 
@@ -1053,14 +1171,14 @@ int tsb_expert_combine_bwd(const void* dout, const void* rows, const void* weigh
   if (n == 0) return TSB_OK;
   const int vec = vector_width(dtype, c, (uintptr_t)dout | (uintptr_t)rows | (uintptr_t)drows);
   const int lanes = row_lanes(c / vec);
-  const int grid = grid_for(n * k * lanes, kThreads, TSB_GRID);
+  const int64_t want = cdiv(n * k * lanes, kThreads);
   return dispatch_pack(dtype, vec, [&](auto tag) -> int {
     using T = typename decltype(tag)::T;
-    constexpr int VEC = decltype(tag)::VEC;
-    combine_grad_kernel<T, VEC><<<grid, kThreads, 0, as_stream(stream)>>>(
-        (const T*)dout, (const T*)rows, weights, weights_dtype, inverse, kept, n * k, row_split(k), c, lanes, (T*)drows, dweights);
-    TSB_LAUNCH_CHECK();
-    return TSB_OK;
+    constexpr int VEC = decltype(tag)::VEC, BYTES = kStepBytes<T, VEC>;
+    const int64_t most = BYTES > 0 ? kRowBlocks : 8 * kSmCount;
+    return launch_wide<combine_grad_kernel<T, VEC>, BYTES>(dim3((unsigned)(want < most ? want : most)), kThreads, as_stream(stream),
+                                                           (const T*)dout, (const T*)rows, weights, weights_dtype, inverse, kept,
+                                                           n * k, row_split(k), c, lanes, (T*)drows, dweights);
   });
 }
 
