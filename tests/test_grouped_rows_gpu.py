@@ -386,6 +386,10 @@ def test_embedding_unaligned_strided_and_empty_tables():
         table = torch.randn(50, 24, generator=g, device="cuda").to(dtype)
         tokens = torch.randint(0, 50, (999, 2), generator=g, device="cuda")
         check_embedding(tokens[:, 1], unaligned(table), 2.0)
+        for c in (1, 2, 3, 5, 7, 12):                            # rows shorter than a vector of the result
+            narrow = torch.randn(50, c, generator=g, device="cuda").to(dtype)
+            for n in (1, 2, 3, 999):
+                check_embedding(tokens[:n, 1] - 3, narrow, 2.0)
         check_embedding(tokens[:, 0], table.t().contiguous().t(), 2.0)
     empty = torch.empty(0, 24, device="cuda", requires_grad=True)
     y = F.embedding(torch.zeros(5, dtype=torch.int64, device="cuda"), empty)

@@ -72,14 +72,14 @@ __device__ __forceinline__ int64_t row_at(const Norm& a, int64_t p) {
 // The `count` rows p, p + step, .. of a thread, U at a time: f(v, at, full) with v[i][u] the vector of array i in row u and
 // at[u] the row's offset, which is -1 for a row that is not there unless `full` says that all are.
 //
-// Vectors of 16 bytes come through shared memory by cp.async, each thread filling and reading slots of its own: three
+// Vectors of 4 bytes and more come through shared memory by cp.async, each thread filling and reading slots of its own: three
 // batches are on their way without holding registers, nothing waits for another thread, and the order and the borders of
-// the samples do not matter.  Narrower vectors are loaded directly.
+// the samples do not matter.  Single 16-bit values are loaded directly.
 constexpr int kPipeDepth = 3;
 template <typename T, int VEC>
-constexpr bool kPiped = VEC * sizeof(T) == 16;
+constexpr int kBatch = VEC * sizeof(T) == 16 ? 4 : 8;      // vectors of a batch, of one array or two
 template <typename T, int VEC>
-constexpr int pipe_bytes(int arrays, int u) { return kPiped<T, VEC> ? kPipeDepth * arrays * u * kNormThreads * 16 : 0; }
+constexpr int kPipeBytes = kAsyncVector<T, VEC> ? kPipeDepth * kBatch<T, VEC> * kNormThreads * VEC * (int)sizeof(T) : 0;
 
 template <typename T, int VEC, int ARRAYS, int U, bool ORDERED, typename F>
 __device__ __forceinline__ void for_rows(const Norm& a, const T* const (&src)[ARRAYS], int64_t p, int step, int count,
@@ -94,16 +94,12 @@ __device__ __forceinline__ void for_rows(const Norm& a, const T* const (&src)[AR
     }
     return base + u * pitch;
   };
-  if constexpr (kPiped<T, VEC>) {
-    constexpr int kStage = ARRAYS * U * kNormThreads * 16;
-    const unsigned char* mine = pipe + threadIdx.x * 16;
-    const unsigned to0 = (unsigned)__cvta_generic_to_shared(mine);
+  if constexpr (kAsyncVector<T, VEC>) {
+    constexpr int kBytes = Pack<T, VEC>::kBytes, kStage = ARRAYS * U * kNormThreads * kBytes;
+    unsigned char* mine = pipe + threadIdx.x * kBytes;
     const auto copy = [&](int stage, int u, int64_t at) {
 #pragma unroll
-      for (int i = 0; i < ARRAYS; ++i)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to0 + stage * kStage + (u * ARRAYS + i) * kNormThreads * 16),
-                     "l"(src[i] + at)
-                     : "memory");
+      for (int i = 0; i < ARRAYS; ++i) async_copy<kBytes>(mine + stage * kStage + (u * ARRAYS + i) * kNormThreads * kBytes, src[i] + at);
     };
     const auto issue = [&](int stage, int k, int64_t base) {
       if (!ORDERED && k + U <= count) {
@@ -116,7 +112,7 @@ __device__ __forceinline__ void for_rows(const Norm& a, const T* const (&src)[AR
           if (at >= 0) copy(stage, u, at);
         }
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");      // an empty group where nothing was left to read
+      async_commit();      // an empty group where nothing was left to read
     };
     constexpr int kAhead = (kPipeDepth - 1) * U;
 #pragma unroll
@@ -124,14 +120,14 @@ __device__ __forceinline__ void for_rows(const Norm& a, const T* const (&src)[AR
     int stage = 0;
     for (int k = 0; k < count; k += U, off += U * pitch) {
       issue(stage == 0 ? kPipeDepth - 1 : stage - 1, k + kAhead, off + kAhead * pitch);
-      asm volatile("cp.async.wait_group %0;" ::"n"(kPipeDepth - 1) : "memory");
+      async_wait<kPipeDepth - 1>();
       Pack<T, VEC> v[ARRAYS][U];
       int64_t at[U];
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int i = 0; i < ARRAYS; ++i)
-          v[i][u].raw = *reinterpret_cast<const uint4*>(mine + stage * kStage + (u * ARRAYS + i) * kNormThreads * 16);
+          v[i][u].raw = *reinterpret_cast<const typename Pack<T, VEC>::Raw*>(mine + stage * kStage + (u * ARRAYS + i) * kNormThreads * kBytes);
       if (!ORDERED && k + U <= count) {
 #pragma unroll
         for (int u = 0; u < U; ++u) at[u] = off + u * pitch;
@@ -143,7 +139,7 @@ __device__ __forceinline__ void for_rows(const Norm& a, const T* const (&src)[AR
       }
       stage = stage + 1 == kPipeDepth ? 0 : stage + 1;
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
+    async_wait<0>();
   } else {
     for (int k = 0; k < count; k += U, off += U * pitch) {
       Pack<T, VEC> v[ARRAYS][U];
@@ -333,13 +329,13 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_stats_kernel(Norm a, con
     const int64_t lo = max(p0, begin), hi = min(p1, offset_of(a, s + 1));
     if (lo >= hi) continue;
     if (lane < lanes) {
-      constexpr int U = 4;
+      constexpr int U = kBatch<T, VEC>;
       Running<VEC, A> run;
       run.clear();
       const T* const src[1] = {xc};
       const int count = (int)lane_rows(hi - lo, lanes, lane);
       int left = count;
-      for_rows<T, VEC, 1, U, ORDERED>(a, src, lo + lane, lanes, count, pipe, [&](Pack<T, VEC> (&v)[1][U], const int64_t (&at)[U], auto) {
+      for_rows<T, VEC, 1, U, ORDERED>(a, src, lo + lane, lanes, count, pipe, [&](auto& v, const auto& at, auto) {
         if constexpr (ORDERED) {
 #pragma unroll
           for (int u = 0; u < U; ++u)
@@ -481,7 +477,7 @@ __device__ __forceinline__ void clear_outside(const Norm& a, int64_t p0, int64_t
 template <typename T, int VEC, int A, bool ORDERED>
 __global__ void __launch_bounds__(kNormThreads, 3) norm_apply_kernel(Norm a, const T* __restrict__ x, const float* __restrict__ mean,
                                                                      const float* __restrict__ rstd, T* __restrict__ y) {
-  constexpr int U = 4, W = VEC / A;
+  constexpr int U = kBatch<T, VEC>, W = VEC / A;
   extern __shared__ __align__(16) unsigned char pipe[];
   const int first = blockIdx.y * a.tile, width = min(a.tile, a.cols - first);
   const int lane = threadIdx.x / width, lanes = kNormThreads / width;
@@ -501,7 +497,7 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_apply_kernel(Norm a, con
     ch.load(a, s, k0, mean, rstd);
     const T* const src[1] = {xc};
     for_rows<T, VEC, 1, U, ORDERED>(a, src, hi - 1 - lane, -lanes, (int)lane_rows(hi - lo, lanes, lane), pipe,
-                                    [&](Pack<T, VEC> (&v)[1][U], const int64_t (&at)[U], auto full) {
+                                    [&](auto& v, const auto& at, auto full) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (!decltype(full)::value && at[u] < 0) continue;
@@ -523,7 +519,7 @@ template <typename T, int VEC, int A, bool ORDERED>
 __global__ void __launch_bounds__(kNormThreads, 3) norm_grad_sums_kernel(Norm a, const T* __restrict__ x, const T* __restrict__ dy,
                                                                          const float* __restrict__ mean,
                                                                          const float* __restrict__ rstd, float2* __restrict__ slots) {
-  constexpr int U = 2, W = VEC / A;
+  constexpr int U = kBatch<T, VEC> / 2, W = VEC / A;
   extern __shared__ __align__(16) unsigned char pipe[];
   __shared__ float2 part[VEC * kNormThreads];
   const int first = blockIdx.y * a.tile, width = min(a.tile, a.cols - first);
@@ -544,7 +540,7 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_grad_sums_kernel(Norm a,
       ch.load(a, s, k0, mean, rstd);
       const T* const src[2] = {xc, gc};
       for_rows<T, VEC, 2, U, ORDERED>(a, src, lo + lane, lanes, (int)lane_rows(hi - lo, lanes, lane), pipe,
-                                      [&](Pack<T, VEC> (&v)[2][U], const int64_t (&at)[U], auto full) {
+                                      [&](auto& v, const auto& at, auto full) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           if (!decltype(full)::value && at[u] < 0) continue;
@@ -662,7 +658,7 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_grad_apply_kernel(Norm a
                                                                           const float2* __restrict__ by_channel,
                                                                           T* __restrict__ dx, void* __restrict__ dw,
                                                                           void* __restrict__ db) {
-  constexpr int U = 2, W = VEC / A;
+  constexpr int U = kBatch<T, VEC> / 2, W = VEC / A;
   extern __shared__ __align__(16) unsigned char pipe[];
   if ((dw || db) && blockIdx.y == 0 && blockIdx.x * 32 < a.c) {      // the first blocks also write the parameters' gradients
     __shared__ float2 part[kNormThreads];
@@ -695,7 +691,7 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_grad_apply_kernel(Norm a
     }
     const T* const src[2] = {xc, gc};
     for_rows<T, VEC, 2, U, ORDERED>(a, src, hi - 1 - lane, -lanes, (int)lane_rows(hi - lo, lanes, lane), pipe,
-                                    [&](Pack<T, VEC> (&v)[2][U], const int64_t (&at)[U], auto full) {
+                                    [&](auto& v, const auto& at, auto full) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (!decltype(full)::value && at[u] < 0) continue;
@@ -1111,7 +1107,8 @@ int tsb_group_norm_fwd(const void* x, const int32_t* order, const int32_t* offse
     constexpr int VEC = decltype(tag)::VEC, A = decltype(each)::value;
     constexpr bool ORDERED = decltype(ordered)::value;
     if (n && b) {
-      const int rc = launch_wide<norm_stats_kernel<T, VEC, A, ORDERED>, pipe_bytes<T, VEC>(1, 4)>(grid, kNormThreads, st, a, (const T*)x, slots);
+      const int rc = launch_wide<norm_stats_kernel<T, VEC, A, ORDERED>, kPipeBytes<T, VEC>>(grid, kNormThreads, st, a, (const T*)x,
+                                                                                              slots);
       if (rc != TSB_OK) return rc;
     }
     if (b) {
@@ -1119,7 +1116,7 @@ int tsb_group_norm_fwd(const void* x, const int32_t* order, const int32_t* offse
       TSB_LAUNCH_CHECK();
     }
     if (n) {
-      const int rc = launch_wide<norm_apply_kernel<T, VEC, A, ORDERED>, pipe_bytes<T, VEC>(1, 4)>(grid, kNormThreads, st, a, (const T*)x, mean,
+      const int rc = launch_wide<norm_apply_kernel<T, VEC, A, ORDERED>, kPipeBytes<T, VEC>>(grid, kNormThreads, st, a, (const T*)x, mean,
                                                             rstd, (T*)y);
       if (rc != TSB_OK) return rc;
     }
@@ -1175,7 +1172,7 @@ int tsb_group_norm_bwd(const void* x, const void* dy, const int32_t* order, cons
     constexpr int VEC = decltype(tag)::VEC, A = decltype(each)::value;
     constexpr bool ORDERED = decltype(ordered)::value;
     if (n && b) {
-      const int rc = launch_wide<norm_grad_sums_kernel<T, VEC, A, ORDERED>, pipe_bytes<T, VEC>(2, 2)>(grid, kNormThreads, st, a, (const T*)x,
+      const int rc = launch_wide<norm_grad_sums_kernel<T, VEC, A, ORDERED>, kPipeBytes<T, VEC>>(grid, kNormThreads, st, a, (const T*)x,
                                                             (const T*)dy, mean, rstd, slots);
       if (rc != TSB_OK) return rc;
     }
@@ -1184,7 +1181,7 @@ int tsb_group_norm_bwd(const void* x, const void* dy, const int32_t* order, cons
       TSB_LAUNCH_CHECK();
     }
     if (n) {
-      const int rc = launch_wide<norm_grad_apply_kernel<T, VEC, A, ORDERED>, pipe_bytes<T, VEC>(2, 2)>(grid, kNormThreads, st, a, (const T*)x,
+      const int rc = launch_wide<norm_grad_apply_kernel<T, VEC, A, ORDERED>, kPipeBytes<T, VEC>>(grid, kNormThreads, st, a, (const T*)x,
                                                             (const T*)dy, mean, rstd, by_group, by_channel, (T*)dx,
                                                             fold ? dweight : nullptr, fold ? dbias : nullptr);
       if (rc != TSB_OK) return rc;

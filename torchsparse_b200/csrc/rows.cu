@@ -422,35 +422,57 @@ constexpr int kThreads = 256;
 // y[i] = scale * table[token[i]], zeros where the token is no row of the table: a thread has U vectors of the result, and the
 // blocks follow one another.  (A grid that stays and reads the tokens of its next vectors ahead took 27 us where this
 // takes 20, for 500009 x 64 bf16: waiting blocks are replaced sooner than waiting loops go round.)
-template <typename T, int VEC>
-constexpr int kTokenVectors = VEC * sizeof(T) >= 8 ? 4 : 8;
-
-template <typename T, int VEC>
+//
+// A vector of the result (16 bytes wherever its rows lie, the result being one run of memory) is made of PARTS loads of VEC
+// values, as wide as the rows of the table allow: a part lies in one row, a vector may lie in two or more.
+template <typename T, int VEC, int PARTS>
 __global__ void __launch_bounds__(kThreads) embed_kernel(const T* __restrict__ table, KeySource src, int64_t total, RowSplit split,
                                                          float scale, T* __restrict__ out) {
-  constexpr int U = kTokenVectors<T, VEC>;
+  constexpr int U = PARTS > 4 ? 2 : 4;
   const int64_t t0 = blockIdx.x * (int64_t)(kThreads * U) + threadIdx.x, c = (int64_t)split.cols * VEC;
-  Pack<T, VEC> v[U];
+  Pack<T, VEC> v[U][PARTS];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int64_t t = t0 + u * kThreads;
-    v[u].clear();
-    if (t < total) {
-      const int64_t i = split.row(t);
-      const unsigned row = read_key(src, i);
-      if (row < src.n_groups) v[u].load(table + (int64_t)row * c + (t - i * split.cols) * VEC);
+    int64_t t = (t0 + u * kThreads) * PARTS, i = split.row(t);      // total and t count parts
+    unsigned col = (unsigned)(t - i * split.cols), row = t < total ? read_key(src, i) : src.n_groups;
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q) {
+      v[u][q].clear();
+      if (row < src.n_groups) v[u][q].load(table + (int64_t)row * c + (int64_t)col * VEC);
+      ++t;
+      if (q + 1 < PARTS && ++col == split.cols) {
+        col = 0;
+        ++i;
+        row = src.n_groups;
+        if (t < total) row = read_key(src, i);
+      }
+      if (t >= total) row = src.n_groups;
     }
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int64_t t = t0 + u * kThreads;
+    const int64_t t = (t0 + u * kThreads) * PARTS;
     if (t >= total) break;
-    float f[VEC];
-    v[u].get(f);
+    Pack<T, VEC * PARTS> o;
+    float f[VEC * PARTS];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) f[e] *= scale;
-    v[u].set(f);
-    v[u].store(out + t * VEC);
+    for (int q = 0; q < PARTS; ++q) {
+      float g[VEC];
+      v[u][q].get(g);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) f[q * VEC + e] = g[e] * scale;
+    }
+    o.set(f);
+    if (PARTS == 1 || t + PARTS <= total) {
+      o.store(out + t * VEC);
+    } else {      // the end of the result
+#pragma unroll
+      for (int q = 0; q < PARTS; ++q) {
+        if (t + q >= total) break;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) out[(t + q) * VEC + e] = from_f32<T>(f[q * VEC + e]);
+      }
+    }
   }
 }
 
@@ -475,9 +497,11 @@ struct EmbedGrad {
   float* tail;
 };
 
-constexpr int kGradRows = 4, kGradAhead = 2;      // rows of a batch, batches on their way
+constexpr int kGradAhead = 2;      // batches on their way
 template <typename T, int VEC>
-constexpr int kGradBytes = VEC * sizeof(T) == 16 ? (kGradAhead + 1) * kGradRows * kThreads * 16 : 0;
+constexpr int kGradRows = VEC * sizeof(T) == 16 ? 4 : 8;      // rows of a batch
+template <typename T, int VEC>
+constexpr int kGradBytes = kAsyncVector<T, VEC> ? (kGradAhead + 1) * kGradRows<T, VEC> * kThreads * VEC * (int)sizeof(T) : 0;
 
 template <typename T, int VEC>
 __device__ __forceinline__ void write_row(const EmbedGrad& a, float (&acc)[VEC], T* __restrict__ to) {
@@ -489,7 +513,7 @@ __device__ __forceinline__ void write_row(const EmbedGrad& a, float (&acc)[VEC],
 }
 
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kThreads, kGradBytes<T, VEC> > 0 ? 3 : 4) embed_grad_kernel(EmbedGrad a, const T* __restrict__ grad, T* __restrict__ dtable,
+__global__ void __launch_bounds__(kThreads, 3) embed_grad_kernel(EmbedGrad a, const T* __restrict__ grad, T* __restrict__ dtable,
                                                               int zero_rows) {
   extern __shared__ __align__(16) unsigned char pipe[];
   __shared__ float s_head[VEC][kThreads], s_tail[VEC][kThreads];
@@ -552,12 +576,13 @@ __global__ void __launch_bounds__(kThreads, kGradBytes<T, VEC> > 0 ? 3 : 4) embe
     const int count = (int)(p1 - p0);
     const unsigned* keys = a.keys + p0;
     const int* order = a.order + p0;
-    if constexpr (kGradBytes<T, VEC> > 0) {
+    constexpr int U = kGradRows<T, VEC>;
+    if constexpr (kAsyncVector<T, VEC>) {
       // Rows come through shared memory by cp.async, kGradAhead batches ahead, in slots of this thread's own; the rows'
       // numbers are read one batch before they are needed, the keys one batch before they are compared.
-      constexpr int U = kGradRows, D = kGradAhead + 1;
-      unsigned char* mine = pipe + threadIdx.x * 16;
-      const auto slot = [&](int stage, int u) { return mine + (stage * U + u) * kThreads * 16; };
+      constexpr int D = kGradAhead + 1, kBytes = Pack<T, VEC>::kBytes;
+      unsigned char* mine = pipe + threadIdx.x * kBytes;
+      const auto slot = [&](int stage, int u) { return mine + (stage * U + u) * kThreads * kBytes; };
       int row[U];
       unsigned key[U], next[U];
       const auto rows_of = [&](int k) {
@@ -567,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, kGradBytes<T, VEC> > 0 ? 3 : 4) embe
       const auto issue = [&](int stage) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (row[u] >= 0) async_copy(slot(stage, u), grad + (int64_t)row[u] * a.c + j);
+          if (row[u] >= 0) async_copy<kBytes>(slot(stage, u), grad + (int64_t)row[u] * a.c + j);
         async_commit();
       };
       rows_of(0);
@@ -597,7 +622,6 @@ __global__ void __launch_bounds__(kThreads, kGradBytes<T, VEC> > 0 ? 3 : 4) embe
       }
       async_wait<0>();
     } else {
-      constexpr int U = 8;
       for (int k = 0; k < count && cur != none; k += U) {
         Pack<T, VEC> v[U];
         unsigned key[U];
@@ -709,7 +733,7 @@ __global__ void __launch_bounds__(kJoinThreads) embed_join_kernel(EmbedGrad a, T
   }
 }
 
-EmbedGrad embed_plan(int64_t n, int64_t n_rows, int64_t c, int vec, int size) {
+EmbedGrad embed_plan(int64_t n, int64_t n_rows, int64_t c, int vec) {
   EmbedGrad a{};
   a.n = n;
   a.n_rows = n_rows;
@@ -718,7 +742,7 @@ EmbedGrad embed_plan(int64_t n, int64_t n_rows, int64_t c, int vec, int size) {
   a.tile = (int)cdiv(vecs, cdiv(vecs, kThreads));
   a.per_block = kThreads / a.tile;
   // one wave of resident blocks where that leaves workers of 8 to 64 positions
-  int64_t len = cdiv(n, cdiv((vec * size == 16 ? 3 : 4) * kSmCount, cdiv(vecs, a.tile)) * a.per_block);
+  int64_t len = cdiv(n, cdiv(3 * kSmCount, cdiv(vecs, a.tile)) * a.per_block);
   len = len < 8 ? 8 : len > 64 ? 64 : len;
   a.len = (int)len;
   a.span = len * a.per_block;
@@ -756,14 +780,14 @@ __global__ void __launch_bounds__(kThreads) dispatch_kernel(const T* __restrict_
 }
 
 // The two kernels below give a row (a choice) to a group of `lanes` threads and let a grid that fits the machine walk over
-// the rows.  A step is what a thread reads at once: of 16-byte vectors, two steps more are on their way through shared
-// memory by cp.async, in slots of the thread's own, and the indices of the step behind them; narrower vectors are loaded
-// when they are needed, with the next step's indices on their way.  (131072 x 2 of 512 bf16: combined in 79 us with loads
+// the rows.  A step is what a thread reads at once: two steps more are on their way through shared memory by cp.async, in slots of the
+// thread's own, and the indices of the step behind them; single 16-bit values are loaded when they are needed, with the
+// next step's indices on their way.  (131072 x 2 of 512 bf16: combined in 79 us with loads
 // into registers, in 64 us so; the gradient in 132 and 104 us.)
-constexpr int kStepAhead = 2, kStepVectors = 4;      // vectors of a thread and step
-constexpr int kRowBlocks = 3 * kSmCount;             // resident: 48 KB of slots each
-template <typename T, int VEC>
-constexpr int kStepBytes = VEC * sizeof(T) == 16 ? (kStepAhead + 1) * kStepVectors * kThreads * 16 : 0;
+constexpr int kStepAhead = 2;
+constexpr int step_vectors(int bytes) { return bytes == 16 ? 4 : 8; }      // of a thread
+constexpr int step_bytes(int bytes) { return bytes >= 4 ? (kStepAhead + 1) * step_vectors(bytes) * kThreads * bytes : 0; }
+constexpr int row_blocks(int bytes) { return (bytes >= 8 ? 3 : 6) * kSmCount; }      // resident: 48 KB of slots each, or 24
 
 // out[i] = sum over j of w[i][j] * rows[inverse[i][j]] (w null: 1), in the order of j.  A step: KU choices of a row, U vectors
 // of each.
@@ -771,8 +795,8 @@ template <typename T, int VEC, int KU>
 __global__ void __launch_bounds__(kThreads) combine_kernel(const T* __restrict__ rows, const void* __restrict__ w, int w_dtype,
                                                            const int* __restrict__ inverse, const int* __restrict__ kept,
                                                            int64_t n, int k, int64_t c, int lanes, T* __restrict__ out) {
-  constexpr int U = kStepVectors / KU;      // 4, 2, 1, 1
-  constexpr bool kAsync = kStepBytes<T, VEC> > 0;
+  constexpr int kBytes = Pack<T, VEC>::kBytes, U = step_vectors(kBytes) / KU;
+  constexpr bool kAsync = kAsyncVector<T, VEC>;
   constexpr int D = kAsync ? kStepAhead + 1 : 1;
   extern __shared__ __align__(16) unsigned char pipe[];
   const int cols = (int)(c / VEC), groups = kThreads / lanes, group = threadIdx.x / lanes, lane = threadIdx.x - group * lanes;
@@ -801,13 +825,13 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const T* __restrict__
       f[u] = in && w ? load_any(w, w_dtype, p.i * k + p.q + u) : 1.f;
     }
   };
-  const auto slot = [&](int stage, int u, int x) { return pipe + (((stage * KU + u) * U + x) * kThreads + threadIdx.x) * 16; };
+  const auto slot = [&](int stage, int u, int x) { return pipe + (((stage * KU + u) * U + x) * kThreads + threadIdx.x) * kBytes; };
   const auto issue = [&](int stage, const Place& p, const unsigned (&pos)[KU]) {
 #pragma unroll
     for (int u = 0; u < KU; ++u)
 #pragma unroll
       for (int x = 0; x < U; ++x)
-        if (pos[u] < n_kept && p.v + x * lanes < cols) async_copy(slot(stage, u, x), rows + (int64_t)pos[u] * c + (p.v + x * lanes) * VEC);
+        if (pos[u] < n_kept && p.v + x * lanes < cols) async_copy<kBytes>(slot(stage, u, x), rows + (int64_t)pos[u] * c + (p.v + x * lanes) * VEC);
     async_commit();
   };
   Place now{blockIdx.x * (int64_t)groups + group, lane, 0}, ahead = now;
@@ -886,8 +910,8 @@ __global__ void __launch_bounds__(kThreads) combine_grad_kernel(const T* __restr
                                                                 const int* __restrict__ inverse, const int* __restrict__ kept,
                                                                 int64_t pairs, RowSplit by_k, int64_t c, int lanes,
                                                                 T* __restrict__ drows, void* __restrict__ dw) {
-  constexpr int U = kStepVectors / 2;
-  constexpr bool kAsync = kStepBytes<T, VEC> > 0;
+  constexpr int kBytes = Pack<T, VEC>::kBytes, U = step_vectors(kBytes) / 2;
+  constexpr bool kAsync = kAsyncVector<T, VEC>;
   constexpr int D = kAsync ? kStepAhead + 1 : 1;
   extern __shared__ __align__(16) unsigned char pipe[];
   const int cols = (int)(c / VEC), lane = threadIdx.x & (lanes - 1), groups = kThreads / lanes;
@@ -908,7 +932,7 @@ __global__ void __launch_bounds__(kThreads) combine_grad_kernel(const T* __restr
     pos = p.q < pairs ? (unsigned)__ldg(inverse + p.q) : none;
     f = p.q < pairs ? load_any(w, w_dtype, p.q) : 0.f;
   };
-  const auto slot = [&](int stage, int i, int u) { return pipe + (((stage * 2 + i) * U + u) * kThreads + threadIdx.x) * 16; };
+  const auto slot = [&](int stage, int i, int u) { return pipe + (((stage * 2 + i) * U + u) * kThreads + threadIdx.x) * kBytes; };
   const auto issue = [&](int stage, const Place& p, unsigned pos) {
     if (pos < n_kept) {
       const T* g = dout + by_k.row(p.q) * c + p.v * VEC;
@@ -916,8 +940,8 @@ __global__ void __launch_bounds__(kThreads) combine_grad_kernel(const T* __restr
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (p.v + u * lanes >= cols) continue;
-        async_copy(slot(stage, 0, u), r + u * lanes * VEC);
-        async_copy(slot(stage, 1, u), g + u * lanes * VEC);
+        async_copy<kBytes>(slot(stage, 0, u), r + u * lanes * VEC);
+        async_copy<kBytes>(slot(stage, 1, u), g + u * lanes * VEC);
       }
     }
     async_commit();
@@ -1038,17 +1062,23 @@ int tsb_embedding_fwd(const void* table, const void* tokens, int32_t tokens_are_
   if (n > kMaxRows || n_rows > kMaxRows || c > kMaxChannels) return TSB_ERR_LIMIT;
   if (n == 0) return TSB_OK;
   const KeySource src{tokens, 1, tokens_are_i64, (unsigned)n_rows, -1};
-  const int vec = vector_width(dtype, c, (uintptr_t)table | (uintptr_t)out);
+  const bool wide = (uintptr_t)out % 16 == 0;
+  const int vec = vector_width(dtype, c, (uintptr_t)table | (wide ? 0 : (uintptr_t)out));
   const int64_t total = n * (c / vec);
   return dispatch_pack(dtype, vec, [&](auto tag) -> int {
     using T = typename decltype(tag)::T;
-    constexpr int VEC = decltype(tag)::VEC;
-    const int64_t blocks = cdiv(total, kThreads * kTokenVectors<T, VEC>);
-    if (blocks > 0x7fffffff) return TSB_ERR_LIMIT;
-    embed_kernel<T, VEC><<<(unsigned)blocks, kThreads, 0, as_stream(stream)>>>((const T*)table, src, total, row_split(c / VEC), scale,
-                                                                               (T*)out);
-    TSB_LAUNCH_CHECK();
-    return TSB_OK;
+    constexpr int VEC = decltype(tag)::VEC, WIDE = 16 / (int)sizeof(T) / VEC;
+    const auto run = [&](auto parts) -> int {
+      constexpr int PARTS = decltype(parts)::value;
+      const int64_t blocks = cdiv(cdiv(total, PARTS), kThreads * (PARTS > 4 ? 2 : 4));
+      if (blocks > 0x7fffffff) return TSB_ERR_LIMIT;
+      embed_kernel<T, VEC, PARTS><<<(unsigned)blocks, kThreads, 0, as_stream(stream)>>>((const T*)table, src, total,
+                                                                                       row_split(c / VEC), scale, (T*)out);
+      TSB_LAUNCH_CHECK();
+      return TSB_OK;
+    };
+    if (wide) return run(std::integral_constant<int, WIDE>());
+    return run(std::integral_constant<int, 1>());
   });
 }
 
@@ -1057,7 +1087,7 @@ size_t tsb_embedding_bwd_workspace_bytes(int64_t n, int64_t n_rows, int64_t c, i
   size_t partials = 0;      // of the vector width that leaves the most
   for (int vec = 1; vec <= 16 / (int)dtype_size(dtype); vec *= 2) {
     if (c % vec) continue;
-    const size_t b = align_up((size_t)embed_plan(n, n_rows, c, vec, (int)dtype_size(dtype)).blocks * c * sizeof(float), 256);
+    const size_t b = align_up((size_t)embed_plan(n, n_rows, c, vec).blocks * c * sizeof(float), 256);
     if (b > partials) partials = b;
   }
   return sort_plan(n, n_rows).bytes + 2 * align_up((size_t)n * 4, 256) + 2 * partials;
@@ -1077,7 +1107,7 @@ int tsb_embedding_bwd(const void* grad, const void* tokens, int32_t tokens_are_i
   }
   if (!workspace || workspace_bytes < tsb_embedding_bwd_workspace_bytes(n, n_rows, c, dtype)) return TSB_ERR_WORKSPACE;
   const int vec = vector_width(dtype, c, (uintptr_t)grad | (uintptr_t)dtable);
-  EmbedGrad a = embed_plan(n, n_rows, c, vec, (int)dtype_size(dtype));
+  EmbedGrad a = embed_plan(n, n_rows, c, vec);
   const int zero_rows = c >= 256 ? 64 : 256;      // rows that a block looks up and clears
   const int64_t blocks = a.blocks + cdiv(n_rows, zero_rows);
   if (blocks > 0x7fffffff) return TSB_ERR_LIMIT;
@@ -1138,14 +1168,14 @@ int tsb_expert_combine(const void* rows, const void* weights, int32_t weights_dt
   if (n == 0) return TSB_OK;
   const int vec = vector_width(dtype, c, (uintptr_t)rows | (uintptr_t)out);
   // choices of a step: as few steps as four at once need, evenly filled; threads of a row: as many as its vectors need
-  const int ku = (int)cdiv(k, cdiv(k, kStepVectors)), u = kStepVectors / ku;
+  const int ku = (int)cdiv(k, cdiv(k, 4)), u = step_vectors(vec * (int)dtype_size(dtype)) / ku;
   const int64_t vecs = c / vec;
   const int lanes = (int)cdiv(vecs, u * cdiv(vecs, kThreads * u));
   const int64_t want = cdiv(n, kThreads / lanes);
   return dispatch_pack(dtype, vec, [&](auto tag) -> int {
     using T = typename decltype(tag)::T;
-    constexpr int VEC = decltype(tag)::VEC, BYTES = kStepBytes<T, VEC>;
-    const int64_t most = BYTES > 0 ? kRowBlocks : 8 * kSmCount;
+    constexpr int VEC = decltype(tag)::VEC, BYTES = step_bytes(Pack<T, VEC>::kBytes);
+    const int64_t most = row_blocks(Pack<T, VEC>::kBytes);
     const dim3 grid((unsigned)(want < most ? want : most));
     const auto run = [&](auto choices) -> int {
       return launch_wide<combine_kernel<T, VEC, decltype(choices)::value>, BYTES>(grid, kThreads, as_stream(stream), (const T*)rows,
@@ -1174,8 +1204,8 @@ int tsb_expert_combine_bwd(const void* dout, const void* rows, const void* weigh
   const int64_t want = cdiv(n * k * lanes, kThreads);
   return dispatch_pack(dtype, vec, [&](auto tag) -> int {
     using T = typename decltype(tag)::T;
-    constexpr int VEC = decltype(tag)::VEC, BYTES = kStepBytes<T, VEC>;
-    const int64_t most = BYTES > 0 ? kRowBlocks : 8 * kSmCount;
+    constexpr int VEC = decltype(tag)::VEC, BYTES = step_bytes(Pack<T, VEC>::kBytes);
+    const int64_t most = row_blocks(Pack<T, VEC>::kBytes);
     return launch_wide<combine_grad_kernel<T, VEC>, BYTES>(dim3((unsigned)(want < most ? want : most)), kThreads, as_stream(stream),
                                                            (const T*)dout, (const T*)rows, weights, weights_dtype, inverse, kept,
                                                            n * k, row_split(k), c, lanes, (T*)drows, dweights);

@@ -33,6 +33,7 @@ struct Pack {
   Raw raw;
   __device__ __forceinline__ void load(const T* p) { raw = __ldg(reinterpret_cast<const Raw*>(p)); }
   __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Raw*>(p) = raw; }
+  static constexpr int kBytes = VEC * (int)sizeof(T);
   __device__ __forceinline__ void clear() { raw = Raw{}; }
   __device__ __forceinline__ void get(float (&v)[VEC]) const {
     const T* e = reinterpret_cast<const T*>(&raw);
@@ -60,6 +61,10 @@ struct PackTag {
   using T = T_;
   static constexpr int VEC = VEC_;
 };
+
+// Vectors that cp.async can move: all but the single 16-bit value.
+template <typename T, int VEC>
+constexpr bool kAsyncVector = VEC * sizeof(T) >= 4;
 
 // f(PackTag<T, VEC>()) for the type and vector width found at run time
 template <typename F>
@@ -128,9 +133,13 @@ inline int launch_wide(dim3 grid, int threads, cudaStream_t st, Q... args) {
   return TSB_OK;
 }
 
-// 16 bytes into shared memory without passing through registers; commit closes a group, wait<N> leaves the N newest open
+// 4, 8 or 16 bytes into shared memory without passing through registers; commit closes a group, wait<N> leaves the N newest
+// open
+template <int BYTES>
 __device__ __forceinline__ void async_copy(void* to, const void* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+  const unsigned at = (unsigned)__cvta_generic_to_shared(to);
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from), "n"(BYTES) : "memory");
 }
 __device__ __forceinline__ void async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
