@@ -651,6 +651,64 @@ def test_calls_on_another_stream_wait_for_nothing_else():
         assert torch.equal(a, b)
 
 
+def test_calls_from_two_threads_at_once():
+    """Each thread on a stream of its own, with inputs of its own."""
+    import threading
+
+    inputs, want, got = [_inputs(s, n=5000 + s) for s in (1, 2)], [], [None, None]
+    want = [_everything(s) for s in inputs]
+    torch.cuda.synchronize()
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got[i] = _everything(inputs[i])
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    for i in (0, 1):
+        for a, b in zip(got[i], want[i]):
+            assert torch.equal(a, b)
+
+
+def test_an_input_changed_before_its_gradient_is_an_error():
+    from torchsparse_b200.nn import functional as F
+
+    off = torch.tensor([0, 10], dtype=torch.int32, device="cuda")
+    x, w = torch.randn(10, 8, device="cuda", requires_grad=True), torch.ones(10, 1, device="cuda", requires_grad=True)
+    rows = F.expert_sort(torch.zeros(10, dtype=torch.int64, device="cuda"), 1)
+    for make in (lambda: F.group_norm(x, off, 2), lambda: F.expert_combine(x, w, rows)):
+        y = make()
+        with torch.no_grad():
+            x.add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+
+
+def test_offsets_and_positions_outside_their_range_are_cut_to_it():
+    from torchsparse_b200.nn import functional as F
+
+    x = torch.randn(10, 8, device="cuda")
+    cut = F.group_norm(x, torch.tensor([0, 3, 10], dtype=torch.int32, device="cuda"), 2)
+    assert torch.equal(F.group_norm(x, torch.tensor([-5, 3, 999], dtype=torch.int32, device="cuda"), 2), cut)
+    big = torch.randn(9000, 8, device="cuda")
+    cut = F.group_norm(big, torch.tensor([0, 3, 9000], dtype=torch.int32, device="cuda"), 2)
+    assert torch.equal(F.group_norm(big, torch.tensor([-5, 3, 99999], dtype=torch.int32, device="cuda"), 2), cut)
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")      # noqa: E731
+    w = torch.ones(2, 1, device="cuda", requires_grad=True)
+    for kept in (-3, 2, 10 ** 9):
+        rows = F.ExpertRows(ints(0, 1), ints(-7, 10 ** 9)[:, None], ints(0, kept))
+        ys = torch.ones(2, 8, device="cuda", requires_grad=True)
+        out = F.expert_combine(ys, w, rows)
+        assert bool((out == 0).all()) and bool((torch.autograd.grad(out.sum(), w)[0] == 0).all())
+        F.expert_dispatch(ys, rows)
+
+
 # ------------------------------------------------------------------------------------------------ refusals
 def test_refusals():
     from torchsparse_b200 import nn as spnn
@@ -677,7 +735,11 @@ def test_refusals():
                 lambda: F.group_norm(x, off.cpu(), 2), lambda: F.embedding(off.cpu(), x)):
         with pytest.raises(RuntimeError):
             bad()
-    with pytest.raises(RuntimeError):      # a second derivative is refused, not wrong
-        leaf = x.clone().requires_grad_()
-        (g,) = torch.autograd.grad(F.group_norm(leaf, off, 2).square().sum(), leaf, create_graph=True)
-        g.sum().backward()
+    # a second derivative is refused, not wrong
+    leaf, gate = x.clone().requires_grad_(), torch.ones(10, 1, device="cuda", requires_grad=True)
+    rows = F.expert_sort(torch.zeros(10, dtype=torch.int64, device="cuda"), 2)
+    for make in (lambda: F.group_norm(leaf, off, 2), lambda: F.embedding(off, leaf), lambda: F.expert_dispatch(leaf, rows),
+                 lambda: F.expert_combine(leaf, gate, rows)):
+        (g,) = torch.autograd.grad(make().square().sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiated once only"):
+            g.sum().backward()

@@ -45,20 +45,27 @@ __device__ __forceinline__ int64_t offset_of(const Norm& a, int s) {
   return v < 0 ? 0 : v > a.n ? a.n : v;
 }
 
-// First sample that ends behind position p (a.b: none).  The whole warp searches: 32 samples per load, so that a batch of
-// usual size costs one round trip.
+// chunk of a position: both are below 2^31
+__device__ __forceinline__ int chunk_of(const Norm& a, int64_t p) { return (int)((unsigned)p / (unsigned)a.chunk); }
+
+// First sample that ends behind position p (a.b: none).  The whole warp searches: up to 128 samples cost one round trip.
 __device__ __forceinline__ int first_sample(const Norm& a, int64_t p) {
   const int lane = threadIdx.x & 31;
   int lo = 0, hi = a.b;      // samples before lo end at or before p; sample hi (if any) ends behind it
-  while (hi - lo > 32) {
+  while (hi - lo > 128) {
     const int step = (hi - lo + 31) / 32, at = lo + (lane + 1) * step - 1;
     const bool before = at < hi && offset_of(a, at + 1) <= p;
     const int k = __popc(__ballot_sync(0xffffffffu, before));
     hi = min(hi, lo + (k + 1) * step - 1);
     lo += k * step;
   }
-  const bool before = lo + lane < hi && offset_of(a, lo + lane + 1) <= p;
-  return lo + __popc(__ballot_sync(0xffffffffu, before));
+  bool before[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) before[i] = lo + lane + 32 * i < hi && offset_of(a, lo + lane + 32 * i + 1) <= p;
+  int k = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) k += __popc(__ballot_sync(0xffffffffu, before[i]));
+  return lo + k;
 }
 
 // Row at a grouped position; -1 for an entry of a caller's order that is no row.
@@ -246,10 +253,12 @@ __device__ __forceinline__ void activate_grad(const float (&z)[N], float (&g)[N]
   }
 }
 
-__device__ __forceinline__ float warp_sum(float v) {
+// sum over `width` neighbouring lanes, a power of two
+__device__ __forceinline__ float warp_sum(float v, int width = 32) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_down_sync(0xffffffffu, v, o);
-  return __shfl_sync(0xffffffffu, v, 0);
+  for (int o = 16; o > 0; o >>= 1)
+    if (o < width) v += __shfl_down_sync(0xffffffffu, v, o, width);
+  return __shfl_sync(0xffffffffu, v, 0, width);
 }
 
 // rows that lane l of `lanes` takes of `rows`
@@ -356,18 +365,21 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_stats_kernel(Norm a, con
       for (int i = 0; i < A; ++i) part[i * kNormThreads + threadIdx.x] = make_float2(run.mean[i], run.m2[i]);
     }
     __syncthreads();
-    // one warp per group of this column tile
+    // `sub` lanes per group of this column tile, a power of two up to a warp
     const int c_lo = first * VEC, c_hi = (first + width) * VEC;
     const int g_lo = c_lo / a.d, g_hi = (c_hi - 1) / a.d;
     const int64_t rows = hi - lo;
     float2* slot = slots + ((int64_t)blockIdx.y * (a.nblk + a.b) + blockIdx.x + s) * a.g;
-    for (int gr = g_lo + (threadIdx.x >> 5); gr <= g_hi; gr += kNormWarps) {
+    const int most = lanes * (min(a.d, c_hi - c_lo) / (VEC / A)), lg = most >= 32 ? 5 : 32 - __clz(most - 1);
+    const int sub = 1 << lg, side = 32 >> lg, in = threadIdx.x & (sub - 1);
+    for (int g0 = g_lo + (threadIdx.x >> 5) * side; g0 <= g_hi; g0 += kNormWarps * side) {      // the same for a warp
+      const int gr = g0 + ((threadIdx.x & 31) >> lg);
       const int k_lo = max(gr * a.d, c_lo), k_hi = min((gr + 1) * a.d, c_hi);
-      const int per_lane = (k_hi - k_lo) / (VEC / A), entries = per_lane * lanes;
+      const int per_lane = (k_hi - k_lo) / (VEC / A), entries = gr <= g_hi ? per_lane * lanes : 0;
       float w = 0.f, m = 0.f, q = 0.f;
       for (int pass = 0; pass < 2; ++pass) {      // the joint mean, then the squares about it
         float acc = 0.f;
-        for (int t = threadIdx.x & 31; t < entries; t += 32) {
+        for (int t = in; t < entries; t += sub) {
           const int l = t / per_lane, k = k_lo + (t - l * per_lane) * (VEC / A) - c_lo;
           const float cnt = (float)lane_rows(rows, lanes, l) * (VEC / A);
           if (cnt == 0.f) continue;
@@ -379,15 +391,15 @@ __global__ void __launch_bounds__(kNormThreads, 3) norm_stats_kernel(Norm a, con
             acc += fmaf(cnt * (e.x - m), e.x - m, e.y);
           }
         }
-        acc = warp_sum(acc);
+        acc = warp_sum(acc, sub);
         if (pass == 0) {
-          w = warp_sum(w);
+          w = warp_sum(w, sub);
           m = acc / w;
         } else {
           q = acc;
         }
       }
-      if ((threadIdx.x & 31) == 0) slot[gr] = make_float2(m, q);
+      if (in == 0 && gr <= g_hi) slot[gr] = make_float2(m, q);
     }
     __syncthreads();
   }
@@ -398,11 +410,11 @@ __global__ void __launch_bounds__(128) norm_join_kernel(Norm a, int vec, int til
                                                         float* __restrict__ mean, float* __restrict__ rstd) {
   const int lane = threadIdx.x & 31;
   for (int64_t t = blockIdx.x * 4 + (threadIdx.x >> 5); t < (int64_t)a.b * a.g; t += (int64_t)gridDim.x * 4) {
-    const int s = (int)(t / a.g), gr = (int)(t - (int64_t)s * a.g);
+    const int s = (int)((unsigned)t / (unsigned)a.g), gr = (int)t - s * a.g;
     const int64_t begin = offset_of(a, s), end = offset_of(a, s + 1);
     float w = 0.f, m = 0.f, q = 0.f;
     if (begin < end) {
-      const int j0 = (int)(begin / a.chunk), j1 = (int)((end - 1) / a.chunk);
+      const int j0 = chunk_of(a, begin), j1 = chunk_of(a, end - 1);
       for (int pass = 0; pass < 2; ++pass) {
         float acc = 0.f;
         for (int y = 0; y < tiles; ++y) {
@@ -581,13 +593,15 @@ __global__ void __launch_bounds__(kJoinThreads) norm_grad_join_kernel(Norm a, co
   const int width = min(a.d, kJoinThreads), lanes = kJoinThreads / width;
   const int lane = threadIdx.x / width, q = threadIdx.x - lane * width;
   for (int64_t t = blockIdx.x; t < (int64_t)a.b * a.g; t += gridDim.x) {
-    const int s = (int)(t / a.g), gr = (int)(t - (int64_t)s * a.g);
+    const int s = (int)((unsigned)t / (unsigned)a.g), gr = (int)t - s * a.g;
     const int64_t begin = offset_of(a, s), end = offset_of(a, s + 1);
     float m1 = 0.f, m2 = 0.f;
     for (int k = q; k - q < a.d; k += width) {
+      const float w = a.w && k < a.d ? load_any(a.w, a.p_dtype, gr * a.d + k) : 1.f;
       float u = 0.f, v = 0.f;
       if (lane < lanes && k < a.d && begin < end) {
-        const int j0 = (int)(begin / a.chunk), j1 = (int)((end - 1) / a.chunk);
+        const int j0 = chunk_of(a, begin), j1 = chunk_of(a, end - 1);
+#pragma unroll 4
         for (int j = j0 + lane; j <= j1; j += lanes) {
           const float2 f = slots[((int64_t)j + s) * a.c + gr * a.d + k];
           u += f.x;
@@ -596,14 +610,19 @@ __global__ void __launch_bounds__(kJoinThreads) norm_grad_join_kernel(Norm a, co
       }
       part[threadIdx.x] = make_float2(u, v);
       __syncthreads();
-      if (lane == 0 && k < a.d) {
-        for (int l = 1; l < lanes; ++l) {
-          u += part[l * width + q].x;
-          v += part[l * width + q].y;
+      for (int half = lanes; half > 1;) {      // the upper half of the lanes onto the lower
+        const int keep = (half + 1) / 2;
+        if (lane + keep < half) {
+          u += part[threadIdx.x + keep * width].x;
+          v += part[threadIdx.x + keep * width].y;
+          part[threadIdx.x] = make_float2(u, v);
         }
+        half = keep;
+        __syncthreads();
+      }
+      if (lane == 0 && k < a.d) {
         const int ch = gr * a.d + k;
         by_channel[(int64_t)s * a.c + ch] = make_float2(u, v);
-        const float w = a.w ? load_any(a.w, a.p_dtype, ch) : 1.f;
         m1 = fmaf(w, u, m1);
         m2 = fmaf(w, v, m2);
       }
@@ -969,7 +988,7 @@ bool good_dtype(int dtype) { return dtype == TSB_F32 || dtype == TSB_F16 || dtyp
 int check_norm(int64_t n, int64_t c, int64_t g, int64_t b, const void* offsets, int dtype, int p_dtype, int act) {
   if (n < 0 || c < 1 || g < 1 || c % g != 0 || b < 0 || (b && !offsets) || act < kActNone || act > kActSilu) return TSB_ERR_BAD_ARG;
   if (!good_dtype(dtype) || !good_dtype(p_dtype)) return TSB_ERR_UNSUPPORTED;
-  if (n > 0x7fffffff || b > 0x3fffffff || c > 65536) return TSB_ERR_LIMIT;
+  if (n > 0x7fffffff || c > 65536 || b > 0x7fffffff / g) return TSB_ERR_LIMIT;
   return TSB_OK;
 }
 

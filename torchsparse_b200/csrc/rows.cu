@@ -240,16 +240,18 @@ __device__ __forceinline__ void load_tile(const PassIn& in, int64_t n, unsigned 
 
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(PassIn in, int64_t n, int shift, int bits, int64_t tiles,
                                                                   unsigned* __restrict__ counts) {
-  __shared__ unsigned short whist[kSortThreads / 32][kMaxDigits];
-  __shared__ unsigned total[kMaxDigits], masks[kSortThreads / 32 * kMaxDigits];
-  const int64_t first = (int64_t)blockIdx.x * kSortTile + (threadIdx.x >> 5) * 32 * kItems + (threadIdx.x & 31);
-  unsigned key[kItems], digit[kItems], rank[kItems];
+  __shared__ unsigned total[kMaxDigits];
+  const int n_digits = 1 << bits;
+  unsigned key[kItems];
   bool on[kItems];
-  load_tile(in, n, key, on, first);
+  load_tile(in, n, key, on, (int64_t)blockIdx.x * kSortTile + (threadIdx.x >> 5) * 32 * kItems + (threadIdx.x & 31));
+  for (int d = threadIdx.x; d < n_digits; d += kSortThreads) total[d] = 0;
+  __syncthreads();
 #pragma unroll
-  for (int it = 0; it < kItems; ++it) digit[it] = (key[it] >> shift) & ((1u << bits) - 1);
-  rank_tile(digit, on, rank, whist, masks, total, 1 << bits);
-  for (int d = threadIdx.x; d < (1 << bits); d += kSortThreads) counts[d * tiles + blockIdx.x] = total[d];
+  for (int it = 0; it < kItems; ++it)
+    if (on[it]) atomicAdd(total + ((key[it] >> shift) & (n_digits - 1)), 1u);
+  __syncthreads();
+  for (int d = threadIdx.x; d < n_digits; d += kSortThreads) counts[d * tiles + blockIdx.x] = total[d];
 }
 
 // one block per digit: exclusive sums over the tiles in place, the digit's count behind them
@@ -801,7 +803,7 @@ __global__ void __launch_bounds__(kThreads) combine_kernel(const T* __restrict__
   extern __shared__ __align__(16) unsigned char pipe[];
   const int cols = (int)(c / VEC), groups = kThreads / lanes, group = threadIdx.x / lanes, lane = threadIdx.x - group * lanes;
   const int64_t step = (int64_t)gridDim.x * groups;
-  const unsigned n_kept = (unsigned)min((int64_t)__ldg(kept), n * k);
+  const unsigned n_kept = (unsigned)min((int64_t)max(__ldg(kept), 0), n * k);
   struct Place {      // row, first vector, first choice
     int64_t i;
     int v, q;
@@ -916,7 +918,7 @@ __global__ void __launch_bounds__(kThreads) combine_grad_kernel(const T* __restr
   extern __shared__ __align__(16) unsigned char pipe[];
   const int cols = (int)(c / VEC), lane = threadIdx.x & (lanes - 1), groups = kThreads / lanes;
   const int64_t step = (int64_t)gridDim.x * groups;
-  const unsigned n_kept = (unsigned)min((int64_t)__ldg(kept), pairs);
+  const unsigned n_kept = (unsigned)min((int64_t)max(__ldg(kept), 0), pairs);
   struct Place {      // choice, first vector
     int64_t q;
     int v;

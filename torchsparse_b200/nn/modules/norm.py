@@ -34,6 +34,9 @@ class GroupNorm(nn.GroupNorm):
     fp32, fp16 and bf16 features on a GPU run on the library's kernels, with parameters of the same or another of these
     dtypes; other features run through torch, sample by sample."""
 
+    activation: Optional[str] = None      # also of modules that were pickled without one
+    negative_slope = 0.01
+
     def __init__(self, num_groups: int, num_channels: int, eps: float = 1e-5, affine: bool = True, device=None, dtype=None,
                  *, activation: Optional[str] = None, negative_slope: float = 0.01) -> None:
         super().__init__(num_groups, num_channels, eps, affine, device, dtype)
