@@ -497,6 +497,40 @@ def test_dropped_choices_hide_nan_of_their_rows():
     assert bool((dys[2:] == 0).all()) and dw.tolist() == [[8.0, 0.0], [8.0, 0.0]]
 
 
+def test_what_belongs_to_nothing_may_hold_anything():
+    """NaN in rows of no sample, of no token and of no expert, and in their gradients, reaches nothing else."""
+    from torchsparse_b200.nn import functional as F
+
+    for n in (600, 20000):                                        # one block per sample and group, and chunks of rows
+        off = torch.tensor([n // 6, n // 2, n - n // 5], dtype=torch.int32, device="cuda")
+        outside = torch.ones(n, dtype=torch.bool, device="cuda")
+        outside[n // 6:n - n // 5] = False
+        for order in (None, torch.randperm(n, device="cuda").int()):
+            x, dy = features(n, 24, torch.float32, 1), features(n, 24, torch.float32, 2)
+            where = outside if order is None else torch.zeros_like(outside).index_put_((order.long(),), outside)
+            w, b = (t.requires_grad_() for t in affine(24))
+            results = []
+            for fill in (0.0, float("nan")):
+                xs = torch.where(where[:, None], fill, x).requires_grad_()
+                y = F.group_norm(xs, off, 3, w, b, activation="silu", order=order)
+                grads = torch.autograd.grad(y, (xs, w, b), torch.where(where[:, None], fill, dy))
+                results.append([y.detach(), *grads])
+            assert bool((results[1][0][where] == 0).all()) and bool((results[1][1][where] == 0).all())
+            for a, c in zip(*results):
+                assert torch.equal(a, c)
+    table = torch.randn(5, 24, device="cuda", requires_grad=True)
+    tokens = torch.tensor([0, -1, 3, 2, 7, 2], device="cuda")
+    dy = torch.ones(6, 24, device="cuda")
+    dy[[1, 3, 4, 5]] = float("nan")                               # no token, the padding, no token, the padding
+    (dt,) = torch.autograd.grad(F.embedding(tokens, table, padding_idx=2), table, dy)
+    assert dt[:, 0].tolist() == [1, 0, 0, 1, 0]
+    rows = F.expert_sort(torch.tensor([[0, -1], [1, 2]], device="cuda"), 2)
+    x = torch.randn(2, 24, device="cuda", requires_grad=True)
+    dxs = torch.ones(4, 24, device="cuda")
+    dxs[2:] = float("inf")                                        # behind the last expert
+    assert bool((torch.autograd.grad(F.expert_dispatch(x, rows), x, dxs)[0] == 1).all())
+
+
 def test_experts_of_no_rows():
     from torchsparse_b200.nn import functional as F
 

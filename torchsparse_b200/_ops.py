@@ -27,5 +27,6 @@ _module = _load()
 group_rows = _module.group_rows
 group_norm = _module.group_norm
 embedding = _module.embedding
+expert_sort = _module.expert_sort
 expert_dispatch = _module.expert_dispatch
 expert_combine = _module.expert_combine

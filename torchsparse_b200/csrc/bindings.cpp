@@ -103,21 +103,37 @@ variable_list once(variable_list grads) {
 }
 
 // ------------------------------------------------------------------------------------------------ grouping
-std::tuple<Tensor, Tensor, Tensor> group_rows(const Tensor& keys, int64_t num_groups, bool want_inverse) {
-  need_cuda(keys);
-  check_index(keys, "keys");
-  TORCH_CHECK_VALUE(keys.dim() == 1, "keys must be a vector, not ", keys.sizes());
+// order, offsets and, where its shape is given, the position of every key
+std::tuple<Tensor, Tensor, Tensor> group(const Tensor& keys, int64_t num_groups, at::OptionalIntArrayRef inverse_shape) {
   TORCH_CHECK_VALUE(num_groups >= 1 && num_groups < (1ll << 31), "the number of groups must be in [1, 2^31), not ", num_groups);
   Call call(keys);
   const int64_t n = keys.size(0);
   const auto opts = keys.options().dtype(at::kInt);
   Tensor order = at::empty({n}, opts), offsets = at::empty({num_groups + 1}, opts), inverse;
-  if (want_inverse) inverse = at::empty({n}, opts);
+  if (inverse_shape.has_value()) inverse = at::empty(*inverse_shape, opts);
   void* ws = call.workspace(tsb_group_rows_workspace_bytes(n, num_groups), keys);
   check_status(tsb_group_rows(keys.const_data_ptr(), keys.scalar_type() == at::kLong, keys.stride(0), n, num_groups,
                               order.mutable_data_ptr<int32_t>(), (int32_t*)out_ptr(inverse), offsets.mutable_data_ptr<int32_t>(), ws,
                               call.bytes, call.stream()),
                "group_rows");
+  return {order, offsets, inverse};
+}
+
+std::tuple<Tensor, Tensor> group_rows(const Tensor& keys, int64_t num_groups) {
+  need_cuda(keys);
+  check_index(keys, "keys");
+  TORCH_CHECK_VALUE(keys.dim() == 1, "keys must be a vector, not ", keys.sizes());
+  auto [order, offsets, inverse] = group(keys, num_groups, std::nullopt);
+  return {order, offsets};
+}
+
+std::tuple<Tensor, Tensor, Tensor> expert_sort(const Tensor& experts, int64_t num_experts) {
+  need_cuda(experts);
+  check_index(experts, "experts");
+  TORCH_CHECK_VALUE(experts.dim() == 1 || experts.dim() == 2, "experts must be [N, k] or [N], not ", experts.sizes());
+  const int64_t shape[2] = {experts.size(0), experts.dim() == 2 ? experts.size(1) : 1};
+  TORCH_CHECK_VALUE(shape[1] >= 1, "every row needs at least one choice");
+  auto [order, offsets, inverse] = group(experts.reshape(-1), num_experts, at::IntArrayRef(shape, 2));
   return {order, inverse, offsets};
 }
 
@@ -353,6 +369,7 @@ Tensor expert_combine(const Tensor& rows, const Tensor& weights, const Tensor& i
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("group_rows", &group_rows);
+  m.def("expert_sort", &expert_sort);
   m.def("group_norm", &group_norm);
   m.def("embedding", &embedding);
   m.def("expert_dispatch", &expert_dispatch);

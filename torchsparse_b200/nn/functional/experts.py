@@ -21,13 +21,7 @@ def expert_sort(experts: torch.Tensor, num_experts: int) -> ExpertRows:
     """Sort the choices of a router: ``experts`` int32 or int64 [N, k] (or [N]) names the weight matrices that row i is
     sent to.  Choices of one expert keep their order; a choice outside [0, num_experts) (-1, say, for one dropped for
     want of room) goes to no expert."""
-    if experts.dim() not in (1, 2):
-        raise ValueError(f"experts must be [N, k] or [N], not {tuple(experts.shape)}")
-    shape = (experts.shape[0], experts.shape[1] if experts.dim() == 2 else 1)
-    if shape[1] < 1:
-        raise ValueError("every row needs at least one choice")
-    order, inverse, offsets = _ops.group_rows(experts.reshape(-1), num_experts, True)
-    return ExpertRows(order, inverse.view(shape), offsets)
+    return ExpertRows(*_ops.expert_sort(experts, num_experts))
 
 
 def expert_dispatch(feats: torch.Tensor, rows: ExpertRows) -> torch.Tensor:

@@ -19,8 +19,7 @@ class RowGroups(NamedTuple):
 def group_rows(keys: torch.Tensor, num_groups: int) -> RowGroups:
     """Group rows by ``keys`` (int32 or int64 [N]); rows of one group keep their order, a key outside
     [0, num_groups) belongs to no group."""
-    order, _, offsets = _ops.group_rows(keys, num_groups, False)
-    return RowGroups(order, offsets)
+    return RowGroups(*_ops.group_rows(keys, num_groups))
 
 
 def sample_rows(input: SparseTensor, batch_size: Optional[int] = None) -> RowGroups:
