@@ -435,7 +435,7 @@ __global__ void __launch_bounds__(128) norm_join_kernel(Norm a, int vec, int til
           const int width = tile_channels(a, vec, y, gr);
           if (width == 0) continue;
           const float2* at = slots + ((int64_t)y * (a.nblk + a.b) + s) * a.g + gr;
-#pragma unroll 8
+#pragma unroll 4
           for (int j = j0 + lane; j <= j1; j += 32) {
             const float cnt = (float)(min(end, (j + 1) * a.chunk) - max(begin, j * a.chunk)) * width;
             const float2 e = at[(int64_t)j * a.g];

@@ -48,7 +48,7 @@ def group_norm(feats: torch.Tensor, offsets: torch.Tensor, num_groups: int, weig
     """``act(group_norm(feats))`` over the rows of each sample, features [N, C] (fp32, fp16 or bf16).
 
     ``offsets`` int32 [samples + 1], ascending: sample s is rows ``offsets[s]`` to ``offsets[s + 1]``, or, with
-    ``order`` int32 [N], the rows ``order[offsets[s] : offsets[s + 1]]`` (see ``group_rows``).  A sample may be empty;
+    ``order`` int32 [N], a permutation, the rows ``order[offsets[s] : offsets[s + 1]]`` (see ``group_rows``).  A sample may be empty;
     rows of no sample become zero.  A group with one value becomes ``act(bias)``.  ``weight`` and ``bias`` [C] may have a
     dtype of their own (fp32 beside 16-bit features).  ``activation``: None, "relu", "leaky_relu" or "silu".
     Statistics and sums are fp32 and run in a fixed order."""
