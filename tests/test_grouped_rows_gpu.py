@@ -289,6 +289,40 @@ def test_group_norm_gradient_against_differences():
         assert abs(float(slope - want)) < 6e-4 * float(dy.abs().sum())
 
 
+@pytest.mark.parametrize("ordered", [False, True])
+@pytest.mark.parametrize("act", [None, "silu", "leaky_relu"])
+def test_group_norm_gradient_differentiated_again(act, ordered):
+    """A gradient penalty: the first derivative under create_graph equals the kernels', the second the definition's in 64
+    bits.  1e-4 of the largest value is some 800 roundings of fp32; the chain of two derivatives has below 100."""
+    from torchsparse_b200.nn import functional as F
+
+    cuts, n, c = [5, 40, 40, 97], 100, 12
+    g = torch.Generator(device="cuda").manual_seed(6)
+    order = torch.randperm(n, generator=g, device="cuda").int() if ordered else None
+    x, dy, (w, b) = features(n, c, torch.float32), torch.randn(n, c, generator=g, device="cuda"), affine(c)
+    leaves = [t.clone().requires_grad_() for t in (x, w, b, dy)]
+    y = F.group_norm(leaves[0], torch.tensor(cuts, dtype=torch.int32, device="cuda"), 3, leaves[1], leaves[2], 1e-5, act, 0.1, order)
+    first = torch.autograd.grad(y, leaves[:3], leaves[3], create_graph=True)
+    plain = torch.autograd.grad(y, leaves[:3], leaves[3], retain_graph=True)
+    wide = [t.double().requires_grad_() for t in (x, w, b, dy)]
+    parts = torch.zeros(n, c, dtype=torch.float64, device="cuda")
+    for lo, hi in zip(cuts, cuts[1:]):
+        rows = torch.arange(lo, hi, device="cuda") if order is None else order[lo:hi].long()
+        if hi > lo:
+            v = torch.nn.functional.group_norm(wide[0][rows].t()[None], 3, wide[1], wide[2], 1e-5)[0].t()
+            v = {None: lambda t: t, "silu": torch.nn.functional.silu,
+                 "leaky_relu": lambda t: torch.nn.functional.leaky_relu(t, 0.1)}[act](v)
+            parts = parts.index_copy(0, rows, v)
+    want = torch.autograd.grad(parts, wide[:3], wide[3], create_graph=True)
+    for a, k, e in zip(first, plain, want):
+        assert float((a - k).detach().abs().max()) < 1e-4 * float(e.detach().abs().max())
+        assert float((a - e).detach().abs().max()) < 1e-4 * float(e.detach().abs().max())
+    # without an activation the bias has no part in the first derivative: zeros
+    second = torch.autograd.grad(sum(t.square().sum() for t in first), leaves, materialize_grads=True)
+    for a, e in zip(second, torch.autograd.grad(sum(t.square().sum() for t in want), wide, materialize_grads=True)):
+        assert float((a - e).abs().max()) < 1e-4 * max(float(e.abs().max()), 1.0)
+
+
 def test_group_norm_beyond_32_bit_offsets():
     from torchsparse_b200.nn import functional as F
 
@@ -772,8 +806,7 @@ def test_refusals():
     # a second derivative is refused, not wrong
     leaf, gate = x.clone().requires_grad_(), torch.ones(10, 1, device="cuda", requires_grad=True)
     rows = F.expert_sort(torch.zeros(10, dtype=torch.int64, device="cuda"), 2)
-    for make in (lambda: F.group_norm(leaf, off, 2), lambda: F.embedding(off, leaf), lambda: F.expert_dispatch(leaf, rows),
-                 lambda: F.expert_combine(leaf, gate, rows)):
+    for make in (lambda: F.embedding(off, leaf), lambda: F.expert_dispatch(leaf, rows), lambda: F.expert_combine(leaf, gate, rows)):
         (g,) = torch.autograd.grad(make().square().sum(), leaf, create_graph=True)
         with pytest.raises(RuntimeError, match="differentiated once only"):
             g.sum().backward()

@@ -183,6 +183,33 @@ std::pair<Tensor, Tensor> norm_forward(const Tensor& x, const Tensor& w, const T
   return {y, stats};
 }
 
+// The same in torch's own operations, for a gradient that is to be differentiated again (a gradient penalty): slower, and
+// differentiable as often as wanted.
+Tensor norm_by_torch(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& offsets, const Tensor& order, const NormArgs& a) {
+  const int64_t n = x.size(0), c = x.size(1), samples = offsets.size(0) - 1;
+  const Tensor rows = order.defined() ? order.to(at::kLong) : order, off = offsets.to(at::kLong).clamp(0, n);
+  const Tensor pos = at::arange(n, off.options());
+  const Tensor found = at::searchsorted(off.slice(0, 1), pos, /*out_int32=*/false, /*right=*/true);
+  const Tensor inside = pos.ge(off[0]).logical_and(found.lt(samples)), sample = found.masked_fill(inside.logical_not(), samples);
+  Tensor v = x.to(at::kFloat);
+  if (rows.defined()) v = v.index_select(0, rows);
+  v = at::where(inside.unsqueeze(1), v, at::zeros({}, v.options()));
+  const Tensor ones = at::ones({n, 1}, v.options());
+  const Tensor count = at::zeros({samples + 1, 1}, v.options()).index_add(0, sample, ones).clamp_min(1) * (c / a.groups);
+  const auto mean = [&](const Tensor& t) {
+    const Tensor sums = at::zeros({samples + 1, a.groups}, v.options()).index_add(0, sample, t.view({n, a.groups, -1}).sum(2));
+    return (sums / count).index_select(0, sample).repeat_interleave(c / a.groups, 1);
+  };
+  const Tensor d = v - mean(v);
+  Tensor z = d * (mean(d * d) + a.eps).rsqrt();
+  if (w.defined()) z = z * w.to(at::kFloat);
+  if (b.defined()) z = z + b.to(at::kFloat);
+  z = a.act == 1 ? at::relu(z) : a.act == 2 ? at::leaky_relu(z, a.slope) : a.act == 3 ? at::silu(z) : z;
+  z = at::where(inside.unsqueeze(1), z, at::zeros({}, z.options()));
+  if (rows.defined()) z = at::zeros_like(z).index_copy(0, rows, z);
+  return z.to(x.scalar_type());
+}
+
 struct GroupNorm : Function<GroupNorm> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias,
                         const Tensor& offsets, const std::optional<Tensor>& order, int64_t groups, double eps, int64_t act,
@@ -192,6 +219,7 @@ struct GroupNorm : Function<GroupNorm> {
     auto [y, stats] = norm_forward(x, w, b, offsets, o, a, (int)p_code, true);
     ctx->save_for_backward({x, w, b, offsets, o, stats});
     ctx->saved_data["groups"] = groups;
+    ctx->saved_data["eps"] = eps;
     ctx->saved_data["act"] = act;
     ctx->saved_data["slope"] = slope;
     ctx->saved_data["code"] = p_code;
@@ -201,6 +229,20 @@ struct GroupNorm : Function<GroupNorm> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1], &b = saved[2], &offsets = saved[3], &order = saved[4], &stats = saved[5];
     const int64_t n = x.size(0), c = x.size(1), samples = offsets.size(0) - 1, groups = ctx->saved_data["groups"].toInt();
+    if (at::GradMode::is_enabled()) {
+      const NormArgs a{groups, ctx->saved_data["eps"].toDouble(), ctx->saved_data["slope"].toDouble(), ctx->saved_data["act"].toInt()};
+      variable_list wanted, made(10);
+      for (const Tensor* t : {&x, &w, &b})
+        if (t->defined() && t->requires_grad()) wanted.push_back(*t);
+      const auto got = torch::autograd::grad({norm_by_torch(x, w, b, offsets, order, a)}, wanted, {grads[0]}, /*retain_graph=*/true,
+                                             /*create_graph=*/true, /*allow_unused=*/true);
+      size_t k = 0, i = 0;
+      for (const Tensor* t : {&x, &w, &b}) {
+        if (t->defined() && t->requires_grad()) made[i] = got[k++];
+        ++i;
+      }
+      return made;
+    }
     Call call(x);
     const Tensor dy = grads[0].contiguous();
     Tensor dx = at::empty_like(x), dw, db;
@@ -214,7 +256,7 @@ struct GroupNorm : Function<GroupNorm> {
                                     dtype, (int)ctx->saved_data["code"].toInt(), out_ptr(dx), out_ptr(dw), out_ptr(db), ws, call.bytes,
                                     call.stream()),
                  "group_norm_backward");
-    auto made = once({dx, dw, db});
+    variable_list made{dx, dw, db};
     made.resize(10);
     return made;
   }
