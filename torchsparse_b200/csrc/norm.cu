@@ -332,7 +332,6 @@ struct Running {
   }
 };
 
-//
 // One read of x.  1M x 64 bf16: 33 us, 3.9 TB/s; 61441 x 96 bf16, which the L2 cache holds: 9 us.  What is left above
 // the copy rate (20 us) is the start of a block (its samples, the first rows) and the join at its end, some 5 us in all:
 // twice as many blocks of half the rows took 36 us, three times as many 41.
