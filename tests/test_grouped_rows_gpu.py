@@ -353,6 +353,8 @@ def test_group_norm_module_matches_torch_and_takes_rows():
         y = m(x)
         assert y.coords is x.coords and y._caches is x._caches and y.stride == x.stride
         assert torch.equal(m(x, F.sample_rows(x)).feats, y.feats)
+        for coords_too in (x.coords.cpu(), x.coords.long(), x.coords.short()):      # wherever and whatever the coordinates are
+            assert torch.equal(m(ts.SparseTensor(x.feats, coords_too)).feats, y.feats)
         for s in range(4):
             rows = x.coords[:, 0] == s
             want = fn(torch.nn.functional.group_norm(x.feats[rows].t()[None].double(), 8, m.weight.double(), m.bias.double(), m.eps))

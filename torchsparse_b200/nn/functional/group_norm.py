@@ -25,7 +25,9 @@ def group_rows(keys: torch.Tensor, num_groups: int) -> RowGroups:
 def sample_rows(input: SparseTensor, batch_size: Optional[int] = None) -> RowGroups:
     """The rows of a tensor grouped by batch sample.  Without ``batch_size`` the largest batch index is read from the
     device.  The result serves every layer on the same coordinates."""
-    batch = input.coords[:, 0]
+    batch = input.coords[:, 0].to(input.feats.device)
+    if batch.dtype not in (torch.int32, torch.int64):
+        batch = batch.long()
     if batch_size is None:
         batch_size = int(batch.max().item()) + 1 if batch.numel() else 0
     return group_rows(batch, max(int(batch_size), 1))
