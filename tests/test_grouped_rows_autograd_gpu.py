@@ -1,0 +1,125 @@
+"""What autograd, forward-mode differentiation, functional transforms and tracing see of the operators over grouped rows.
+
+Tolerances are shares of the largest value of a result: 2e-5 is 335 roundings of fp32 (2^-24 each).  The longest chain of a
+first derivative or a tangent is below 200 of them: a sum over a sample is joined piece by piece, at most 100 deep, and some
+twenty steps lie before and behind each of the two sums.  A second derivative goes through that twice and takes differences
+of its terms: 1e-4."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+FIRST, SECOND = 2e-5, 1e-4
+ACTS = {None: lambda t: t, "relu": torch.relu, "leaky_relu": lambda t: torch.nn.functional.leaky_relu(t, 0.1),
+        "silu": torch.nn.functional.silu}
+
+
+def definition(x, w, b, cuts, order, groups, act, eps=1e-5):
+    """Sample by sample with torch's own group norm, in the type of x; zeros in rows of no sample."""
+    y = torch.zeros_like(x)
+    for lo, hi in zip(cuts, cuts[1:]):
+        if hi > lo:
+            rows = torch.arange(lo, hi, device=x.device) if order is None else order[lo:hi].long()
+            z = torch.nn.functional.group_norm(x[rows].t()[None], groups, w, b, eps)[0].t()
+            y = y.index_copy(0, rows, ACTS[act](z))
+    return y
+
+
+def near(got, want, share):
+    assert got.shape == want.shape
+    if got.numel():
+        off = float((got.detach().double() - want.detach()).abs().max())
+        assert off <= share * float(want.detach().abs().max()), f"off by {off / max(float(want.detach().abs().max()), 1e-300):.3g}"
+
+
+def data(n, c, seed=0, samples=None):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    make = lambda *s: torch.randn(*s, generator=g, device="cuda")      # noqa: E731
+    x = make(n, c) + 0.5
+    w, b = torch.rand(c, generator=g, device="cuda") + 0.5, make(c) * 0.3
+    order = torch.randperm(n, generator=g, device="cuda").int() if samples is None else None
+    return x, w, b, make(n, c), order, make
+
+
+def ints(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+# ------------------------------------------------------------------------------------------------ a gradient of a gradient
+def test_gradient_of_a_very_long_sample_to_be_differentiated_again():
+    """More rows than fp32 counts one by one, and a mean that is no zero."""
+    from torchsparse_b200.nn import functional as F
+
+    n, c = 17_000_003, 2
+    x, w, b, dy, _, _ = data(n, c, 1, samples=1)
+    x += 2.0
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = F.group_norm(leaves[0], ints([0, n]), 1, leaves[1], leaves[2])
+    got = torch.autograd.grad(y, leaves, dy, create_graph=True)
+    wide = [t.detach().double().requires_grad_() for t in leaves]
+    want = torch.autograd.grad(definition(*wide, [0, n], None, 1, None), wide, dy.double())
+    for a, e in zip(got, want):
+        near(a, e, FIRST)
+
+
+@pytest.mark.parametrize("ordered", [False, True])
+def test_second_derivative_of_long_samples(ordered):
+    from torchsparse_b200.nn import functional as F
+
+    n, c, cuts = 4_000_003, 4, [2, 3_999_000, 3_999_000, 4_000_000]
+    x, w, b, dy, order, _ = data(n, c, 2, None if ordered else 1)
+    leaves = [t.requires_grad_() for t in (x, w, b, dy)]
+    y = F.group_norm(leaves[0], ints(cuts), 2, leaves[1], leaves[2], activation="silu", order=order)
+    first = torch.autograd.grad(y, leaves[:3], leaves[3], create_graph=True)
+    wide = [t.detach().double().requires_grad_() for t in leaves]
+    want = torch.autograd.grad(definition(*wide[:3], cuts, order, 2, "silu"), wide[:3], wide[3], create_graph=True)
+    for a, e in zip(first, want):
+        near(a, e, FIRST)
+    second = torch.autograd.grad(first[0].square().sum(), leaves)
+    for a, e in zip(second, torch.autograd.grad(want[0].square().sum(), wide)):
+        near(a, e, SECOND)
+
+
+def test_second_derivative_gives_the_same_bits():
+    from torchsparse_b200.nn import functional as F
+
+    x, w, b, dy, order, _ = data(300_000, 8, 3)
+    runs = []
+    for _ in range(4):
+        leaves = [t.clone().requires_grad_() for t in (x, w, b, dy)]
+        y = F.group_norm(leaves[0], ints([0, 100_000, 299_000]), 2, leaves[1], leaves[2], activation="silu", order=order)
+        first = torch.autograd.grad(y, leaves[:3], leaves[3], create_graph=True)
+        runs.append(list(first) + list(torch.autograd.grad(first[0].square().sum(), leaves)))
+    for run in runs[1:]:
+        for a, e in zip(run, runs[0]):
+            assert torch.equal(a, e)
+
+
+@pytest.mark.parametrize("n,cuts", [(0, [0]), (0, [0, 0, 0]), (5, [0]), (5, [2, 2])])
+def test_second_derivative_of_no_rows(n, cuts):
+    from torchsparse_b200.nn import functional as F
+
+    x, w, b, dy, order, _ = data(n, 12, 4)
+    for o in (None, order):
+        leaves = [t.clone().requires_grad_() for t in (x, w, b, dy)]
+        y = F.group_norm(leaves[0], ints(cuts), 3, leaves[1], leaves[2], activation="silu", order=o)
+        first = torch.autograd.grad(y, leaves[:3], leaves[3], create_graph=True)
+        assert [t.shape for t in first] == [x.shape, w.shape, b.shape] and all(bool((t == 0).all()) for t in first)
+        second = torch.autograd.grad(sum(t.square().sum() for t in first), leaves, materialize_grads=True)
+        assert all(bool((t == 0).all()) for t in second)
+
+
+@pytest.mark.parametrize("n", [40, 70_001])
+def test_second_derivative_with_an_order_that_is_no_permutation(n):
+    """Wrong values, and no fault: entries that are no rows go nowhere, as in the kernels."""
+    from torchsparse_b200.nn import functional as F
+
+    x, w, b, dy, order, _ = data(n, 12, 10)
+    order[::7], order[1], order[2] = n, -1, 2 ** 31 - 1
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    y = F.group_norm(leaves[0], ints([-5, n // 3, 2 * n]), 3, leaves[1], leaves[2], activation="silu", order=order)
+    first = torch.autograd.grad(y, leaves, dy, create_graph=True)
+    second = torch.autograd.grad(first[0].square().sum(), leaves)
+    for t in (*first, *second):
+        assert bool(t.isfinite().all())
