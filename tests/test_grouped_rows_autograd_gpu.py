@@ -46,6 +46,72 @@ def ints(values):
     return torch.tensor(values, dtype=torch.int32, device="cuda")
 
 
+# ------------------------------------------------------------------------------------------------ traced programs
+def test_traced_operators_are_in_the_graph_and_run_on_new_inputs():
+    from torchsparse_b200.nn import functional as F
+
+    def everything(x, w, b, offsets, tokens, choice, gate, table):
+        y = F.group_norm(x, offsets, 3, w, b, activation="silu") + F.embedding(tokens, table, 2.0)
+        rows = F.expert_sort(choice, 4)
+        return F.expert_combine(F.expert_dispatch(y, rows), gate, rows), F.group_rows(tokens, 9).order
+
+    def inputs(seed):
+        x, w, b, _, _, make = data(500, 12, seed)
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        return (x, w, b, ints([0, 100 + seed, 500]), torch.randint(0, 9, (500,), generator=g, device="cuda"),
+                torch.randint(-1, 4, (500, 2), generator=g, device="cuda"), make(500, 2), make(9, 12))
+
+    for record in (False, True):
+        with torch.set_grad_enabled(record):
+            args = [t.requires_grad_() if record and t.is_floating_point() else t for t in inputs(1)]
+            traced = torch.jit.trace(everything, args, check_trace=False)
+        kinds = {node.kind() for node in traced.graph.nodes()}
+        for name in ("group_norm", "embedding", "expert_sort", "expert_dispatch", "expert_combine", "group_rows"):
+            assert f"torchsparse_b200::{name}" in kinds
+        with torch.no_grad():
+            for got, want in zip(traced(*inputs(2)), everything(*inputs(2))):
+                assert torch.equal(got, want)
+
+
+def test_a_traced_norm_layer_runs_on_new_features():
+    import torchsparse_b200 as ts
+    from torchsparse_b200 import nn as spnn
+
+    m = spnn.GroupNorm(4, 16, activation="silu").cuda().requires_grad_(False)      # a function is traced, so they are constants
+    coords = torch.randint(0, 9, (400, 4), generator=torch.Generator().manual_seed(0)).int().cuda()
+    coords[:, 0] = torch.arange(400, device="cuda") % 3
+    run = lambda x: m(ts.SparseTensor(x, coords)).feats      # noqa: E731
+    with torch.no_grad():
+        traced = torch.jit.trace(run, data(400, 16, 1)[0], check_trace=False)
+        x = data(400, 16, 2)[0]
+        assert torch.equal(traced(x), run(x))
+
+
+def test_gradients_recorded_by_a_dispatch_mode():
+    """A recorder below autograd sees the operators and their gradients, not what their kernels leave behind."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from torchsparse_b200.nn import functional as F
+
+    tokens = torch.randint(-1, 9, (300,), generator=torch.Generator().manual_seed(3)).cuda()
+    rows = F.expert_sort(torch.randint(-1, 4, (300, 2), generator=torch.Generator().manual_seed(4)).cuda(), 4)
+    offsets = ints([0, 100, 300])
+
+    def step(x, w, b, table, gate, dout):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b, table, gate)]
+        y = F.group_norm(leaves[0], offsets, 3, leaves[1], leaves[2], activation="silu") + F.embedding(tokens, leaves[3], 2.0)
+        out = F.expert_combine(F.expert_dispatch(y, rows), leaves[4], rows)
+        return [out.detach()] + list(torch.autograd.grad(out, leaves, dout))
+
+    def inputs(seed):
+        x, w, b, dout, _, make = data(300, 12, seed)
+        return x, w, b, make(9, 12), make(300, 2), dout
+
+    graph = make_fx(step)(*inputs(1))
+    for got, want in zip(graph(*inputs(2)), step(*inputs(2))):
+        assert torch.equal(got, want)
+
+
 # ------------------------------------------------------------------------------------------------ a gradient of a gradient
 def test_gradient_of_a_very_long_sample_to_be_differentiated_again():
     """More rows than fp32 counts one by one, and a mean that is no zero."""

@@ -2,7 +2,9 @@
 // C++ because at the sizes of one resolution level a call through ctypes and Python autograd costs several times what
 // its kernels take (embedding with its gradient, smallest sizes: 97 us a pass there, 58 us here).
 //
-// Every call goes to the C entries of include/tsb200.h, on the current stream of the tensors' device.
+// Every call goes to the C entries of include/tsb200.h, on the current stream of the tensors' device.  All operators are
+// registered with torch's dispatcher, gradients included: what traces or records a program sees them, and not merely
+// the empty tensors that their kernels fill.
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
@@ -80,6 +82,12 @@ struct Call {
   tsb_stream_t stream() const { return c10::cuda::getCurrentCUDAStream().stream(); }
 };
 
+// the dispatcher's handle of an operator that is registered below
+template <typename Signature>
+c10::TypedOperatorHandle<Signature> registered(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Signature>();
+}
+
 bool wants_grad(std::initializer_list<Tensor> ts) {
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor& t : ts)
@@ -129,6 +137,11 @@ std::tuple<Tensor, Tensor> group_rows(const Tensor& keys, int64_t num_groups) {
   return {order, offsets};
 }
 
+std::tuple<Tensor, Tensor> call_group_rows(const Tensor& keys, int64_t num_groups) {
+  static const auto op = registered<decltype(group_rows)>("torchsparse_b200::group_rows");
+  return op.call(keys, num_groups);
+}
+
 std::tuple<Tensor, Tensor, Tensor> expert_sort(const Tensor& experts, int64_t num_experts) {
   need_cuda(experts);
   check_index(experts, "experts");
@@ -137,6 +150,11 @@ std::tuple<Tensor, Tensor, Tensor> expert_sort(const Tensor& experts, int64_t nu
   TORCH_CHECK_VALUE(shape[1] >= 1, "every row needs at least one choice");
   auto [order, offsets, inverse] = group(experts.reshape(-1), num_experts, at::IntArrayRef(shape, 2));
   return {order, inverse, offsets};
+}
+
+std::tuple<Tensor, Tensor, Tensor> call_expert_sort(const Tensor& experts, int64_t num_experts) {
+  static const auto op = registered<decltype(expert_sort)>("torchsparse_b200::expert_sort");
+  return op.call(experts, num_experts);
 }
 
 // ------------------------------------------------------------------------------------------------ group norm
@@ -209,9 +227,7 @@ Tensor group_mean(const Tensor& t, const Tensor& offsets, const std::optional<Te
 }
 
 Tensor call_group_mean(const Tensor& t, const Tensor& offsets, const std::optional<Tensor>& order, int64_t groups) {
-  static const auto op = c10::Dispatcher::singleton()
-                             .findSchemaOrThrow("torchsparse_b200::group_mean", "")
-                             .typed<Tensor(const Tensor&, const Tensor&, const std::optional<Tensor>&, int64_t)>();
+  static const auto op = registered<decltype(group_mean)>("torchsparse_b200::group_mean");
   return op.call(t, offsets, order, groups);
 }
 
@@ -263,28 +279,77 @@ Tensor norm_by_torch(const Tensor& x, const Tensor& w, const Tensor& b, const Te
   return at::where(inside, z, zero).to(x.scalar_type());
 }
 
+Tensor group_norm(const Tensor& feats, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, const Tensor& offsets,
+                  const std::optional<Tensor>& order, int64_t groups, double eps, int64_t act, double slope) {
+  const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor()), o = order.value_or(Tensor());
+  const int code = check_norm(feats, w, b, offsets, o, groups);
+  return norm_forward(packed(feats), packed(w), packed(b), offsets, o, NormArgs{groups, eps, slope, act}, code, false).first;
+}
+
+// with the means and reciprocal deviations that the gradient needs
+std::tuple<Tensor, Tensor> group_norm_stats(const Tensor& feats, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias,
+                                            const Tensor& offsets, const std::optional<Tensor>& order, int64_t groups, double eps,
+                                            int64_t act, double slope) {
+  const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor()), o = order.value_or(Tensor());
+  const int code = check_norm(feats, w, b, offsets, o, groups);
+  return norm_forward(packed(feats), packed(w), packed(b), offsets, o, NormArgs{groups, eps, slope, act}, code, true);
+}
+
+std::tuple<Tensor, Tensor, Tensor> group_norm_backward(const Tensor& grad, const Tensor& feats, const std::optional<Tensor>& weight,
+                                                       const std::optional<Tensor>& bias, const Tensor& offsets,
+                                                       const std::optional<Tensor>& order_, const Tensor& stats_, int64_t groups,
+                                                       int64_t act, double slope) {
+  const Tensor x = packed(feats), dy = packed(grad), w = packed(weight.value_or(Tensor())), b = packed(bias.value_or(Tensor()));
+  const Tensor order = order_.value_or(Tensor()), stats = packed(stats_);
+  const int code = check_norm(x, w, b, offsets, order, groups);
+  same_device(x, {dy, stats});
+  const int64_t n = x.size(0), c = x.size(1), samples = offsets.size(0) - 1;
+  TORCH_CHECK_VALUE(dy.sizes() == x.sizes() && dy.scalar_type() == x.scalar_type(), "the gradient is not like the features");
+  TORCH_CHECK_VALUE(stats.scalar_type() == at::kFloat && stats.numel() == 2 * samples * groups, "stats must be fp32 [2, ", samples, ", ",
+                    groups, "]");
+  Call call(x);
+  Tensor dx = at::empty_like(x), dw, db;
+  if (w.defined()) dw = at::empty_like(w);
+  if (b.defined()) db = at::empty_like(b);
+  const float* mean = stats.const_data_ptr<float>();
+  const int dtype = dtype_code(x);
+  void* ws = call.workspace(tsb_group_norm_bwd_workspace_bytes(n, c, groups, samples, dtype), x);
+  check_status(tsb_group_norm_bwd(ptr(x), ptr(dy), ints(order), ints(offsets), ptr(w), ptr(b), mean, mean + samples * groups, n, c,
+                                  groups, samples, (int)act, (float)slope, dtype, code, out_ptr(dx), out_ptr(dw), out_ptr(db), ws,
+                                  call.bytes, call.stream()),
+               "group_norm_backward");
+  return {dx, dw, db};
+}
+
+Tensor call_group_norm(const Tensor& feats, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias,
+                       const Tensor& offsets, const std::optional<Tensor>& order, int64_t groups, double eps, int64_t act,
+                       double slope) {
+  static const auto op = registered<decltype(group_norm)>("torchsparse_b200::group_norm");
+  return op.call(feats, weight, bias, offsets, order, groups, eps, act, slope);
+}
+
 struct GroupNorm : Function<GroupNorm> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias,
                         const Tensor& offsets, const std::optional<Tensor>& order, int64_t groups, double eps, int64_t act,
-                        double slope, int64_t p_code) {
-    const NormArgs a{groups, eps, slope, act};
-    const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor()), o = order.value_or(Tensor());
-    auto [y, stats] = norm_forward(x, w, b, offsets, o, a, (int)p_code, true);
-    ctx->save_for_backward({x, w, b, offsets, o, stats});
+                        double slope) {
+    static const auto op = registered<decltype(group_norm_stats)>("torchsparse_b200::group_norm_stats");
+    at::AutoDispatchBelowAutograd below;
+    auto [y, stats] = op.call(x, weight, bias, offsets, order, groups, eps, act, slope);
+    ctx->save_for_backward({x, weight.value_or(Tensor()), bias.value_or(Tensor()), offsets, order.value_or(Tensor()), stats});
     ctx->saved_data["groups"] = groups;
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["act"] = act;
     ctx->saved_data["slope"] = slope;
-    ctx->saved_data["code"] = p_code;
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1], &b = saved[2], &offsets = saved[3], &order = saved[4], &stats = saved[5];
-    const int64_t n = x.size(0), c = x.size(1), samples = offsets.size(0) - 1, groups = ctx->saved_data["groups"].toInt();
+    const NormArgs a{ctx->saved_data["groups"].toInt(), ctx->saved_data["eps"].toDouble(), ctx->saved_data["slope"].toDouble(),
+                     ctx->saved_data["act"].toInt()};
+    variable_list made(9);
     if (at::GradMode::is_enabled()) {
-      const NormArgs a{groups, ctx->saved_data["eps"].toDouble(), ctx->saved_data["slope"].toDouble(), ctx->saved_data["act"].toInt()};
-      variable_list wanted, made(10);
+      variable_list wanted;
       for (const Tensor* t : {&x, &w, &b})
         if (t->defined() && t->requires_grad()) wanted.push_back(*t);
       const auto got = torch::autograd::grad({norm_by_torch(x, w, b, offsets, order, a)}, wanted, {grads[0]}, /*retain_graph=*/true,
@@ -296,80 +361,98 @@ struct GroupNorm : Function<GroupNorm> {
       }
       return made;
     }
-    Call call(x);
-    const Tensor dy = grads[0].contiguous();
-    Tensor dx = at::empty_like(x), dw, db;
-    if (w.defined()) dw = at::empty_like(w);
-    if (b.defined()) db = at::empty_like(b);
-    const float* mean = stats.const_data_ptr<float>();
-    const int dtype = dtype_code(x);
-    void* ws = call.workspace(tsb_group_norm_bwd_workspace_bytes(n, c, groups, samples, dtype), x);
-    check_status(tsb_group_norm_bwd(ptr(x), ptr(dy), ints(order), ints(offsets), ptr(w), ptr(b), mean, mean + samples * groups, n, c,
-                                    groups, samples, (int)ctx->saved_data["act"].toInt(), (float)ctx->saved_data["slope"].toDouble(),
-                                    dtype, (int)ctx->saved_data["code"].toInt(), out_ptr(dx), out_ptr(dw), out_ptr(db), ws, call.bytes,
-                                    call.stream()),
-                 "group_norm_backward");
-    variable_list made{dx, dw, db};
-    made.resize(10);
+    static const auto op = registered<decltype(group_norm_backward)>("torchsparse_b200::group_norm_backward");
+    std::tie(made[0], made[1], made[2]) =
+        op.call(grads[0], x, given(w), given(b), offsets, given(order), stats, a.groups, a.act, a.slope);
     return made;
   }
 };
 
-Tensor group_norm(const Tensor& feats, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias, const Tensor& offsets,
-                  const std::optional<Tensor>& order, int64_t groups, double eps, int64_t act, double slope) {
-  const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor()), o = order.value_or(Tensor());
-  const int code = check_norm(feats, w, b, offsets, o, groups);
-  if (wants_grad({feats, w, b}))
-    return GroupNorm::apply(packed(feats), given(packed(w)), given(packed(b)), offsets, given(o), groups, eps, act, slope,
-                            (int64_t)code);
-  return norm_forward(packed(feats), packed(w), packed(b), offsets, o, NormArgs{groups, eps, slope, act}, code, false).first;
+Tensor group_norm_autograd(const Tensor& feats, const std::optional<Tensor>& weight, const std::optional<Tensor>& bias,
+                           const Tensor& offsets, const std::optional<Tensor>& order, int64_t groups, double eps, int64_t act,
+                           double slope) {
+  const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+  if (!wants_grad({feats, w, b})) {
+    at::AutoDispatchBelowAutograd below;
+    return call_group_norm(feats, weight, bias, offsets, order, groups, eps, act, slope);
+  }
+  check_norm(feats, w, b, offsets, order.value_or(Tensor()), groups);
+  return GroupNorm::apply(packed(feats), given(packed(w)), given(packed(b)), offsets, order, groups, eps, act, slope);
 }
 
 // ------------------------------------------------------------------------------------------------ embedding
-Tensor embedding_forward(const Tensor& table, const Tensor& indices, double scale) {
+void check_embedding(const Tensor& table, const Tensor& indices) {
+  same_device(table, {indices});
+  check_index(indices, "indices");
+  dtype_code(table);
+  TORCH_CHECK_VALUE(table.dim() == 2 && table.size(1) >= 1, "embedding expects a table [rows, channels], not ", table.sizes());
+}
+
+// padding: the row that gets no gradient, -1 for none
+Tensor embedding(const Tensor& table_, const Tensor& indices, double scale, int64_t /*padding*/) {
+  check_embedding(table_, indices);
+  const Tensor table = packed(table_), flat = (indices.dim() == 1 ? indices : indices.reshape(-1)).contiguous();
   Call call(table);
-  const int64_t n = indices.size(0), c = table.size(1);
+  const int64_t n = flat.size(0), c = table.size(1);
   Tensor out = at::empty({n, c}, table.options());
-  check_status(tsb_embedding_fwd(ptr(table), ptr(indices), indices.scalar_type() == at::kLong, n, table.size(0), c, (float)scale,
+  check_status(tsb_embedding_fwd(ptr(table), ptr(flat), flat.scalar_type() == at::kLong, n, table.size(0), c, (float)scale,
                                  dtype_code(table), out_ptr(out), call.stream()),
                "embedding");
-  return out;
+  if (indices.dim() == 1) return out;
+  auto shape = indices.sizes().vec();
+  shape.push_back(c);
+  return out.view(shape);
+}
+
+Tensor embedding_backward(const Tensor& grad, const Tensor& indices, int64_t rows, double scale, int64_t padding) {
+  same_device(grad, {indices});
+  check_index(indices, "indices");
+  TORCH_CHECK_VALUE(grad.dim() == indices.dim() + 1 && grad.sizes().slice(0, indices.dim()) == indices.sizes() && grad.size(-1) >= 1 &&
+                        rows >= 0,
+                    "the gradient is not like the vectors of the indices");
+  const int64_t n = indices.numel(), c = grad.size(-1);
+  const Tensor dy = grad.contiguous(), flat = indices.contiguous();
+  Call call(dy);
+  Tensor dtable = at::empty({rows, c}, dy.options());
+  const int dtype = dtype_code(dy);
+  void* ws = call.workspace(tsb_embedding_bwd_workspace_bytes(n, rows, c, dtype), dy);
+  check_status(tsb_embedding_bwd(ptr(dy), ptr(flat), flat.scalar_type() == at::kLong, n, rows, c, (float)scale, padding, dtype,
+                                 out_ptr(dtable), ws, call.bytes, call.stream()),
+               "embedding_backward");
+  return dtable;
+}
+
+Tensor call_embedding(const Tensor& table, const Tensor& indices, double scale, int64_t padding) {
+  static const auto op = registered<decltype(embedding)>("torchsparse_b200::embedding");
+  return op.call(table, indices, scale, padding);
 }
 
 struct Embedding : Function<Embedding> {
   static Tensor forward(AutogradContext* ctx, const Tensor& table, const Tensor& indices, double scale, int64_t padding) {
+    at::AutoDispatchBelowAutograd below;
     ctx->save_for_backward({indices});
     ctx->saved_data["rows"] = table.size(0);
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["padding"] = padding;
-    return embedding_forward(table, indices, scale);
+    return call_embedding(table, indices, scale, padding);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    const Tensor indices = ctx->get_saved_variables()[0], dy = grads[0].contiguous();
-    const int64_t n = indices.size(0), rows = ctx->saved_data["rows"].toInt(), c = dy.size(1);
-    Call call(dy);
-    Tensor dtable = at::empty({rows, c}, dy.options());
-    const int dtype = dtype_code(dy);
-    void* ws = call.workspace(tsb_embedding_bwd_workspace_bytes(n, rows, c, dtype), dy);
-    check_status(tsb_embedding_bwd(ptr(dy), ptr(indices), indices.scalar_type() == at::kLong, n, rows, c,
-                                   (float)ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt(), dtype,
-                                   out_ptr(dtable), ws, call.bytes, call.stream()),
-                 "embedding_backward");
-    auto made = once({dtable});
+    static const auto op = registered<decltype(embedding_backward)>("torchsparse_b200::embedding_backward");
+    auto made = once({op.call(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["rows"].toInt(),
+                              ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt())});
     made.resize(4);
     return made;
   }
 };
 
-// padding: the row that gets no gradient, -1 for none
-Tensor embedding(const Tensor& table, const Tensor& indices, double scale, int64_t padding) {
-  same_device(table, {indices});
-  check_index(indices, "indices");
-  dtype_code(table);
-  TORCH_CHECK_VALUE(table.dim() == 2 && table.size(1) >= 1, "embedding expects a table [rows, channels], not ", table.sizes());
+Tensor embedding_autograd(const Tensor& table, const Tensor& indices, double scale, int64_t padding) {
+  if (!wants_grad({table})) {
+    at::AutoDispatchBelowAutograd below;
+    return call_embedding(table, indices, scale, padding);
+  }
+  check_embedding(table, indices);
   const Tensor flat = (indices.dim() == 1 ? indices : indices.reshape(-1)).contiguous();
-  const Tensor out = wants_grad({table}) ? Embedding::apply(packed(table), flat, scale, padding)
-                                         : embedding_forward(packed(table), flat, scale);
+  const Tensor out = Embedding::apply(packed(table), flat, scale, padding);
   if (indices.dim() == 1) return out;
   auto shape = indices.sizes().vec();
   shape.push_back(table.size(1));
@@ -387,17 +470,36 @@ std::tuple<int64_t, int32_t, const int32_t*> plan(const Tensor& inverse, const T
   return {inverse.size(0), (int32_t)inverse.size(1), ints(offsets) + offsets.size(0) - 1};
 }
 
-Tensor dispatch(const Tensor& x, const Tensor& inverse, const Tensor& offsets) {
+Tensor expert_dispatch(const Tensor& feats, const Tensor& inverse, const Tensor& offsets) {
+  same_device(feats, {inverse, offsets});
   const auto [n, k, kept] = plan(inverse, offsets);
+  TORCH_CHECK_VALUE(feats.dim() == 2 && feats.size(0) == n && feats.size(1) >= 1, "expert_dispatch expects features [", n, ", C], not ",
+                    feats.sizes());
+  const int dtype = dtype_code(feats);
+  const Tensor x = packed(feats);
   Call call(x);
   Tensor out = at::empty({n * k, x.size(1)}, x.options());
-  check_status(tsb_expert_dispatch(ptr(x), ints(inverse), kept, n, k, x.size(1), dtype_code(x), out_ptr(out), call.stream()),
+  check_status(tsb_expert_dispatch(ptr(x), ints(inverse), kept, n, k, x.size(1), dtype, out_ptr(out), call.stream()),
                "expert_dispatch");
   return out;
 }
 
-Tensor combine(const Tensor& rows, const Tensor& weights, const Tensor& inverse, const Tensor& offsets) {
+void check_combine(const Tensor& rows, const Tensor& weights, int64_t n, int64_t k) {
+  TORCH_CHECK_VALUE(rows.dim() == 2 && rows.size(0) == n * k && rows.size(1) >= 1, "expert_combine expects sorted rows [", n * k,
+                    ", C], not ", rows.sizes());
+  dtype_code(rows);
+  if (!weights.defined()) return;
+  TORCH_CHECK_VALUE(weights.dim() == 2 && weights.size(0) == n && weights.size(1) == k, "expert_combine expects weights [", n, ", ", k,
+                    "], not ", weights.sizes());
+  dtype_code(weights);
+}
+
+// no weights: 1
+Tensor expert_combine(const Tensor& feats, const std::optional<Tensor>& weights_, const Tensor& inverse, const Tensor& offsets) {
+  const Tensor rows = packed(feats), weights = packed(weights_.value_or(Tensor()));
+  same_device(rows, {weights, inverse, offsets});
   const auto [n, k, kept] = plan(inverse, offsets);
+  check_combine(rows, weights, n, k);
   Call call(rows);
   Tensor out = at::empty({n, rows.size(1)}, rows.options());
   check_status(tsb_expert_combine(ptr(rows), ptr(weights), weights.defined() ? dtype_code(weights) : (int)TSB_F32, ints(inverse), kept,
@@ -406,14 +508,46 @@ Tensor combine(const Tensor& rows, const Tensor& weights, const Tensor& inverse,
   return out;
 }
 
+std::tuple<Tensor, Tensor> expert_combine_backward(const Tensor& grad, const Tensor& feats, const Tensor& weights_,
+                                                   const Tensor& inverse, const Tensor& offsets) {
+  const Tensor dout = packed(grad), rows = packed(feats), weights = packed(weights_);
+  same_device(rows, {dout, weights, inverse, offsets});
+  const auto [n, k, kept] = plan(inverse, offsets);
+  check_combine(rows, weights, n, k);
+  TORCH_CHECK_VALUE(dout.dim() == 2 && dout.size(0) == n && dout.size(1) == rows.size(1) && dout.scalar_type() == rows.scalar_type(),
+                    "the gradient is not like the sums of the rows");
+  Call call(rows);
+  Tensor drows = at::empty_like(rows), dweights = at::empty_like(weights);
+  check_status(tsb_expert_combine_bwd(ptr(dout), ptr(rows), ptr(weights), dtype_code(weights), ints(inverse), kept, n, k, rows.size(1),
+                                      dtype_code(rows), out_ptr(drows), out_ptr(dweights), call.stream()),
+               "expert_combine_backward");
+  return {drows, dweights};
+}
+
+Tensor call_expert_dispatch(const Tensor& feats, const Tensor& inverse, const Tensor& offsets) {
+  static const auto op = registered<decltype(expert_dispatch)>("torchsparse_b200::expert_dispatch");
+  return op.call(feats, inverse, offsets);
+}
+
+Tensor call_expert_combine(const Tensor& feats, const std::optional<Tensor>& weights, const Tensor& inverse, const Tensor& offsets) {
+  static const auto op = registered<decltype(expert_combine)>("torchsparse_b200::expert_combine");
+  return op.call(feats, weights, inverse, offsets);
+}
+
 struct Dispatch : Function<Dispatch> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& inverse, const Tensor& offsets) {
+    at::AutoDispatchBelowAutograd below;
     ctx->save_for_backward({inverse, offsets});
-    return dispatch(x, inverse, offsets);
+    return call_expert_dispatch(x, inverse, offsets);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    auto made = once({combine(grads[0].contiguous(), Tensor(), saved[0], saved[1])});
+    Tensor dx;
+    {
+      at::AutoDispatchBelowAutograd below;
+      dx = call_expert_combine(grads[0], std::nullopt, saved[0], saved[1]);
+    }
+    auto made = once({dx});
     made.resize(3);
     return made;
   }
@@ -421,60 +555,87 @@ struct Dispatch : Function<Dispatch> {
 
 struct Combine : Function<Combine> {
   static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& weights, const Tensor& inverse, const Tensor& offsets) {
+    at::AutoDispatchBelowAutograd below;
     ctx->save_for_backward({rows, weights, inverse, offsets});
-    return combine(rows, weights, inverse, offsets);
+    return call_expert_combine(rows, weights, inverse, offsets);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    static const auto op = registered<decltype(expert_combine_backward)>("torchsparse_b200::expert_combine_backward");
     const auto saved = ctx->get_saved_variables();
-    const Tensor &rows = saved[0], &weights = saved[1], dout = grads[0].contiguous();
-    const auto [n, k, kept] = plan(saved[2], saved[3]);
-    Call call(rows);
-    Tensor drows = at::empty_like(rows), dweights = at::empty_like(weights);
-    check_status(tsb_expert_combine_bwd(ptr(dout), ptr(rows), ptr(weights), dtype_code(weights), ints(saved[2]), kept, n, k,
-                                        rows.size(1), dtype_code(rows), out_ptr(drows), out_ptr(dweights), call.stream()),
-                 "expert_combine_backward");
+    auto [drows, dweights] = op.call(grads[0], saved[0], saved[1], saved[2], saved[3]);
     auto made = once({drows, dweights});
     made.resize(4);
     return made;
   }
 };
 
-Tensor expert_dispatch(const Tensor& x, const Tensor& inverse, const Tensor& offsets) {
-  same_device(x, {inverse, offsets});
-  const int64_t n = std::get<0>(plan(inverse, offsets));
-  TORCH_CHECK_VALUE(x.dim() == 2 && x.size(0) == n && x.size(1) >= 1, "expert_dispatch expects features [", n, ", C], not ", x.sizes());
-  dtype_code(x);
-  return wants_grad({x}) ? Dispatch::apply(packed(x), inverse, offsets) : dispatch(packed(x), inverse, offsets);
+Tensor expert_dispatch_autograd(const Tensor& feats, const Tensor& inverse, const Tensor& offsets) {
+  if (wants_grad({feats})) return Dispatch::apply(packed(feats), inverse, offsets);
+  at::AutoDispatchBelowAutograd below;
+  return call_expert_dispatch(feats, inverse, offsets);
 }
 
-Tensor expert_combine(const Tensor& rows, const Tensor& weights, const Tensor& inverse, const Tensor& offsets) {
-  same_device(rows, {weights, inverse, offsets});
-  const auto [n, k, kept] = plan(inverse, offsets);
-  TORCH_CHECK_VALUE(rows.dim() == 2 && rows.size(0) == n * k && rows.size(1) >= 1, "expert_combine expects sorted rows [", n * k,
-                    ", C], not ", rows.sizes());
-  TORCH_CHECK_VALUE(weights.dim() == 2 && weights.size(0) == n && weights.size(1) == k, "expert_combine expects weights [", n, ", ", k,
-                    "], not ", weights.sizes());
-  dtype_code(rows);
-  dtype_code(weights);
-  return wants_grad({rows, weights}) ? Combine::apply(packed(rows), packed(weights), inverse, offsets)
-                                     : combine(packed(rows), packed(weights), inverse, offsets);
+Tensor expert_combine_autograd(const Tensor& feats, const std::optional<Tensor>& weights, const Tensor& inverse,
+                               const Tensor& offsets) {
+  if (wants_grad({feats, weights.value_or(Tensor())})) {
+    TORCH_CHECK(weights.has_value(), "expert_combine without weights has no gradient");
+    return Combine::apply(packed(feats), packed(*weights), inverse, offsets);
+  }
+  at::AutoDispatchBelowAutograd below;
+  return call_expert_combine(feats, weights, inverse, offsets);
 }
 
 }  // namespace
 
 TORCH_LIBRARY(torchsparse_b200, m) {
+  m.def("group_rows(Tensor keys, int num_groups) -> (Tensor, Tensor)");
+  m.def("expert_sort(Tensor experts, int num_experts) -> (Tensor, Tensor, Tensor)");
   m.def("group_mean(Tensor t, Tensor offsets, Tensor? order, int groups) -> Tensor");
+  m.def("group_norm(Tensor feats, Tensor? weight, Tensor? bias, Tensor offsets, Tensor? order, int groups, float eps, int act, "
+        "float slope) -> Tensor");
+  m.def("group_norm_stats(Tensor feats, Tensor? weight, Tensor? bias, Tensor offsets, Tensor? order, int groups, float eps, int act, "
+        "float slope) -> (Tensor, Tensor)");
+  m.def("group_norm_backward(Tensor grad, Tensor feats, Tensor? weight, Tensor? bias, Tensor offsets, Tensor? order, Tensor stats, "
+        "int groups, int act, float slope) -> (Tensor, Tensor, Tensor)");
+  m.def("embedding(Tensor table, Tensor indices, float scale, int padding) -> Tensor");
+  m.def("embedding_backward(Tensor grad, Tensor indices, int rows, float scale, int padding) -> Tensor");
+  m.def("expert_dispatch(Tensor feats, Tensor inverse, Tensor offsets) -> Tensor");
+  m.def("expert_combine(Tensor feats, Tensor? weights, Tensor inverse, Tensor offsets) -> Tensor");
+  m.def("expert_combine_backward(Tensor grad, Tensor feats, Tensor weights, Tensor inverse, Tensor offsets) -> (Tensor, Tensor)");
 }
 
-TORCH_LIBRARY_IMPL(torchsparse_b200, CompositeExplicitAutograd, m) { m.impl("group_mean", &group_mean); }
+TORCH_LIBRARY_IMPL(torchsparse_b200, CompositeExplicitAutograd, m) {
+  m.impl("group_rows", &group_rows);
+  m.impl("expert_sort", &expert_sort);
+  m.impl("group_mean", &group_mean);
+  m.impl("group_norm", &group_norm);
+  m.impl("group_norm_stats", &group_norm_stats);
+  m.impl("group_norm_backward", &group_norm_backward);
+  m.impl("embedding", &embedding);
+  m.impl("embedding_backward", &embedding_backward);
+  m.impl("expert_dispatch", &expert_dispatch);
+  m.impl("expert_combine", &expert_combine);
+  m.impl("expert_combine_backward", &expert_combine_backward);
+}
 
-TORCH_LIBRARY_IMPL(torchsparse_b200, Autograd, m) { m.impl("group_mean", &group_mean_autograd); }
+TORCH_LIBRARY_IMPL(torchsparse_b200, Autograd, m) {
+  m.impl("group_mean", &group_mean_autograd);
+  m.impl("group_norm", &group_norm_autograd);
+  m.impl("embedding", &embedding_autograd);
+  m.impl("expert_dispatch", &expert_dispatch_autograd);
+  m.impl("expert_combine", &expert_combine_autograd);
+  for (const char* name : {"group_rows", "expert_sort"}) m.impl(name, torch::CppFunction::makeFallthrough());      // integers only
+  for (const char* name : {"group_norm_stats", "group_norm_backward", "embedding_backward", "expert_combine_backward"})
+    m.impl(name, torch::CppFunction::makeFallthrough());      // parts of the nodes above, which are what autograd sees
+}
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-  m.def("group_rows", &group_rows);
-  m.def("expert_sort", &expert_sort);
-  m.def("group_norm", &group_norm);
-  m.def("embedding", &embedding);
-  m.def("expert_dispatch", &expert_dispatch);
-  m.def("expert_combine", &expert_combine);
+  m.def("group_rows", &call_group_rows);
+  m.def("expert_sort", &call_expert_sort);
+  m.def("group_norm", &call_group_norm);
+  m.def("embedding", &call_embedding);
+  m.def("expert_dispatch", &call_expert_dispatch);
+  m.def("expert_combine", [](const Tensor& feats, const Tensor& weights, const Tensor& inverse, const Tensor& offsets) {
+    return call_expert_combine(feats, weights, inverse, offsets);
+  });
 }
