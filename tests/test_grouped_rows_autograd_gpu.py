@@ -12,7 +12,7 @@ pytestmark = pytest.mark.gpu
 
 FIRST, SECOND = 2e-5, 1e-4
 ACTS = {None: lambda t: t, "relu": torch.relu, "leaky_relu": lambda t: torch.nn.functional.leaky_relu(t, 0.1),
-        "silu": torch.nn.functional.silu}
+        "silu": lambda t: t * torch.sigmoid(t)}
 
 
 def definition(x, w, b, cuts, order, groups, act, eps=1e-5):
@@ -189,3 +189,79 @@ def test_second_derivative_with_an_order_that_is_no_permutation(n):
     second = torch.autograd.grad(first[0].square().sum(), leaves)
     for t in (*first, *second):
         assert bool(t.isfinite().all())
+
+
+# ------------------------------------------------------------------------------------------------ forward-mode tangents
+@pytest.mark.parametrize("ordered", [False, True])
+@pytest.mark.parametrize("recorded", ["off", "frozen", "trained"])
+def test_tangents_of_group_norm(ordered, recorded):
+    import torch.autograd.forward_ad as fwAD
+
+    from torchsparse_b200.nn import functional as F
+
+    cuts = [3, 5000, 5000, 9001]
+    x, w, b, _, order, make = data(9010, 12, 5, None if ordered else 1)
+    tangents = [make(*t.shape) for t in (x, w, b)]
+    if recorded == "trained":
+        w.requires_grad_()
+        b.requires_grad_()
+    for which in ((0,), (1, 2), (0, 1, 2)):
+        with torch.set_grad_enabled(recorded != "off"), fwAD.dual_level():
+            args = [fwAD.make_dual(t, d) if i in which else t for i, (t, d) in enumerate(zip((x, w, b), tangents))]
+            y = F.group_norm(args[0], ints(cuts), 3, args[1], args[2], activation="silu", order=order)
+            got = fwAD.unpack_dual(y).tangent
+            assert got is not None
+        wide = [t.detach().double() for t in (x, w, b)]
+        moved = [d.double() if i in which else torch.zeros_like(d).double() for i, d in enumerate(tangents)]
+        _, want = torch.func.jvp(lambda *a: definition(*a, cuts, order, 3, "silu"), tuple(wide), tuple(moved))
+        near(got, want, FIRST)
+
+
+def test_tangents_of_embedding_and_expert_rows():
+    import torch.autograd.forward_ad as fwAD
+
+    from torchsparse_b200.nn import functional as F
+
+    g = torch.Generator(device="cuda").manual_seed(6)
+    make = lambda *s: torch.randn(*s, generator=g, device="cuda")      # noqa: E731
+    tokens = torch.randint(-1, 9, (200,), generator=g, device="cuda")
+    rows = F.expert_sort(torch.randint(-1, 4, (200, 2), generator=g, device="cuda"), 4)
+    table, x, ys, gate = make(9, 16), make(200, 16), make(400, 16), make(200, 2)
+    for record in (False, True):
+        leaves = [t.clone().requires_grad_(record) for t in (table, x, ys, gate)]
+        t_table, t_x, t_ys, t_gate = (make(*t.shape) for t in leaves)
+        with fwAD.dual_level():
+            dual = fwAD.make_dual
+            tangent = lambda t: fwAD.unpack_dual(t).tangent      # noqa: E731
+            table_, x_, ys_, gate_ = leaves
+            assert torch.equal(tangent(F.embedding(tokens, dual(table_, t_table), 2.0)), F.embedding(tokens, t_table, 2.0))
+            assert torch.equal(tangent(F.expert_dispatch(dual(x_, t_x), rows)), F.expert_dispatch(t_x, rows))
+            by_rows, by_gate = F.expert_combine(t_ys, gate, rows), F.expert_combine(ys, t_gate, rows)
+            assert torch.equal(tangent(F.expert_combine(dual(ys_, t_ys), gate_, rows)), by_rows)
+            assert torch.equal(tangent(F.expert_combine(ys_, dual(gate_, t_gate), rows)), by_gate)
+            both = F.expert_combine(dual(ys_, t_ys), dual(gate_, t_gate), rows)
+            assert torch.equal(tangent(both), by_rows + by_gate)
+            if record:      # a gradient of the values next to the tangents
+                (got,) = torch.autograd.grad(fwAD.unpack_dual(both).primal.sum(), gate_)
+                assert torch.equal(got, torch.autograd.grad(F.expert_combine(ys_, gate_, rows).sum(), gate_)[0])
+
+
+def test_a_tangent_in_a_gradient_is_carried_or_refused():
+    import torch.autograd.forward_ad as fwAD
+
+    from torchsparse_b200.nn import functional as F
+
+    x, w, b, dy, _, make = data(300, 12, 7)
+    tokens = torch.randint(0, 9, (300,), generator=torch.Generator().manual_seed(7)).cuda()
+    rows = F.expert_sort(tokens, 9)
+    leaf, t_dy = x.clone().requires_grad_(), make(300, 12)
+    y = F.group_norm(leaf, ints([0, 300]), 3, w, b, activation="silu")
+    wide = x.double().requires_grad_()
+    (want,) = torch.autograd.grad(definition(wide, w.double(), b.double(), [0, 300], None, 3, "silu"), wide, t_dy.double())
+    with fwAD.dual_level():
+        (dx,) = torch.autograd.grad(y, leaf, fwAD.make_dual(dy, t_dy))
+        near(fwAD.unpack_dual(dx).tangent, want, FIRST)      # linear in dy
+        table, gate = make(9, 12).requires_grad_(), make(300, 1).requires_grad_()
+        for out in (F.embedding(tokens, table), F.expert_dispatch(leaf, rows), F.expert_combine(leaf, gate, rows)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(out, [t for t in (table, leaf, gate)], fwAD.make_dual(dy, t_dy), allow_unused=True)

@@ -95,6 +95,16 @@ bool wants_grad(std::initializer_list<Tensor> ts) {
   return false;
 }
 
+// Forward-mode differentiation: the tangent that goes with a tensor, and values put together with theirs.
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+Tensor tangent(const Tensor& t) { return t._fw_grad(/*level=*/0); }
+Tensor primal(const Tensor& t) { return has_tangent(t) ? t._fw_primal(/*level=*/0) : t; }
+Tensor dual(const Tensor& value, const Tensor& tangent) { return at::_make_dual(value, tangent, /*level=*/0); }
+
+void refuse_tangent(const Tensor& grad) {
+  TORCH_CHECK(!has_tangent(grad), "the gradient of this operator of torchsparse_b200 has no forward-mode derivative");
+}
+
 // What a backward call returns: its kernels have no gradient of their own, and asking for one is an error, not a zero.
 variable_list once(variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -262,11 +272,12 @@ Tensor group_mean_autograd(const Tensor& t, const Tensor& offsets, const std::op
     mean = call_group_mean(t, offsets, order, groups);
   }
   if (node) torch::autograd::set_history(mean, node);
+  if (has_tangent(t)) mean._set_fw_grad(call_group_mean(tangent(t), offsets, order, groups), /*level=*/0, /*is_inplace_op=*/false);
   return mean;
 }
 
-// The same in torch's own operations and group_mean, for a gradient that is to be differentiated again (a gradient penalty):
-// slower, and differentiable as often as wanted.
+// The same in torch's own operations and group_mean, for a gradient that is to be differentiated again (a gradient penalty) and
+// for forward-mode tangents: slower, and differentiable as often as wanted.
 Tensor norm_by_torch(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& offsets, const Tensor& order, const NormArgs& a) {
   const Tensor inside = row_samples(offsets, order, x.size(0)).lt(offsets.size(0) - 1).unsqueeze(1);
   const auto mean = [&](const Tensor& t) { return call_group_mean(t, offsets, given(order), a.groups); };
@@ -275,7 +286,7 @@ Tensor norm_by_torch(const Tensor& x, const Tensor& w, const Tensor& b, const Te
   Tensor z = d * (mean(d * d) + a.eps).rsqrt();
   if (w.defined()) z = z * w.to(at::kFloat);
   if (b.defined()) z = z + b.to(at::kFloat);
-  z = a.act == 1 ? at::relu(z) : a.act == 2 ? at::leaky_relu(z, a.slope) : a.act == 3 ? at::silu(z) : z;
+  z = a.act == 1 ? at::relu(z) : a.act == 2 ? at::leaky_relu(z, a.slope) : a.act == 3 ? z * at::sigmoid(z) : z;      // silu's gradient has no tangent
   return at::where(inside, z, zero).to(x.scalar_type());
 }
 
@@ -348,12 +359,14 @@ struct GroupNorm : Function<GroupNorm> {
     const NormArgs a{ctx->saved_data["groups"].toInt(), ctx->saved_data["eps"].toDouble(), ctx->saved_data["slope"].toDouble(),
                      ctx->saved_data["act"].toInt()};
     variable_list made(9);
-    if (at::GradMode::is_enabled()) {
+    const bool again = at::GradMode::is_enabled();
+    if (again || has_tangent(grads[0])) {
+      at::AutoGradMode record(true);
       variable_list wanted;
       for (const Tensor* t : {&x, &w, &b})
         if (t->defined() && t->requires_grad()) wanted.push_back(*t);
-      const auto got = torch::autograd::grad({norm_by_torch(x, w, b, offsets, order, a)}, wanted, {grads[0]}, /*retain_graph=*/true,
-                                             /*create_graph=*/true, /*allow_unused=*/true);
+      const auto got = torch::autograd::grad({norm_by_torch(x, w, b, offsets, order, a)}, wanted, {grads[0]}, /*retain_graph=*/again,
+                                             /*create_graph=*/again, /*allow_unused=*/true);
       size_t k = 0, i = 0;
       for (const Tensor* t : {&x, &w, &b}) {
         if (t->defined() && t->requires_grad()) made[i] = got[k++];
@@ -372,6 +385,10 @@ Tensor group_norm_autograd(const Tensor& feats, const std::optional<Tensor>& wei
                            const Tensor& offsets, const std::optional<Tensor>& order, int64_t groups, double eps, int64_t act,
                            double slope) {
   const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+  if (has_tangent(feats) || has_tangent(w) || has_tangent(b)) {
+    check_norm(feats, w, b, offsets, order.value_or(Tensor()), groups);
+    return norm_by_torch(feats, w, b, offsets, order.value_or(Tensor()), NormArgs{groups, eps, slope, act});
+  }
   if (!wants_grad({feats, w, b})) {
     at::AutoDispatchBelowAutograd below;
     return call_group_norm(feats, weight, bias, offsets, order, groups, eps, act, slope);
@@ -438,6 +455,7 @@ struct Embedding : Function<Embedding> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     static const auto op = registered<decltype(embedding_backward)>("torchsparse_b200::embedding_backward");
+    refuse_tangent(grads[0]);
     auto made = once({op.call(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["rows"].toInt(),
                               ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt())});
     made.resize(4);
@@ -446,6 +464,8 @@ struct Embedding : Function<Embedding> {
 };
 
 Tensor embedding_autograd(const Tensor& table, const Tensor& indices, double scale, int64_t padding) {
+  if (has_tangent(table))      // linear
+    return dual(call_embedding(primal(table), indices, scale, padding), call_embedding(tangent(table), indices, scale, padding));
   if (!wants_grad({table})) {
     at::AutoDispatchBelowAutograd below;
     return call_embedding(table, indices, scale, padding);
@@ -542,6 +562,7 @@ struct Dispatch : Function<Dispatch> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
+    refuse_tangent(grads[0]);
     Tensor dx;
     {
       at::AutoDispatchBelowAutograd below;
@@ -562,6 +583,7 @@ struct Combine : Function<Combine> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     static const auto op = registered<decltype(expert_combine_backward)>("torchsparse_b200::expert_combine_backward");
     const auto saved = ctx->get_saved_variables();
+    refuse_tangent(grads[0]);
     auto [drows, dweights] = op.call(grads[0], saved[0], saved[1], saved[2], saved[3]);
     auto made = once({drows, dweights});
     made.resize(4);
@@ -570,6 +592,8 @@ struct Combine : Function<Combine> {
 };
 
 Tensor expert_dispatch_autograd(const Tensor& feats, const Tensor& inverse, const Tensor& offsets) {
+  if (has_tangent(feats))      // linear
+    return dual(call_expert_dispatch(primal(feats), inverse, offsets), call_expert_dispatch(tangent(feats), inverse, offsets));
   if (wants_grad({feats})) return Dispatch::apply(packed(feats), inverse, offsets);
   at::AutoDispatchBelowAutograd below;
   return call_expert_dispatch(feats, inverse, offsets);
@@ -577,6 +601,18 @@ Tensor expert_dispatch_autograd(const Tensor& feats, const Tensor& inverse, cons
 
 Tensor expert_combine_autograd(const Tensor& feats, const std::optional<Tensor>& weights, const Tensor& inverse,
                                const Tensor& offsets) {
+  const bool moves = has_tangent(feats), weighs = weights.has_value() && has_tangent(*weights);
+  if (moves || weighs) {      // linear in both
+    const std::optional<Tensor> w = weights.has_value() ? std::optional<Tensor>(primal(*weights)) : std::nullopt;
+    const Tensor rows = primal(feats);
+    Tensor t;
+    if (moves) t = call_expert_combine(tangent(feats), w, inverse, offsets);
+    if (weighs) {
+      const Tensor by_weights = call_expert_combine(rows, tangent(*weights), inverse, offsets);
+      t = t.defined() ? t + by_weights : by_weights;
+    }
+    return dual(call_expert_combine(rows, w, inverse, offsets), t);
+  }
   if (wants_grad({feats, weights.value_or(Tensor())})) {
     TORCH_CHECK(weights.has_value(), "expert_combine without weights has no gradient");
     return Combine::apply(packed(feats), packed(*weights), inverse, offsets);
