@@ -265,3 +265,46 @@ def test_a_tangent_in_a_gradient_is_carried_or_refused():
         for out in (F.embedding(tokens, table), F.expert_dispatch(leaf, rows), F.expert_combine(leaf, gate, rows)):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 torch.autograd.grad(out, [t for t in (table, leaf, gate)], fwAD.make_dual(dy, t_dy), allow_unused=True)
+
+
+# ------------------------------------------------------------------------------------------------ functional transforms
+def _layer():
+    import torchsparse_b200 as ts
+    from torchsparse_b200 import nn as spnn
+
+    m = spnn.GroupNorm(3, 12, activation="silu").cuda()
+    coords = torch.randint(0, 9, (600, 4), generator=torch.Generator().manual_seed(0)).int().cuda()
+    coords[:, 0] = torch.arange(600, device="cuda") % 2
+    order = torch.cat([torch.arange(0, 600, 2), torch.arange(1, 600, 2)]).int().cuda()
+
+    def run(x, w, b):
+        return torch.func.functional_call(m, {"weight": w, "bias": b}, (ts.SparseTensor(x, coords),)).feats
+
+    return run, lambda *a: definition(*a, [0, 300, 600], order, 3, "silu")
+
+
+def test_functional_gradient_jvp_and_hessian_product_of_a_norm_layer():
+    run, plain = _layer()
+    x, w, b, dy, _, make = data(600, 12, 8)
+    wide = tuple(t.double() for t in (x, w, b))
+    loss = lambda f, out: lambda *a: (f(*a) * out).sum()      # noqa: E731
+    got = torch.func.grad(loss(run, dy), (0, 1, 2))(x, w, b)
+    want = torch.func.grad(loss(plain, dy.double()), (0, 1, 2))(*wide)
+    for a, e in zip(got, want):
+        near(a, e, FIRST)
+    moved = tuple(make(*t.shape) for t in (x, w, b))
+    near(torch.func.jvp(run, (x, w, b), moved)[1], torch.func.jvp(plain, wide, tuple(t.double() for t in moved))[1], FIRST)
+    got = torch.func.jvp(torch.func.grad(loss(run, dy), (0, 1, 2)), (x, w, b), moved)[1]
+    want = torch.func.jvp(torch.func.grad(loss(plain, dy.double()), (0, 1, 2)), wide, tuple(t.double() for t in moved))[1]
+    for a, e in zip(got, want):
+        near(a, e, SECOND)
+
+
+def test_vmap_over_a_norm_layer():
+    run, _ = _layer()
+    x, w, b, dy, _, make = data(600, 12, 9)
+    xs = make(3, 600, 12)
+    assert torch.equal(torch.func.vmap(lambda t: run(t, w, b))(xs), torch.stack([run(t, w, b) for t in xs]))
+    got = torch.func.vmap(torch.func.grad(lambda t: (run(t, w, b) * dy).sum()))(xs)
+    for a, t in zip(got, xs):
+        near(a, torch.func.grad(lambda u: (run(u, w, b) * dy).sum())(t).double(), FIRST)

@@ -95,6 +95,9 @@ bool wants_grad(std::initializer_list<Tensor> ts) {
   return false;
 }
 
+// Inside torch.func.grad and its like, which take torch's own operations and no C++ Function.
+bool in_transform() { return c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerBackMode); }
+
 // Forward-mode differentiation: the tangent that goes with a tensor, and values put together with theirs.
 bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
 Tensor tangent(const Tensor& t) { return t._fw_grad(/*level=*/0); }
@@ -277,7 +280,7 @@ Tensor group_mean_autograd(const Tensor& t, const Tensor& offsets, const std::op
 }
 
 // The same in torch's own operations and group_mean, for a gradient that is to be differentiated again (a gradient penalty) and
-// for forward-mode tangents: slower, and differentiable as often as wanted.
+// for forward-mode tangents and functional transforms: slower, and differentiable as often as wanted.
 Tensor norm_by_torch(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& offsets, const Tensor& order, const NormArgs& a) {
   const Tensor inside = row_samples(offsets, order, x.size(0)).lt(offsets.size(0) - 1).unsqueeze(1);
   const auto mean = [&](const Tensor& t) { return call_group_mean(t, offsets, given(order), a.groups); };
@@ -385,11 +388,12 @@ Tensor group_norm_autograd(const Tensor& feats, const std::optional<Tensor>& wei
                            const Tensor& offsets, const std::optional<Tensor>& order, int64_t groups, double eps, int64_t act,
                            double slope) {
   const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
-  if (has_tangent(feats) || has_tangent(w) || has_tangent(b)) {
+  const bool wanted = wants_grad({feats, w, b});
+  if (has_tangent(feats) || has_tangent(w) || has_tangent(b) || (wanted && in_transform())) {
     check_norm(feats, w, b, offsets, order.value_or(Tensor()), groups);
     return norm_by_torch(feats, w, b, offsets, order.value_or(Tensor()), NormArgs{groups, eps, slope, act});
   }
-  if (!wants_grad({feats, w, b})) {
+  if (!wanted) {
     at::AutoDispatchBelowAutograd below;
     return call_group_norm(feats, weight, bias, offsets, order, groups, eps, act, slope);
   }
