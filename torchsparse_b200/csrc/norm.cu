@@ -988,7 +988,7 @@ __global__ void __launch_bounds__(kSmallThreads) norm_small_grad_kernel(Norm a, 
         v += f.y;
       }
     }
-    v *= rstd;
+    v = hi > lo ? v * rstd : 0.f;      // an empty sample has no deviation: with eps = 0 its rstd is infinite
     const int ch = gr * a.d + k;
     if (a.b > 1) {
       by_channel[(int64_t)s * a.c + ch] = make_float2(u, v);
