@@ -23,3 +23,39 @@ def test_an_empty_sample_without_eps_leaves_the_parameters_gradients(n):
     leaf = w.clone().requires_grad_()
     y = F.group_norm(x, ints([0, 0]), 3, leaf, b, eps=0.0)      # nothing but an empty sample
     assert bool((y == 0).all()) and bool((torch.autograd.grad(y.sum(), leaf)[0] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("c,groups", [(16, 4), (24, 12), (96, 8), (64, 64), (99, 9), (98, 7), (256, 32), (2056, 257), (2057, 11)])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_group_norm_of_long_interleaved_samples(dtype, c, groups, ragged):
+    """The kernels that walk chunks of rows, through an order: groups inside a vector, across vectors and across tiles of
+    columns, single 16-bit values, rows before the first sample and behind the last."""
+    n = -(-(9 << 20) // (c * torch.finfo(dtype).bits // 8))      # one block serves a sample and group up to 8 MB in all
+    cuts = [7, n // 3, n // 3 + 1, n // 3 + 1, n - 11] if ragged else [0, n]
+    order = torch.randperm(n, generator=torch.Generator(device="cuda").manual_seed(n + c), device="cuda").int()
+    w, b = affine(c)
+    y, got = check_norm(features(n, c, dtype), cuts, groups, w, b, "silu", order=order)
+    outside = torch.cat([order[:cuts[0]], order[cuts[-1]:]]).long()
+    assert bool((y[outside] == 0).all()) and bool((got["dx"][outside] == 0).all())
+
+
+def test_group_norm_through_the_layer_on_long_interleaved_scans():
+    import torchsparse_b200 as ts
+    from torchsparse_b200 import nn as spnn
+
+    n, c = 60_011, 96
+    g = torch.Generator(device="cuda").manual_seed(2)
+    coords = torch.randint(0, 50, (n, 4), generator=g, device="cuda").int()
+    coords[:, 0] = torch.randint(0, 3, (n,), generator=g, device="cuda")
+    m = spnn.GroupNorm(8, c, activation="silu").cuda()
+    for dtype in TYPES:
+        x = features(n, c, dtype)
+        y = m(ts.SparseTensor(x, coords)).feats.detach()
+        for s in range(3):
+            rows = coords[:, 0] == s
+            z = torch.nn.functional.group_norm(x[rows].double().t()[None], 8, m.weight.double(), m.bias.double(), m.eps)[0].t()
+            want = torch.nn.functional.silu(z).detach()
+            # 32 roundings of the statistics and the affine step, magnified by |x| / sigma, below 8 here; silu' is below 1.1
+            bound = torch.finfo(dtype).eps / 2 * want.abs() + 1.1 * 32 * U * (8 + want.abs()) + 2.0 ** -25
+            assert bool(((y[rows].double() - want).abs() <= bound).all())
