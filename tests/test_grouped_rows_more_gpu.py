@@ -25,6 +25,24 @@ def test_an_empty_sample_without_eps_leaves_the_parameters_gradients(n):
     assert bool((y == 0).all()) and bool((torch.autograd.grad(y.sum(), leaf)[0] == 0).all())
 
 
+def test_a_group_of_one_value_is_refused_by_the_layer_wherever_it_runs():
+    """As torch's layer does; F.group_norm, and the layer with rows that the caller grouped, give act(bias)."""
+    import torchsparse_b200 as ts
+    from torchsparse_b200 import nn as spnn
+    from torchsparse_b200.nn import functional as F
+
+    coords = torch.tensor([[0, 1, 1, 1], [0, 2, 1, 1], [1, 3, 1, 1]], dtype=torch.int32)
+    x = torch.randn(3, 8, generator=torch.Generator().manual_seed(0))
+    for device in ("cpu", "cuda"):
+        m, s = spnn.GroupNorm(8, 8).to(device), ts.SparseTensor(x.to(device), coords.to(device))
+        with pytest.raises(ValueError, match="more than 1 value"):
+            m(s)
+        m(ts.SparseTensor(s.feats[:2], s.coords[:2]))                     # two rows in each group
+        spnn.GroupNorm(4, 8).to(device)(s)                                # two channels in each group
+    y = m(s, F.sample_rows(s))
+    assert torch.equal(y.feats[2], m.bias)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("c,groups", [(16, 4), (24, 12), (96, 8), (64, 64), (99, 9), (98, 7), (256, 32), (2056, 257), (2057, 11)])
 @pytest.mark.parametrize("ragged", [False, True])

@@ -31,6 +31,7 @@ class GroupNorm(nn.GroupNorm):
 
     ``activation`` ("relu", "leaky_relu", "silu") is applied in the same kernel.  ``forward`` takes the rows grouped by
     sample (``F.sample_rows``) when the caller has them; else it groups them and reads the batch size from the device.
+    As in ``nn.GroupNorm`` a group of one value is then a ValueError; with ``rows`` it becomes ``act(bias)``.
     fp32, fp16 and bf16 features on a GPU run on the library's kernels, with parameters of the same or another of these
     dtypes; other features run through torch, sample by sample."""
 
@@ -50,6 +51,8 @@ class GroupNorm(nn.GroupNorm):
         if feats.is_cuda and feats.dtype in _KERNEL_DTYPES:
             if rows is None:
                 rows = F.sample_rows(input)
+                if self.num_groups == self.num_channels and bool((rows.offsets.diff() == 1).any()):
+                    raise ValueError("Expected more than 1 value per channel: a sample of one row in groups of one channel")
             nfeats = F.group_norm(feats, rows.offsets, self.num_groups, self.weight, self.bias, self.eps, self.activation,
                                   self.negative_slope, rows.order)
         else:
