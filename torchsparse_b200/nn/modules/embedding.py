@@ -22,6 +22,16 @@ class Embedding(nn.Embedding):
         super().__init__(num_embeddings, embedding_dim, padding_idx, device=device, dtype=dtype)
         self.scale = float(scale)
 
+    @classmethod
+    def from_pretrained(cls, embeddings: torch.Tensor, freeze: bool = True, padding_idx: Optional[int] = None, *,
+                        scale: float = 1.0) -> "Embedding":
+        """A layer on the rows of ``embeddings`` [rows, C], which it shares; not trained where ``freeze`` is set."""
+        if embeddings.dim() != 2:
+            raise ValueError(f"from_pretrained expects a table [rows, channels], not {tuple(embeddings.shape)}")
+        layer = cls(*embeddings.shape, padding_idx, scale, device="meta", dtype=embeddings.dtype)
+        layer.weight = nn.Parameter(embeddings, requires_grad=not freeze)
+        return layer
+
     def forward(self, input: Union[SparseTensor, torch.Tensor]) -> Union[SparseTensor, torch.Tensor]:
         if isinstance(input, SparseTensor):
             return fapply(input, self._labels)
