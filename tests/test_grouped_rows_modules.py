@@ -16,3 +16,37 @@ def test_embedding_from_a_pretrained_table():
     for bad in (table[0], table[None]):
         with pytest.raises(ValueError):
             spnn.Embedding.from_pretrained(bad)
+
+
+def test_the_package_imports_without_the_torch_operators():
+    """A missing or unusable module is an error of the operators that it holds, and of nothing else."""
+    import subprocess
+    import sys
+    import textwrap
+
+    code = """
+        import os
+        import torch
+
+        found = os.path.exists
+        os.path.exists = lambda path: not str(path).endswith("_bindings.so") and found(path)
+        import torchsparse_b200 as ts
+        from torchsparse_b200 import _ops, nn as spnn
+        from torchsparse_b200.nn import functional as F
+
+        spnn.Conv3d(4, 4, 3)
+        y = spnn.GroupNorm(2, 4)(ts.SparseTensor(torch.randn(5, 4), torch.zeros(5, 4, dtype=torch.int32)))
+        assert y.feats.shape == (5, 4)
+        try:
+            F.embedding(torch.zeros(3, dtype=torch.int64), torch.zeros(2, 4))
+        except ImportError as e:
+            assert "_bindings.so is missing" in str(e)
+        else:
+            raise AssertionError("no error")
+        try:
+            _ops.nothing
+        except AttributeError:
+            print("as expected")
+    """
+    got = subprocess.run([sys.executable, "-c", textwrap.dedent(code)], capture_output=True, text=True, timeout=300)
+    assert got.returncode == 0 and "as expected" in got.stdout, got.stderr
