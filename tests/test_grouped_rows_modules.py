@@ -50,3 +50,15 @@ def test_the_package_imports_without_the_torch_operators():
     """
     got = subprocess.run([sys.executable, "-c", textwrap.dedent(code)], capture_output=True, text=True, timeout=300)
     assert got.returncode == 0 and "as expected" in got.stdout, got.stderr
+
+
+def test_one_block_per_sample_and_group_only_where_every_split_of_the_rows_suits_it():
+    """The kernels of one block need no workspace.  They are taken by what a batch can hold, not by its mean alone: a batch
+    of many nominal samples may have all its rows in one."""
+    from torchsparse_b200._lib import lib
+
+    small = lambda n, c, g, b, dtype: lib.tsb_group_norm_fwd_workspace_bytes(n, c, g, b, dtype) == 0      # noqa: E731
+    assert small(1217, 256, 32, 1, 1) and small(4000, 64, 8, 1, 1) and small(16384, 64, 8, 16, 1) and small(8000, 256, 32, 16, 1)
+    assert not small(16384, 64, 8, 64, 0)                  # 32768 vectors of a group: on 8 blocks if one sample has them
+    assert not small(130_000, 32, 8, 64, 1)
+    assert not small(16000, 64, 64, 16, 1)                 # groups of one 16-bit channel: 33 MB in reads of 32 bytes

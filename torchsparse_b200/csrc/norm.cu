@@ -1071,13 +1071,19 @@ int norm_vector(int dtype, int64_t c, int64_t g, uintptr_t bits) {
   return vec * (int)dtype_size(dtype) == 16 && d % part != 0 ? vec / 2 : vec;
 }
 
-// One block per sample and group where a sample of mean length fits the block's registers and the whole input is small.
-// Forward and backward on the device against the three launches each of the streaming kernels: 4000 rows of 64 channels
-// bf16 in one sample 10 + 17 us against 12 + 14, 60000 rows of 32 channels fp16 in 16 samples 8 + 13 against 18 + 21, and
-// two launches less for the host each way; one sample of 8085 rows 15 + 32 against 12 + 14.
+// One block per sample and group where a sample of mean length fits the block's registers, the whole input is small (a row of a
+// group counts as 32 bytes at least, what a read of it moves) and one sample that had nearly all rows would fit four times
+// the registers: the offsets are on the device, so the lengths are not known here.
+// Forward and backward on the device against the streaming kernels, which take two or three launches more each way; first
+// samples of equal lengths, then one of a third of the rows, then one of all among empty ones:
+//   8000 rows of 64 channels bf16, 4 samples, 8 groups    8 + 15 / 14 + 17     9 + 17 / 14 + 17   15 + 35 / 12 + 14 us
+//   16384 rows, 16 samples                                 8 + 13 / 11 + 14    12 + 27 / 15 + 18   37 + 65 / 11 + 14 us
+//   30000 rows, 16 samples                                 9 + 15 / 16 + 19    20 + 43 / 16 + 19   72 + 113 / 14 + 16 us
+//   60000 rows of 64 channels, 64 samples, 64 groups     120 + 167 / 29 + 33
 bool norm_small(int64_t n, int64_t c, int64_t g, int64_t b, int dtype) {
-  const int64_t d = c / g, dv = d / vector_width(dtype, d, 0);
-  return b <= 65535 && dv <= 64 && cdiv(n, b > 1 ? b : 1) * dv <= kSmallVectors && n * c * (int64_t)dtype_size(dtype) <= (8 << 20);
+  const int64_t d = c / g, dv = d / vector_width(dtype, d, 0), bytes = d * (int64_t)dtype_size(dtype);
+  return b <= 65535 && dv <= 64 && cdiv(n, b > 1 ? b : 1) * dv <= kSmallVectors && n * dv <= 4 * kSmallVectors &&
+         n * g * (bytes < 32 ? 32 : bytes) <= (8 << 20);
 }
 
 // threads of a block of the small kernels: two vectors each for a sample of mean length
