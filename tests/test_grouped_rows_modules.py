@@ -62,3 +62,13 @@ def test_one_block_per_sample_and_group_only_where_every_split_of_the_rows_suits
     assert not small(16384, 64, 8, 64, 0)                  # 32768 vectors of a group: on 8 blocks if one sample has them
     assert not small(130_000, 32, 8, 64, 1)
     assert not small(16000, 64, 64, 16, 1)                 # groups of one 16-bit channel: 33 MB in reads of 32 bytes
+
+
+def test_sizes_whose_flat_index_a_launch_cannot_hold_are_refused():
+    from torchsparse_b200._lib import lib
+
+    x, n, c = 256, (1 << 31) - 1, 1 << 20      # addresses are never read: every call is refused before a launch
+    for channels in (c, c - 1):
+        assert lib.tsb_embedding_fwd(x, x, 0, n, 3, channels, 1.0, 1, x, None) == 5
+        assert lib.tsb_expert_dispatch(x, x, x, n, 1, channels, 1, x, None) == 5
+    assert lib.tsb_embedding_fwd(x, x, 0, 5, 3, c + 1, 1.0, 1, x, None) == 5

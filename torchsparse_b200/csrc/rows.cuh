@@ -102,7 +102,9 @@ struct RowSplit {
   __device__ __forceinline__ int64_t row(int64_t t) const { return m ? (int64_t)__umul64hi((uint64_t)t, m) : t; }
 };
 inline RowSplit row_split(int64_t cols) { return RowSplit{cols == 1 ? 0 : ~0ull / (uint64_t)cols + 1, (unsigned)cols}; }
-constexpr int64_t kMaxChannels = 1 << 20;      // keeps index * cols of a row split below 2^64
+// A launch has fewer than 2^31 blocks, which the entries check, and a block at most 4096 vectors of the result: a flat index
+// is below 2^43 + 2^12, and with rows of at most 2^20 vectors index * cols stays below 2^64.
+constexpr int64_t kMaxChannels = 1 << 20;
 
 // One value of an array whose type is a run-time argument (parameters, router weights: few values, read once).
 __device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
