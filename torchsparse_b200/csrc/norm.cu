@@ -332,9 +332,10 @@ struct Running {
   }
 };
 
-// One read of x.  1M x 64 bf16: 33 us, 3.9 TB/s; 61441 x 96 bf16, which the L2 cache holds: 9 us.  What is left above
-// the copy rate (20 us) is the start of a block (its samples, the first rows) and the join at its end, some 5 us in all:
-// twice as many blocks of half the rows took 36 us, three times as many 41.
+// One read of x.  1M x 64 bf16: 33 us, 3.9 TB/s, where the copy rate takes 20; 61441 x 96 bf16, which the L2 cache holds: 9
+// us.  Some 5 us are the start of a block (its samples, the first rows) and the join at its end: twice as many blocks of
+// half the rows took 36 us, three times as many 41.  For the other 8 the counters name no one limit: memory is 52 % busy, 0.59
+// instructions issue per cycle, and a warp's first stall is the wait for its rows.
 template <typename T, int VEC, int A, bool ORDERED>
 __global__ void __launch_bounds__(kNormThreads, 3) norm_stats_kernel(Norm a, const T* __restrict__ x, float2* __restrict__ slots) {
   extern __shared__ __align__(16) unsigned char pipe[];
@@ -498,8 +499,9 @@ __device__ __forceinline__ void clear_outside(const Norm& a, int64_t p0, int64_t
   }
 }
 
-// The rows are walked from the end of the chunk to its beginning: what the statistics read last is still in the L2 cache.
-// 1M x 64 bf16 with SiLU: 42 us where reading and writing everything takes 39.
+// The rows are walked from the end of the chunk to its beginning: what the statistics read last is still in the L2 cache.  Of x
+// 33 MB of 77 are read from memory a second time (400003 x 96 fp16), 85 of 128 (1M x 64 bf16).  The latter with SiLU: 42
+// us, where 213 MB take 33 at the copy rate; shared loads and the special functions share a queue (MIO throttle).
 template <typename T, int VEC, int A, bool ORDERED>
 __global__ void __launch_bounds__(kNormThreads, 3) norm_apply_kernel(Norm a, const T* __restrict__ x, const float* __restrict__ mean,
                                                                      const float* __restrict__ rstd, T* __restrict__ y) {

@@ -15,7 +15,7 @@ def embedding(indices: torch.Tensor, table: torch.Tensor, scale: float = 1.0,
     and the shape of ``indices`` with C behind it.  An index that is no row of the table (a negative one, say) gives
     zeros and no gradient.  ``padding_idx`` names a row that gets no gradient (negative: counted from the end).
     The gradient is accumulated in fp32 in the order of the indices and rounded once: the same call gives the same
-    bits."""
+    bits.  It cannot be differentiated again."""
     if padding_idx is None:
         return _ops.embedding(table, indices, scale, -1)
     rows = table.shape[0]

@@ -33,5 +33,6 @@ def expert_dispatch(feats: torch.Tensor, rows: ExpertRows) -> torch.Tensor:
 def expert_combine(feats: torch.Tensor, weights: torch.Tensor, rows: ExpertRows) -> torch.Tensor:
     """[N, C]: row i is the sum over its choices of ``weights[i, j]`` times the sorted row of that choice (``feats``
     [N * k, C], what the experts made of the dispatched rows); a choice without an expert adds nothing.  Products and
-    sums are fp32.  ``weights`` fp32, fp16 or bf16 [N, k]."""
+    sums are fp32.  ``weights`` fp32, fp16 or bf16 [N, k].  The gradients of this and of ``expert_dispatch`` cannot be
+    differentiated again."""
     return _ops.expert_combine(feats, weights, rows.inverse, rows.offsets)

@@ -53,5 +53,6 @@ def group_norm(feats: torch.Tensor, offsets: torch.Tensor, num_groups: int, weig
     ``order`` int32 [N], a permutation, the rows ``order[offsets[s] : offsets[s + 1]]`` (see ``group_rows``).  A sample may be empty;
     rows of no sample become zero.  A group with one value becomes ``act(bias)``.  ``weight`` and ``bias`` [C] may have a
     dtype of their own (fp32 beside 16-bit features).  ``activation``: None, "relu", "leaky_relu" or "silu".
-    Statistics and sums are fp32 and run in a fixed order."""
+    Statistics and sums are fp32 and run in a fixed order.  Differentiable as often as wanted, in forward mode and under
+    ``torch.func`` too; beyond the plain gradient it is then composed of slower operations."""
     return _ops.group_norm(feats, weight, bias, offsets, order, num_groups, eps, activation_code(activation), negative_slope)
