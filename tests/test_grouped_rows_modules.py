@@ -72,3 +72,16 @@ def test_sizes_whose_flat_index_a_launch_cannot_hold_are_refused():
         assert lib.tsb_embedding_fwd(x, x, 0, n, 3, channels, 1.0, 1, x, None) == 5
         assert lib.tsb_expert_dispatch(x, x, x, n, 1, channels, 1, x, None) == 5
     assert lib.tsb_embedding_fwd(x, x, 0, 5, 3, c + 1, 1.0, 1, x, None) == 5
+
+
+def test_workspaces_of_wide_rows_go_by_the_blocks_that_run():
+    from torchsparse_b200._lib import lib
+
+    fwd, bwd = lib.tsb_group_norm_fwd_workspace_bytes, lib.tsb_group_norm_bwd_workspace_bytes
+    # at most 256 column tiles, 444 blocks over all of them and a slot more for each tile and sample
+    for n, c, g, b in ((10, 65536, 65536, 1), (300, 4096, 4096, 4), (300, 4096, 4096, 1000), (5000, 2048, 32, 4), (1_000_000, 64, 8, 8)):
+        for dtype in (0, 1, 2):
+            tiles = -(-c // 256)
+            assert fwd(n, c, g, b, dtype) <= (444 + 2 * tiles + tiles * b) * g * 8 + 3 * 256 + 2 * b * g * 4
+            assert bwd(n, c, g, b, dtype) <= (min(444, -(-n // 4)) + 2 * b) * c * 8 + b * g * 8 + 3 * 256
+    assert fwd(10, 65536, 65536, 1, 1) < 512 << 20

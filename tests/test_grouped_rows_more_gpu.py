@@ -58,6 +58,13 @@ def test_group_norm_of_long_interleaved_samples(dtype, c, groups, ragged):
     assert bool((y[outside] == 0).all()) and bool((got["dx"][outside] == 0).all())
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,c,groups", [(10, 65536, 65536), (300, 4096, 4096), (700, 8192, 2), (65, 65535, 5)])
+def test_group_norm_of_few_wide_rows(dtype, n, c, groups):
+    w, b = affine(c)
+    check_norm(features(n, c, dtype), [0, n // 2, n // 2, n], groups, w, b, "silu")
+
+
 def test_group_norm_through_the_layer_on_long_interleaved_scans():
     import torchsparse_b200 as ts
     from torchsparse_b200 import nn as spnn

@@ -1099,9 +1099,23 @@ int dispatch_small(int dtype, int vec, bool ordered, F&& f) {
   return dispatch_pack(dtype, vec, [&](auto tag) -> int { return ordered ? f(tag, std::true_type()) : f(tag, std::false_type()); });
 }
 
-// parts of the workspaces, for the vector width that needs the most column tiles
-size_t fwd_slot_bytes(int64_t n, int64_t c, int64_t g, int64_t b) {
-  return align_up((size_t)cdiv(c, kNormThreads) * (kNormBlocks + b) * g * sizeof(float2), 256);
+// Parts of the workspaces, for the vector width that needs the most: which one a call takes is up to its addresses.
+// f(shape) of every width that divides a row, the largest
+template <typename F>
+int64_t most_of_widths(int64_t n, int64_t c, int64_t g, int64_t b, int dtype, F&& f) {
+  int64_t most = 0;
+  for (int vec = 1; vec * (int)dtype_size(dtype) <= 16 && c % vec == 0; vec *= 2) {
+    const int64_t need = f(norm_shape(n, c, g, b, vec));
+    if (need > most) most = need;
+  }
+  return most;
+}
+size_t fwd_slot_bytes(int64_t n, int64_t c, int64_t g, int64_t b, int dtype) {
+  const int64_t slots = most_of_widths(n, c, g, b, dtype, [&](const Norm& a) { return cdiv(a.cols, a.tile) * (a.nblk + b); });
+  return align_up((size_t)slots * g * sizeof(float2), 256);
+}
+int64_t grad_slots(int64_t n, int64_t c, int64_t g, int64_t b, int dtype) {
+  return most_of_widths(n, c, g, b, dtype, [&](const Norm& a) { return a.nblk + b; });
 }
 size_t stat_bytes(int64_t g, int64_t b) { return align_up((size_t)b * g * sizeof(float), 256); }
 size_t channel_bytes(int64_t c, int64_t b) { return align_up((size_t)b * c * sizeof(float2), 256); }
@@ -1128,7 +1142,7 @@ extern "C" {
 
 size_t tsb_group_norm_fwd_workspace_bytes(int64_t n, int64_t c, int64_t g, int64_t b, int32_t dtype) {
   if (check_norm(n, c, g, 0, nullptr, dtype, 0, 0) != TSB_OK || b < 0 || norm_small(n, c, g, b, dtype)) return 0;
-  return fwd_slot_bytes(n, c, g, b) + 2 * stat_bytes(g, b);
+  return fwd_slot_bytes(n, c, g, b, dtype) + 2 * stat_bytes(g, b);
 }
 
 int tsb_group_norm_fwd(const void* x, const int32_t* order, const int32_t* offsets, const void* weight, const void* bias,
@@ -1153,14 +1167,14 @@ int tsb_group_norm_fwd(const void* x, const int32_t* order, const int32_t* offse
       return TSB_OK;
     });
   }
-  if (workspace_bytes < fwd_slot_bytes(n, c, g, b) + 2 * stat_bytes(g, b) || !workspace) return TSB_ERR_WORKSPACE;
+  if (workspace_bytes < fwd_slot_bytes(n, c, g, b, dtype) + 2 * stat_bytes(g, b) || !workspace) return TSB_ERR_WORKSPACE;
   const int vec = norm_vector(dtype, c, g, bits);
   const Norm a = norm_args(norm_shape(n, c, g, b, vec), order, offsets, weight, bias, param_dtype, eps, act, slope);
   char* ws = static_cast<char*>(workspace);
   float2* slots = reinterpret_cast<float2*>(ws);
   if (!mean) {
-    mean = reinterpret_cast<float*>(ws + fwd_slot_bytes(n, c, g, b));
-    rstd = reinterpret_cast<float*>(ws + fwd_slot_bytes(n, c, g, b) + stat_bytes(g, b));
+    mean = reinterpret_cast<float*>(ws + fwd_slot_bytes(n, c, g, b, dtype));
+    rstd = reinterpret_cast<float*>(ws + fwd_slot_bytes(n, c, g, b, dtype) + stat_bytes(g, b));
   }
   const int tiles = (int)cdiv(a.cols, a.tile);
   const dim3 grid((unsigned)a.nblk, (unsigned)tiles);
@@ -1189,7 +1203,7 @@ int tsb_group_norm_fwd(const void* x, const int32_t* order, const int32_t* offse
 size_t tsb_group_norm_bwd_workspace_bytes(int64_t n, int64_t c, int64_t g, int64_t b, int32_t dtype) {
   if (check_norm(n, c, g, 0, nullptr, dtype, 0, 0) != TSB_OK || b < 0) return 0;
   if (norm_small(n, c, g, b, dtype)) return b > 1 ? channel_bytes(c, b) : 0;
-  return channel_bytes(c, kNormBlocks + b) + channel_bytes(c, b) + channel_bytes(g, b);
+  return channel_bytes(c, grad_slots(n, c, g, b, dtype)) + channel_bytes(c, b) + channel_bytes(g, b);
 }
 
 int tsb_group_norm_bwd(const void* x, const void* dy, const int32_t* order, const int32_t* offsets, const void* weight,
@@ -1225,8 +1239,9 @@ int tsb_group_norm_bwd(const void* x, const void* dy, const int32_t* order, cons
   const int vec = norm_vector(dtype, c, g, bits);
   const Norm a = norm_args(norm_shape(n, c, g, b, vec), order, offsets, weight, bias, param_dtype, 0.f, act, slope);
   float2* slots = reinterpret_cast<float2*>(ws);
-  float2* by_channel = reinterpret_cast<float2*>(ws + channel_bytes(c, kNormBlocks + b));
-  float2* by_group = reinterpret_cast<float2*>(ws + channel_bytes(c, kNormBlocks + b) + channel_bytes(c, b));
+  const size_t slot_bytes = channel_bytes(c, grad_slots(n, c, g, b, dtype));
+  float2* by_channel = reinterpret_cast<float2*>(ws + slot_bytes);
+  float2* by_group = reinterpret_cast<float2*>(ws + slot_bytes + channel_bytes(c, b));
   const dim3 grid((unsigned)a.nblk, (unsigned)cdiv(a.cols, a.tile));
   const bool fold = (int64_t)a.nblk * 32 >= c;      // enough blocks for the parameters: no launch of their own
   return dispatch_norm(dtype, vec, a.d, order != nullptr, [&](auto tag, auto each, auto ordered) -> int {
